@@ -53,6 +53,10 @@ enum DeviceError : unsigned {
   kErrWaitAccFull = 0x104,   // epilogue gave up waiting for the accumulator
   kErrWaitAccEmpty = 0x105,  // MMA issuer gave up waiting for the epilogue
   kErrWaitDrain = 0x106,     // unwinding after an abort took too long
+  kErrBadSlot = 0x201,       // a cache slot past the last page: the row was not stored / read as zeros
+  kErrBadPosition = 0x202,   // a position outside the rotation tables: the token's rows are zeros
+  kErrBadPage = 0x203,       // a page index outside the cache: its keys were left out
+  kErrBadLength = 0x204,     // a length past the page table's row: cut to what the row can hold
 };
 
 __device__ unsigned int g_mxfp4_error;

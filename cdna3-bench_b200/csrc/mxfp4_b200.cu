@@ -16,6 +16,8 @@
 #include "gemm_small.cuh"
 #include "gemm_small_sk.cuh"
 #include "gemm_small_tc.cuh"
+#include "kv_rows.cuh"
+#include "paged_attention.cuh"
 #include "quant.cuh"
 
 namespace mxb {
@@ -663,6 +665,125 @@ int launch_gemv_mx(const uint8_t* ws, const uint8_t* wmx, void* C, int c_dtype, 
                     static_cast<__nv_bfloat16*>(C));
 }
 
+// ------------------------------------------------------------------ head rows, cache, attention
+bool valid_page_size(int n) { return n == 16 || n == 32 || n == 64 || n == 128 || n == 256; }
+
+// 0 or the error code; *v is the kernels' view of the cache.
+int cache_view(const mxfp4_kv_cache* c, KvCacheView* v, int* fmt) {
+  if (!c || !c->k_codes || !c->v_codes || !c->k_scales || !c->v_scales) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (c->num_pages <= 0 || c->num_kv_heads <= 0) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (c->format != MXFP4_KV_MXFP8 && c->format != MXFP4_KV_MXFP4) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return MXFP4_ERR_UNSUPPORTED_SHAPE;
+  if (!valid_page_size(c->page_size)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
+  if (static_cast<long long>(c->num_pages) * c->page_size >= (1ll << 31)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
+  if (!aligned16(c->k_codes) || !aligned16(c->v_codes) || !aligned16(c->k_scales) || !aligned16(c->v_scales))
+    return MXFP4_ERR_MISALIGNED;
+  int shift = 4;
+  while ((1 << shift) < c->page_size) ++shift;
+  *v = KvCacheView{c->k_codes, c->v_codes, c->k_scales, c->v_scales, c->num_pages, c->num_kv_heads, shift, c->head_dim};
+  *fmt = c->format == MXFP4_KV_MXFP8 ? kFmtE4M3 : kFmtE2M1;
+  return 0;
+}
+
+// Tokens per launch of a storing pass: every block looks through the slots behind its own.
+constexpr int kStoreTokens = 4096;
+
+template <int LPR, int kFmt>
+int launch_head_rows(const RowArgs& a, cudaStream_t s, const DeviceState* d) {
+  constexpr int rows = 32 / LPR;
+  const int groups = ceil_div(a.q_heads, rows) + ceil_div(a.kv_heads, rows) * (kFmt == kFmtNone ? 1 : 2);
+  const int most = kFmt == kFmtNone ? a.tokens : kStoreTokens;
+  for (int first = 0; first < a.tokens; first += most) {
+    const int n = std::min(most, a.tokens - first);
+    // few tokens: their rows are spread over blocks until the SMs have eight each
+    const int per_block = kRowThreads / 32;
+    const int y = std::max(1, std::min(ceil_div(groups, per_block), ceil_div(8 * d->sm_count, n)));
+    head_rows_kernel<LPR, kFmt><<<dim3(n, y), kRowThreads, 0, s>>>(a, first);
+    const int rc = launch_status();
+    if (rc) return rc;
+  }
+  return 0;
+}
+
+template <int kFmt>
+int launch_head_rows_dim(const RowArgs& a, cudaStream_t s) {
+  DeviceState* d = nullptr;
+  const int rc = current_device(&d);
+  if (rc) return rc;
+  if (a.dim <= 32) return launch_head_rows<4, kFmt>(a, s, d);
+  if (a.dim <= 64) return launch_head_rows<8, kFmt>(a, s, d);
+  if (a.dim <= 128) return launch_head_rows<16, kFmt>(a, s, d);
+  return launch_head_rows<32, kFmt>(a, s, d);
+}
+
+// Checks what the two norm-and-rotation entry points share and fills the arguments.
+int rope_args(RowArgs* a, const void* qkv, long long row_stride, int tokens, int q_heads, int kv_heads, int dim,
+              const float* cos, const float* sin, int table_rows, int rot, int interleaved, const int* positions,
+              const void* q_weight, const void* k_weight, int weight_dtype, double eps, void* q_out) {
+  if (tokens < 0 || q_heads <= 0 || kv_heads <= 0 || dim <= 0 || rot < 0) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (tokens > 0 && (!qkv || !q_out)) return MXFP4_ERR_INVALID_ARGUMENT;
+  if ((q_weight == nullptr) != (k_weight == nullptr) || !(eps >= 0.0)) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (weight_dtype != MXFP4_DTYPE_F32 && weight_dtype != MXFP4_DTYPE_BF16) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (dim % 32 || dim > 256 || rot % 16 || rot > dim) return MXFP4_ERR_UNSUPPORTED_SHAPE;
+  if (rot > 0 && (!cos || !sin || table_rows <= 0)) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (rot > 0 && !positions && table_rows < tokens) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (row_stride < (static_cast<long long>(q_heads) + 2ll * kv_heads) * dim) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (row_stride % 8 || !aligned16(qkv) || !aligned16(q_out) || !aligned16(cos) || !aligned16(sin) ||
+      !aligned16(q_weight) || !aligned16(k_weight))
+    return MXFP4_ERR_MISALIGNED;
+  const auto* x = static_cast<const __nv_bfloat16*>(qkv);
+  *a = RowArgs{};
+  a->q = x;
+  a->k = x + static_cast<size_t>(q_heads) * dim;
+  a->v = a->k + static_cast<size_t>(kv_heads) * dim;
+  a->q_stride = a->k_stride = a->v_stride = row_stride;
+  a->tokens = tokens, a->q_heads = q_heads, a->kv_heads = kv_heads, a->dim = dim;
+  a->cos = cos, a->sin = sin, a->table_rows = table_rows, a->rot = rot, a->interleaved = interleaved != 0;
+  a->positions = positions, a->q_weight = q_weight, a->k_weight = k_weight;
+  a->weight_f32 = weight_dtype == MXFP4_DTYPE_F32, a->eps = eps;
+  a->q_out = static_cast<__nv_bfloat16*>(q_out);
+  return 0;
+}
+
+// Blocks of the attention kernel: as many as are resident together.  kResident is the kernel's
+// launch bound, so this needs no query and holds without a device (148 SMs then).
+struct AttnPlan {
+  int nt, unit_keys, chunks, blocks;
+  size_t bytes;
+};
+AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int max_pages, int page_size, int sm_count) {
+  AttnPlan p;
+  const int group = q_heads / kv_heads;
+  p.nt = group > 8 && dim < 256 ? 2 : 1;  // two operand tiles of 8 heads fit the registers below D = 256
+  p.unit_keys = attn_unit_keys(dim, fmt, p.nt);
+  p.chunks = ceil_div(group, 8 * p.nt);
+  const long long keys = static_cast<long long>(max_pages) * page_size;
+  const long long units = (keys + p.unit_keys - 1) / p.unit_keys * seqs * kv_heads * p.chunks;
+  p.blocks = static_cast<int>(std::min<long long>(std::max<long long>(units, 1), 1ll * sm_count * attn_resident(dim, p.nt)));
+  p.bytes = static_cast<size_t>(p.blocks) * 2 * 8 * p.nt * (dim + 2) * sizeof(float);
+  return p;
+}
+
+template <int D, int kFmt, int NT>
+int launch_attention(const AttnArgs& a, int unit_keys, cudaStream_t s) {
+  constexpr int smem = kAttnWarps * 8 * NT * (D + 4 + 2) * static_cast<int>(sizeof(float));
+  static_assert(smem <= 48 * 1024, "");
+  attn_kernel<D, kFmt, NT><<<a.blocks, kAttnThreads, smem, s>>>(a);
+  int rc = launch_status();
+  if (rc) return rc;
+  const int heads = a.seqs * a.cache.heads * a.chunks;
+  return launch_pdl_grid(attn_join_kernel<D, NT>, dim3(heads), 128, 0, s, a, unit_keys);
+}
+
+template <int kFmt>
+int launch_attention_dim(const AttnArgs& a, const AttnPlan& p, cudaStream_t s) {
+  switch (a.cache.dim) {
+    case 64: return p.nt == 1 ? launch_attention<64, kFmt, 1>(a, p.unit_keys, s) : launch_attention<64, kFmt, 2>(a, p.unit_keys, s);
+    case 128: return p.nt == 1 ? launch_attention<128, kFmt, 1>(a, p.unit_keys, s) : launch_attention<128, kFmt, 2>(a, p.unit_keys, s);
+    default: return launch_attention<256, kFmt, 1>(a, p.unit_keys, s);
+  }
+}
+
 }  // namespace
 }  // namespace mxb
 
@@ -909,6 +1030,120 @@ int mxfp4_gemm_mx(const void* A, const uint8_t* w_mx, void* C, int c_dtype, int 
                                       : launch_mx<__nv_bfloat16, true>(ws, w_mx, C, M, N, K, s, d);
   return c_dtype == MXFP4_DTYPE_F32 ? launch_mx<float, false>(ws, w_mx, C, M, N, K, s, d)
                                     : launch_mx<__nv_bfloat16, false>(ws, w_mx, C, M, N, K, s, d);
+}
+
+int mxfp4_qk_norm_rope(const void* qkv, long long row_stride, int tokens, int num_heads, int num_kv_heads,
+                       int head_dim, const float* cos, const float* sin, int table_rows, int rot, int interleaved,
+                       const int* positions, const void* q_weight, const void* k_weight, int weight_dtype,
+                       double eps, void* q_out, void* k_out, void* stream) {
+  RowArgs a;
+  const int rc = rope_args(&a, qkv, row_stride, tokens, num_heads, num_kv_heads, head_dim, cos, sin, table_rows, rot,
+                           interleaved, positions, q_weight, k_weight, weight_dtype, eps, q_out);
+  if (rc) return rc;
+  if (tokens == 0) return 0;
+  if (!k_out) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (!aligned16(k_out)) return MXFP4_ERR_MISALIGNED;
+  a.k_out = static_cast<__nv_bfloat16*>(k_out);
+  return launch_head_rows_dim<kFmtNone>(a, static_cast<cudaStream_t>(stream));
+}
+
+int mxfp4_qk_norm_rope_cache(const void* qkv, long long row_stride, int tokens, int num_heads, const float* cos,
+                             const float* sin, int table_rows, int rot, int interleaved, const int* positions,
+                             const void* q_weight, const void* k_weight, int weight_dtype, double eps, void* q_out,
+                             const mxfp4_kv_cache* cache, const int* slots, void* stream) {
+  KvCacheView c;
+  int fmt = 0;
+  int rc = cache_view(cache, &c, &fmt);
+  if (rc) return rc;
+  RowArgs a;
+  rc = rope_args(&a, qkv, row_stride, tokens, num_heads, c.heads, c.dim, cos, sin, table_rows, rot, interleaved,
+                 positions, q_weight, k_weight, weight_dtype, eps, q_out);
+  if (rc) return rc;
+  if (tokens == 0) return 0;
+  if (!slots) return MXFP4_ERR_INVALID_ARGUMENT;
+  a.cache = c;
+  a.slots = slots;
+  auto s = static_cast<cudaStream_t>(stream);
+  return fmt == kFmtE4M3 ? launch_head_rows_dim<kFmtE4M3>(a, s) : launch_head_rows_dim<kFmtE2M1>(a, s);
+}
+
+int mxfp4_kv_cache_write(const mxfp4_kv_cache* cache, const void* k, long long k_stride, const void* v,
+                         long long v_stride, const int* slots, int tokens, void* stream) {
+  RowArgs a = {};
+  int fmt = 0;
+  const int rc = cache_view(cache, &a.cache, &fmt);
+  if (rc) return rc;
+  if (tokens < 0) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (tokens == 0) return 0;
+  if (!k || !v || !slots) return MXFP4_ERR_INVALID_ARGUMENT;
+  const long long width = static_cast<long long>(a.cache.heads) * a.cache.dim;
+  if (k_stride < width || v_stride < width) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (k_stride % 8 || v_stride % 8 || !aligned16(k) || !aligned16(v)) return MXFP4_ERR_MISALIGNED;
+  a.k = static_cast<const __nv_bfloat16*>(k), a.v = static_cast<const __nv_bfloat16*>(v);
+  a.k_stride = k_stride, a.v_stride = v_stride;
+  a.tokens = tokens, a.kv_heads = a.cache.heads, a.dim = a.cache.dim;
+  a.slots = slots;
+  auto s = static_cast<cudaStream_t>(stream);
+  return fmt == kFmtE4M3 ? launch_head_rows_dim<kFmtE4M3>(a, s) : launch_head_rows_dim<kFmtE2M1>(a, s);
+}
+
+int mxfp4_kv_cache_read(const mxfp4_kv_cache* cache, const int* slots, int tokens, void* k, void* v, void* stream) {
+  KvCacheView c;
+  int fmt = 0;
+  int rc = cache_view(cache, &c, &fmt);
+  if (rc) return rc;
+  if (tokens < 0) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (tokens == 0) return 0;
+  if (!slots || !k || !v) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (!aligned16(k) || !aligned16(v)) return MXFP4_ERR_MISALIGNED;
+  DeviceState* d = nullptr;
+  rc = current_device(&d);
+  if (rc) return rc;
+  auto s = static_cast<cudaStream_t>(stream);
+  const int blocks = ceil_div(tokens, kReadRows);
+  auto *ko = static_cast<__nv_bfloat16*>(k), *vo = static_cast<__nv_bfloat16*>(v);
+  if (fmt == kFmtE4M3) kv_read_kernel<kFmtE4M3><<<blocks, kReadThreads, 0, s>>>(c, slots, tokens, ko, vo);
+  else kv_read_kernel<kFmtE2M1><<<blocks, kReadThreads, 0, s>>>(c, slots, tokens, ko, vo);
+  return launch_status();
+}
+
+size_t mxfp4_paged_attention_workspace_bytes(const mxfp4_kv_cache* cache, int seqs, int num_heads, int max_pages) {
+  KvCacheView c;
+  int fmt = 0;
+  if (cache_view(cache, &c, &fmt) || seqs <= 0 || num_heads <= 0 || num_heads % c.heads || max_pages <= 0) return 0;
+  DeviceState* d = nullptr;
+  const int sms = current_device(&d) == 0 ? d->sm_count : 148;
+  return attn_plan(c.dim, fmt, c.heads, num_heads, seqs, max_pages, cache->page_size, sms).bytes;
+}
+
+int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cache* cache, const int* page_table,
+                          long long page_stride, int max_pages, const int* lengths, int seqs, int num_heads,
+                          float scale, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  AttnArgs a = {};
+  int fmt = 0;
+  int rc = cache_view(cache, &a.cache, &fmt);
+  if (rc) return rc;
+  if (seqs < 0 || num_heads <= 0 || max_pages <= 0 || page_stride < max_pages) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (num_heads % a.cache.heads || static_cast<long long>(max_pages) * cache->page_size >= (1ll << 31))
+    return MXFP4_ERR_UNSUPPORTED_SHAPE;
+  if (static_cast<long long>(seqs) * num_heads >= (1ll << 31)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
+  if (q_stride < static_cast<long long>(num_heads) * a.cache.dim) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (seqs == 0) return 0;
+  if (!q || !page_table || !lengths || !out) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (q_stride % 8 || !aligned16(q) || !aligned16(out) || !aligned16(workspace)) return MXFP4_ERR_MISALIGNED;
+  DeviceState* d = nullptr;
+  rc = current_device(&d);
+  if (rc) return rc;
+  const AttnPlan p = attn_plan(a.cache.dim, fmt, a.cache.heads, num_heads, seqs, max_pages, cache->page_size, d->sm_count);
+  if (!workspace || workspace_bytes < p.bytes) return MXFP4_ERR_WORKSPACE;
+  a.q = static_cast<const __nv_bfloat16*>(q), a.q_stride = q_stride;
+  a.table = page_table, a.table_stride = page_stride, a.max_pages = max_pages;
+  a.lengths = lengths, a.seqs = seqs, a.q_heads = num_heads, a.group = num_heads / a.cache.heads, a.chunks = p.chunks;
+  a.scale = scale;
+  a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
+  a.parts = static_cast<float*>(workspace), a.blocks = p.blocks;
+  auto s = static_cast<cudaStream_t>(stream);
+  return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p, s) : launch_attention_dim<kFmtE2M1>(a, p, s);
 }
 
 }  // extern "C"

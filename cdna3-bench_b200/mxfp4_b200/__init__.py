@@ -49,10 +49,25 @@ _OPS = (
     "gemm_mx",
 )
 
-__all__ = list(_OPS)
+# between the QKV GEMM and the output GEMM of an attention layer (mxfp4_b200.attention)
+_ATTENTION_OPS = (
+    "MXKVCache",
+    "new_kv_cache",
+    "qk_norm_rope",
+    "qk_norm_rope_cache",
+    "kv_cache_write",
+    "kv_cache_read",
+    "paged_attention",
+)
+
+__all__ = list(_OPS + _ATTENTION_OPS)
 
 
 def __getattr__(name):
+    if name in _ATTENTION_OPS:
+        from . import attention
+
+        return getattr(attention, name)
     if name in _OPS:
         from . import kernels
 

@@ -20,6 +20,7 @@ PATH_AUTO, PATH_TC, PATH_TC_SMEM, PATH_GEMV = 0, 1, 2, 3
 RULE_REF, RULE_OCP = 0, 1
 MX_Q8, MX_SPLIT2 = 0, 1
 MX_MODES = {"q8": MX_Q8, "split2": MX_SPLIT2}
+KV_MXFP8, KV_MXFP4 = 0, 1
 
 PATH_NAMES = {"auto": PATH_AUTO, "tc": PATH_TC, "tc_smem": PATH_TC_SMEM, "gemv": PATH_GEMV}
 
@@ -51,6 +52,12 @@ EXPORTED = (
     "mxfp4_mx_workspace_bytes",
     "mxfp4_quantize_act_mx8",
     "mxfp4_gemm_mx",
+    "mxfp4_qk_norm_rope",
+    "mxfp4_qk_norm_rope_cache",
+    "mxfp4_kv_cache_write",
+    "mxfp4_kv_cache_read",
+    "mxfp4_paged_attention_workspace_bytes",
+    "mxfp4_paged_attention",
 )
 
 
@@ -71,12 +78,29 @@ class DeviceInfo(ctypes.Structure):
     ]
 
 
+class KVCache(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int),
+        ("num_kv_heads", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("format", ctypes.c_int),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_LL = ctypes.c_longlong
+_F = ctypes.c_float
+_D = ctypes.c_double
 
 
 def _declare(lib):
@@ -107,6 +131,12 @@ def _declare(lib):
         "mxfp4_mx_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
         "mxfp4_quantize_act_mx8": (_I, [_P, _I, _I, _I, _P, _P]),
         "mxfp4_gemm_mx": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ, _P]),
+        "mxfp4_qk_norm_rope": (_I, [_P, _LL, _I, _I, _I, _I, _P, _P, _I, _I, _I, _P, _P, _P, _I, _D, _P, _P, _P]),
+        "mxfp4_qk_norm_rope_cache": (_I, [_P, _LL, _I, _I, _P, _P, _I, _I, _I, _P, _P, _P, _I, _D, _P, _P, _P, _P]),
+        "mxfp4_kv_cache_write": (_I, [_P, _P, _LL, _P, _LL, _P, _I, _P]),
+        "mxfp4_kv_cache_read": (_I, [_P, _P, _I, _P, _P, _P]),
+        "mxfp4_paged_attention_workspace_bytes": (_SZ, [_P, _I, _I, _I]),
+        "mxfp4_paged_attention": (_I, [_P, _LL, _P, _P, _LL, _I, _P, _I, _I, _F, _P, _P, _P, _SZ, _P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

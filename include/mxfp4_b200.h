@@ -227,6 +227,82 @@ int mxfp4_quantize_act_mx8(const void* A, int M, int K, int mode, uint8_t* dst, 
 int mxfp4_gemm_mx(const void* A, const uint8_t* w_mx, void* C, int c_dtype, int M, int N, int K, int mode,
                   void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Between the QKV GEMM and the output GEMM of an attention layer ------------------------
+ * (no counterpart in the reference, which stops at the GEMMs.)
+ *
+ * Index arrays (positions, slots, page tables, lengths) are int32 on the device.  An index out of
+ * range is found by the kernels, which leave the access out and set the device error word
+ * (mxfp4_device_error): 0x201 a slot past the last page (not stored; reads as zeros), 0x202 a
+ * position outside the tables (the token's outputs are zeros, nothing is stored), 0x203 a page
+ * outside the cache (its keys are left out), 0x204 a length past the page table's row (cut). */
+
+/* A paged key-value cache in an MX format.  Per page and kv head: page_size rows, in k_codes /
+ * v_codes of head_dim E4M3 codes (MXFP8) or head_dim / 2 bytes of E2M1 pairs (MXFP4, even element
+ * in the low nibble), and in k_scales / v_scales of head_dim / 32 E8M0 bytes:
+ *   codes  uint8 [num_pages][num_kv_heads][page_size][head_dim or head_dim / 2]
+ *   scales uint8 [num_pages][num_kv_heads][page_size][head_dim / 32]
+ * A group of 32 is coded by the OCP MX rule: e = floor(log2(amax)) - 8 (E4M3) or - 2 (E2M1), clipped
+ * to [-127, 127] (-127 for an all-zero group), elements * 2**-e rounded to nearest even and
+ * saturated at 448 / 6, scale byte e + 127.  A group holding a NaN gets the byte 255 and reads as
+ * NaN.  Slot s is row s % page_size of page s / page_size.  head_dim 64, 128 or 256; page_size 16,
+ * 32, 64, 128 or 256; num_pages * page_size < 2**31; all four arrays 16-byte aligned. */
+#define MXFP4_KV_MXFP8 0
+#define MXFP4_KV_MXFP4 1
+typedef struct mxfp4_kv_cache {
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  uint8_t* k_scales;
+  uint8_t* v_scales;
+  int num_pages, num_kv_heads, page_size, head_dim, format;
+} mxfp4_kv_cache;
+
+/* RMS norm of every query and key head and its rotation, in one pass over the QKV GEMM's output.
+ * qkv bf16 [tokens] rows of num_heads query, num_kv_heads key and num_kv_heads value heads of
+ * head_dim (a multiple of 32 up to 256), rows row_stride elements apart (a multiple of 8).
+ * q_weight / k_weight [head_dim] in weight_dtype, both or neither (NULL: no norm); y = x * weight /
+ * sqrt(mean(x*x) + eps).  The first rot values of a head (a multiple of 16, 0: no rotation) turn
+ * by cos / sin fp32 [table_rows][rot / 2], row positions[token] (NULL: the token's index):
+ * interleaved == 0 pairs value i with i + rot / 2, otherwise 2i with 2i + 1.
+ * q_out [tokens][num_heads][head_dim], k_out [tokens][num_kv_heads][head_dim], bf16; they must not
+ * overlap qkv. */
+int mxfp4_qk_norm_rope(const void* qkv, long long row_stride, int tokens, int num_heads, int num_kv_heads,
+                       int head_dim, const float* cos, const float* sin, int table_rows, int rot, int interleaved,
+                       const int* positions, const void* q_weight, const void* k_weight, int weight_dtype,
+                       double eps, void* q_out, void* k_out, void* stream);
+
+/* The same pass with the keys (normed, rotated, then coded without a rounding in between) and the
+ * values written into `cache` (its num_kv_heads and head_dim) at slots[token]; a negative slot
+ * stores nothing.  Of two tokens with the same slot the later one is stored.  The key path runs
+ * in 64 bits, so the stored bytes do not depend on how a sum was ordered. */
+int mxfp4_qk_norm_rope_cache(const void* qkv, long long row_stride, int tokens, int num_heads, const float* cos,
+                             const float* sin, int table_rows, int rot, int interleaved, const int* positions,
+                             const void* q_weight, const void* k_weight, int weight_dtype, double eps, void* q_out,
+                             const mxfp4_kv_cache* cache, const int* slots, void* stream);
+
+/* Writes k and v rows [tokens][num_kv_heads][head_dim] bf16 (rows k_stride / v_stride elements
+ * apart, multiples of 8) into the cache at slots[token], as above. */
+int mxfp4_kv_cache_write(const mxfp4_kv_cache* cache, const void* k, long long k_stride, const void* v,
+                         long long v_stride, const int* slots, int tokens, void* stream);
+
+/* Reads the rows that `slots` names back: k and v bf16 [tokens][num_kv_heads][head_dim]; a negative
+ * slot reads zeros. */
+int mxfp4_kv_cache_read(const mxfp4_kv_cache* cache, const int* slots, int tokens, void* k, void* v, void* stream);
+
+/* Attention of one new token per sequence: out[s][h] = softmax(scale * q[s][h] . k) v over the
+ * first lengths[s] keys of the sequence, key j being row j % page_size of page
+ * page_table[s][j / page_size] of kv head h / (num_heads / num_kv_heads); the keys and values are
+ * those mxfp4_kv_cache_read returns before its rounding to bf16 (value scales of 2**64 and more count as
+ * 2**63).  lse (NULL: not wanted) fp32 [seqs][num_heads] is the natural log of the sum of
+ * exp(scale * q . k).  A length of zero or less gives zeros and -inf.  Page-table entries past a
+ * sequence's last page are not read.
+ * q bf16 [seqs] rows of num_heads * head_dim, q_stride elements apart (a multiple of 8); out bf16
+ * [seqs][num_heads][head_dim]; page_table rows page_stride ints apart.  Results do not depend on
+ * timing: the same call gives the same bits. */
+size_t mxfp4_paged_attention_workspace_bytes(const mxfp4_kv_cache* cache, int seqs, int num_heads, int max_pages);
+int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cache* cache, const int* page_table,
+                          long long page_stride, int max_pages, const int* lengths, int seqs, int num_heads,
+                          float scale, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
