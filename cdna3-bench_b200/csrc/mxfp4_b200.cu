@@ -42,6 +42,7 @@ struct DeviceState {
   std::atomic<bool> sk_attr[4] = {false, false, false, false};
   std::atomic<bool> mx_attr[4] = {false, false, false, false};
   std::atomic<bool> gm_attr{false};
+  std::atomic<bool> attn_attr[12] = {};
 };
 
 constexpr int kMaxDevices = 64;
@@ -748,39 +749,42 @@ int rope_args(RowArgs* a, const void* qkv, long long row_stride, int tokens, int
 // Blocks of the attention kernel: as many as are resident together.  kResident is the kernel's
 // launch bound, so this needs no query and holds without a device (148 SMs then).
 struct AttnPlan {
-  int nt, unit_keys, chunks, blocks;
+  int nt, chunks, blocks;
   size_t bytes;
 };
-AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int max_pages, int page_size, int sm_count) {
+AttnPlan attn_plan(int dim, int kv_heads, int q_heads, int seqs, int max_pages, int page_size, int sm_count) {
   AttnPlan p;
   const int group = q_heads / kv_heads;
   p.nt = group > 8 && dim < 256 ? 2 : 1;  // two operand tiles of 8 heads fit the registers below D = 256
-  p.unit_keys = attn_unit_keys(dim, fmt, p.nt);
   p.chunks = ceil_div(group, 8 * p.nt);
   const long long keys = static_cast<long long>(max_pages) * page_size;
-  const long long units = (keys + p.unit_keys - 1) / p.unit_keys * seqs * kv_heads * p.chunks;
+  const long long units = (keys + kAttnUnitKeys - 1) / kAttnUnitKeys * seqs * kv_heads * p.chunks;
   p.blocks = static_cast<int>(std::min<long long>(std::max<long long>(units, 1), 1ll * sm_count * attn_resident(dim, p.nt)));
   p.bytes = static_cast<size_t>(p.blocks) * 2 * 8 * p.nt * (dim + 2) * sizeof(float);
   return p;
 }
 
 template <int D, int kFmt, int NT>
-int launch_attention(const AttnArgs& a, int unit_keys, cudaStream_t s) {
-  constexpr int smem = kAttnWarps * 8 * NT * (D + 4 + 2) * static_cast<int>(sizeof(float));
-  static_assert(smem <= 48 * 1024, "");
+int launch_attention(const AttnArgs& a, DeviceState* d, cudaStream_t s) {
+  constexpr int smem = attn_smem_bytes(D, kFmt, NT);
+  std::atomic<bool>& done = d->attn_attr[((D == 64 ? 0 : D == 128 ? 1 : 2) * 2 + (kFmt - 1)) * 2 + NT - 1];
+  if (!done.load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(attn_kernel<D, kFmt, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return ret(e);
+    done.store(true, std::memory_order_release);
+  }
   attn_kernel<D, kFmt, NT><<<a.blocks, kAttnThreads, smem, s>>>(a);
-  int rc = launch_status();
+  const int rc = launch_status();
   if (rc) return rc;
-  const int heads = a.seqs * a.cache.heads * a.chunks;
-  return launch_pdl_grid(attn_join_kernel<D, NT>, dim3(heads), 128, 0, s, a, unit_keys);
+  return launch_pdl_grid(attn_join_kernel<D, NT>, dim3(a.seqs * a.cache.heads * a.chunks, std::min(8 * NT, a.group)), kAttnThreads, 0, s, a);
 }
 
 template <int kFmt>
-int launch_attention_dim(const AttnArgs& a, const AttnPlan& p, cudaStream_t s) {
+int launch_attention_dim(const AttnArgs& a, int nt, DeviceState* d, cudaStream_t s) {
   switch (a.cache.dim) {
-    case 64: return p.nt == 1 ? launch_attention<64, kFmt, 1>(a, p.unit_keys, s) : launch_attention<64, kFmt, 2>(a, p.unit_keys, s);
-    case 128: return p.nt == 1 ? launch_attention<128, kFmt, 1>(a, p.unit_keys, s) : launch_attention<128, kFmt, 2>(a, p.unit_keys, s);
-    default: return launch_attention<256, kFmt, 1>(a, p.unit_keys, s);
+    case 64: return nt == 1 ? launch_attention<64, kFmt, 1>(a, d, s) : launch_attention<64, kFmt, 2>(a, d, s);
+    case 128: return nt == 1 ? launch_attention<128, kFmt, 1>(a, d, s) : launch_attention<128, kFmt, 2>(a, d, s);
+    default: return launch_attention<256, kFmt, 1>(a, d, s);
   }
 }
 
@@ -1113,7 +1117,7 @@ size_t mxfp4_paged_attention_workspace_bytes(const mxfp4_kv_cache* cache, int se
   if (cache_view(cache, &c, &fmt) || seqs <= 0 || num_heads <= 0 || num_heads % c.heads || max_pages <= 0) return 0;
   DeviceState* d = nullptr;
   const int sms = current_device(&d) == 0 ? d->sm_count : 148;
-  return attn_plan(c.dim, fmt, c.heads, num_heads, seqs, max_pages, cache->page_size, sms).bytes;
+  return attn_plan(c.dim, c.heads, num_heads, seqs, max_pages, cache->page_size, sms).bytes;
 }
 
 int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cache* cache, const int* page_table,
@@ -1134,7 +1138,7 @@ int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cach
   DeviceState* d = nullptr;
   rc = current_device(&d);
   if (rc) return rc;
-  const AttnPlan p = attn_plan(a.cache.dim, fmt, a.cache.heads, num_heads, seqs, max_pages, cache->page_size, d->sm_count);
+  const AttnPlan p = attn_plan(a.cache.dim, a.cache.heads, num_heads, seqs, max_pages, cache->page_size, d->sm_count);
   if (!workspace || workspace_bytes < p.bytes) return MXFP4_ERR_WORKSPACE;
   a.q = static_cast<const __nv_bfloat16*>(q), a.q_stride = q_stride;
   a.table = page_table, a.table_stride = page_stride, a.max_pages = max_pages;
@@ -1143,7 +1147,7 @@ int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cach
   a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
   a.parts = static_cast<float*>(workspace), a.blocks = p.blocks;
   auto s = static_cast<cudaStream_t>(stream);
-  return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p, s) : launch_attention_dim<kFmtE2M1>(a, p, s);
+  return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p.nt, d, s) : launch_attention_dim<kFmtE2M1>(a, p.nt, d, s);
 }
 
 }  // extern "C"

@@ -31,6 +31,8 @@
 // others go to the workspace and attn_join_kernel adds them in the blocks' order.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "gemm_small.cuh"
 #include "kv_rows.cuh"
@@ -39,18 +41,23 @@ namespace mxb {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
+constexpr int kAttnUnitKeys = 16 * kAttnWarps;  // one tile of 16 keys per warp
 
-// Tiles of 16 keys a warp takes per step: about 32 registers each of K and V codes in flight.
-__host__ __device__ constexpr int attn_tiles(int dim, int fmt, int nt) {
-  const int t = (fmt == kFmtE4M3 ? 256 : 512) / dim / nt;
-  return t < 1 ? 1 : (t > 4 ? 4 : t);
+// Blocks resident per SM (the kernel's launch bound) and tiles in a warp's ring.
+__host__ __device__ constexpr int attn_resident(int dim, int nt) {
+  return dim == 256 ? 2 : (nt == 2 ? 3 : (dim == 128 ? 4 : 5));
 }
-__host__ __device__ constexpr int attn_unit_keys(int dim, int fmt, int nt) {
-  return 16 * kAttnWarps * attn_tiles(dim, fmt, nt);
+__host__ __device__ constexpr int attn_ring(int dim, int fmt) { return fmt == kFmtE4M3 && dim >= 128 ? 3 : 4; }
+__host__ __device__ constexpr int attn_row_bytes(int dim, int fmt) { return fmt == kFmtE4M3 ? dim : dim / 2; }
+// K codes, V codes, K scales, V scales of 16 keys
+__host__ __device__ constexpr int attn_tile_bytes(int dim, int fmt) {
+  return 16 * 2 * (attn_row_bytes(dim, fmt) + dim / 32);
 }
-
-// Blocks resident per SM (the kernel's launch bound).
-__host__ __device__ constexpr int attn_resident(int dim, int nt) { return dim == 256 || nt == 2 ? 2 : 3; }
+__host__ __device__ constexpr int attn_smem_bytes(int dim, int fmt, int nt) {
+  const int ring = kAttnWarps * attn_ring(dim, fmt) * attn_tile_bytes(dim, fmt);
+  const int join = kAttnWarps * 8 * nt * (dim + 4 + 2) * 4;  // the warps' parts, after the ring
+  return ring > join ? ring : join;
+}
 
 struct AttnArgs {
   const __nv_bfloat16* q;  // [seqs][q_heads][dim], rows q_stride apart
@@ -156,69 +163,98 @@ __device__ __forceinline__ void attn_find(const AttnArgs& a, int unit_keys, long
   begin = base;
 }
 
+// Placement of the 16-byte units of key row r (0..15) of a tile in shared memory: unit u of the row
+// goes to u ^ attn_swizzle.  The rows a load instruction touches in one phase (K: rows pi(g), see
+// below; V: rows t + 4 i) then lie in different banks.
+template <int D, int kFmt, bool kV>
+__device__ __forceinline__ constexpr int attn_swizzle(int r) {
+  constexpr int kRowBytes = attn_row_bytes(D, kFmt);
+  if constexpr (kFmt == kFmtE4M3) {
+    if constexpr (kV) return kRowBytes == 64 ? r & 2 : (kRowBytes == 128 ? 2 * (r & 3) : (r & 1) | ((r & 2) << 1));
+    return kRowBytes == 64 ? (r >> 1) & 2 : ((r >> 1) & 2) | ((r & 1) << 2);
+  } else {
+    if constexpr (kV) return kRowBytes == 32 ? 0 : (kRowBytes == 64 ? r & 2 : 2 * (r & 3));
+    return kRowBytes == 32 ? (r >> 2) & 1 : (kRowBytes == 64 ? (r >> 1) & 3 : r & 7);
+  }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Copies the 16 keys of a tile into shared memory at dst (one warp): codes from k and v, scales
+// from sc, each with the lane's own offset already in it.  base_k and base_v: the lane's first
+// place in the tile; a later one differs by whole rows and, as the swizzle is linear over xor in
+// the row's bits, by an xor with a constant.
+template <int D, int kFmt, bool kV>
+__device__ __forceinline__ uint32_t attn_copy_base() {
+  constexpr int kRowBytes = attn_row_bytes(D, kFmt), kUnits = kRowBytes / 16;
+  const int lane = threadIdx.x & 31, r = lane / kUnits, u = lane % kUnits;
+  return r * kRowBytes + 16 * (u ^ attn_swizzle<D, kFmt, kV>(r));
+}
 template <int D, int kFmt>
-struct AttnTile {
-  static constexpr int kGroups = D / 32;
-  static constexpr int kKWords = kFmt == kFmtE4M3 ? D / 8 : D / 16;  // words of K codes a lane holds, 2 keys
-  static constexpr int kVWords = kFmt == kFmtE4M3 ? D / 8 : D / 16;  // words of V codes a lane holds, 4 keys
-  uint32_t k[kKWords];        // [key g / g+8][group][words]
-  uint32_t ks[2][(kGroups + 3) / 4];
-  uint32_t v[kVWords];        // [key 2t, 2t+1, 2t+8, 2t+9][words]
-  uint32_t vs[4];
-};
+__device__ __forceinline__ void attn_copy_tile(const uint8_t* k, const uint8_t* v, const uint8_t* sc, uint32_t dst,
+                                               uint32_t base_k, uint32_t base_v) {
+  constexpr int kRowBytes = attn_row_bytes(D, kFmt), kUnits = kRowBytes / 16, kRows = 32 / kUnits;
+#pragma unroll
+  for (int j = 0; j < kUnits / 2; ++j) {
+    cp_async16(dst + (base_k ^ (16 * attn_swizzle<D, kFmt, false>(kRows * j))) + 512 * j, k + 512 * j);
+    cp_async16(dst + (base_v ^ (16 * attn_swizzle<D, kFmt, true>(kRows * j))) + 512 * j + 16 * kRowBytes, v + 512 * j);
+  }
+  const int lane = threadIdx.x & 31;
+  if (lane < D / 16) cp_async16(dst + 32 * kRowBytes + 16 * lane, sc);
+}
 
 template <int kWords>
-__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t* w) {
   if constexpr (kWords % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < kWords; i += 4) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + 4 * i));
-      w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
-    }
+    const uint4 u = lds128(a);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
   } else if constexpr (kWords == 2) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-    w[0] = u.x, w[1] = u.y;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
   } else {
-    static_assert(kWords == 1, "");
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    w[0] = lds32(a);
   }
 }
 
-// K codes and scales of the 16 keys whose first cache row is `row`.
-template <int D, int kFmt>
-__device__ __forceinline__ void load_k(const KvCacheView& c, size_t row, AttnTile<D, kFmt>& x) {
-  using T = AttnTile<D, kFmt>;
-  constexpr int kRowBytes = kFmt == kFmtE4M3 ? D : D / 2, kGroupBytes = kRowBytes / T::kGroups;
-  constexpr int kW = kGroupBytes / 16;  // words per lane and group: 2 (E4M3) or 1
-  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const size_t r = row + g + 8 * h;
-#pragma unroll
-    for (int b = 0; b < T::kGroups; ++b)
-      load_words<kW>(c.k_codes + r * kRowBytes + b * kGroupBytes + 4 * kW * t, x.k + (h * T::kGroups + b) * kW);
-    const uint8_t* s = c.k_scales + r * T::kGroups;
-    if constexpr (T::kGroups == 2) x.ks[h][0] = __ldg(reinterpret_cast<const uint16_t*>(s));
-    else load_words<T::kGroups / 4>(s, x.ks[h]);
-  }
+// Four E4M3 codes as f16x2 words, exact.
+__device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
-
-template <int D, int kFmt>
-__device__ __forceinline__ void load_v(const KvCacheView& c, size_t row, AttnTile<D, kFmt>& x) {
-  using T = AttnTile<D, kFmt>;
-  constexpr int kRowBytes = kFmt == kFmtE4M3 ? D : D / 2, kW = kRowBytes / 32;  // words per lane and key
-  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const size_t r = row + 2 * t + (j & 1) + 8 * (j >> 1);
-    load_words<kW>(c.v_codes + r * kRowBytes + 4 * kW * g, x.v + j * kW);
-    x.vs[j] = __ldg(c.v_scales + r * T::kGroups + (g * D / 8) / 32);
-  }
+// Two E8M0 bytes as bf16x2: 2^(b - 127), 255 is NaN.
+__device__ __forceinline__ uint32_t e8m0x2_bf16x2(uint32_t b) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(b)));
+  return r;
 }
+// Four of them (the low two, the high two).
+__device__ __forceinline__ void e8m0x4_bf16x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.bf16x2.ue8m0x2 %0, l;\n\t"
+      "cvt.rn.bf16x2.ue8m0x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+__device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xFFFF0000u); }
 
-// bf16x2 multiplier of two keys' scale bytes (see kCarry at the top): 2^(b - 63), 255 is NaN.
-__device__ __forceinline__ uint32_t v_factor(uint32_t b) {
-  return b == 255u ? 0x7FC0u : (min(b + 64u, 254u) << 7);
+// bf16x2 multiplier of two keys' scale bytes (see kCarry at the top): 2^(b - 63), at most 2^127
+// (0x7F00), NaN for 255.
+__device__ __forceinline__ uint32_t v_factor(uint32_t b0, uint32_t b1) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(mul_bf16x2(e8m0x2_bf16x2(prmt(b0, b1, 0x0040)), 0x5F805F80u)), "r"(0x7F007F00u));
+  return r;
 }
 
 // V operand words of one pair of keys: for each of the lane's D / 8 values, (key a, key b) as
@@ -247,35 +283,39 @@ __device__ __forceinline__ void v_pairs(const uint32_t* a, const uint32_t* b, ui
 
 template <int D, int kFmt, int NT>
 __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kernel(const __grid_constant__ AttnArgs a) {
-  using T = AttnTile<D, kFmt>;
-  constexpr int KT = attn_tiles(D, kFmt, NT);
-  constexpr int kUnitTiles = kAttnWarps * KT, kUnitKeys = 16 * kUnitTiles;
-  constexpr int kGroups = D / 32, kHeads = 8 * NT;
+  constexpr int kGroups = D / 32, kHeads = 8 * NT, kRing = attn_ring(D, kFmt);
+  constexpr int kRowBytes = attn_row_bytes(D, kFmt), kTile = attn_tile_bytes(D, kFmt);
+  constexpr int kKw = kRowBytes / kGroups / 16;  // words of K codes per lane, key and group: 2 or 1
+  constexpr int kVw = kRowBytes / 32;            // words of V codes per lane and key
   constexpr float kCarry = kFmt == kFmtE4M3 ? 56.0f : 62.0f;  // p carries 2^kCarry, v 2^-kCarry
+  constexpr float kRise = 8.0f;                               // see below
   constexpr int kStride = D + 4;                              // floats per head of a warp's part in shared memory
   constexpr float kInf = __builtin_huge_valf();
-  extern __shared__ float sm[];                               // [warps][kHeads][kStride], then m, l [warps][kHeads]
-  float* sm_m = sm + kAttnWarps * kHeads * kStride;
+  extern __shared__ __align__(128) float sm[];                // the warps' rings; then [warps][kHeads][kStride]
+  float* sm_m = sm + kAttnWarps * kHeads * kStride;           // and m, l [warps][kHeads]
   float* sm_l = sm_m + kAttnWarps * kHeads;
   __shared__ long long red[2 * kAttnWarps];
 
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int key_g = (g >> 1) + 4 * (g & 1);  // pi(g): the key of operand row g (and key_g + 8 of row g + 8)
+  const uint32_t ring = smem_u32(sm) + warp * kRing * kTile;
+  const uint32_t base_k = attn_copy_base<D, kFmt, false>(), base_v = attn_copy_base<D, kFmt, true>();
 
   long long total, none;
-  attn_count_units(a, kUnitKeys, 0, total, none, red);
+  attn_count_units(a, kAttnUnitKeys, 0, total, none, red);
   const long long share = attn_share(total, a.blocks);
   long long u = share * blockIdx.x;
   const long long u_end = min(u + share, total);
   if (u >= u_end) return;
   int seq;
   long long begin;
-  attn_find(a, kUnitKeys, u, seq, begin);
+  attn_find(a, kAttnUnitKeys, u, seq, begin);
 
   while (u < u_end) {
     // the segment: units [first, last) of head (seq, head, chunk)
     const int len = attn_length(a, seq);
-    const int units = (len + kUnitKeys - 1) / kUnitKeys;
+    const int units = (len + kAttnUnitKeys - 1) / kAttnUnitKeys;
     if (units == 0) {
       ++seq;
       continue;
@@ -287,20 +327,39 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kerne
     const int h0 = head * a.group + chunk * kHeads;                  // first q head
     const int nh = min(kHeads, a.group - chunk * kHeads);            // q heads here
     const int* table = a.table + a.table_stride * seq;
-    const int tiles = (len + 15) >> 4;
-
-    // the cache row of a tile's first key, or -1 if there is none
     const int tile_shift = a.cache.page_shift - 4;
-    auto tile_row = [&](int tile) -> long long {
-      if (tile >= tiles) return -1;
-      const int page = __ldg(table + (tile >> tile_shift));
-      if (page < 0 || page >= a.cache.num_pages) {
-        record_error(kErrBadPage);
-        return -1;
+    const int tile_last = min(last * kAttnWarps, (len + 15) >> 4);
+
+    // Copies into the ring, one commit group per tile; the page of the tile after is on its way.
+    // `good` has a bit for each of the last copies: whether its page is one of the cache's.
+    uint32_t good = 0;
+    int copy_tile = first * kAttnWarps + warp, copy_slot = 0;
+    int page = copy_tile < tile_last ? __ldg(table + (copy_tile >> tile_shift)) : 0;
+    const uint32_t page_rows = static_cast<uint32_t>(a.cache.heads) << a.cache.page_shift;
+    const size_t head_rows = static_cast<size_t>(head) << a.cache.page_shift;
+    const uint8_t* k_lane = a.cache.k_codes + head_rows * kRowBytes + 16 * lane;
+    const uint8_t* v_lane = a.cache.v_codes + head_rows * kRowBytes + 16 * lane;
+    const uint8_t* s_lane = (lane < kGroups ? a.cache.k_scales + 16 * lane : a.cache.v_scales + 16 * (lane - kGroups)) +
+                            head_rows * kGroups;
+    auto copy_next = [&]() {
+      good <<= 1;
+      if (copy_tile < tile_last) {
+        if (page >= 0 && page < a.cache.num_pages) {
+          const size_t row = static_cast<size_t>(page) * page_rows + ((copy_tile & ((1 << tile_shift) - 1)) << 4);
+          attn_copy_tile<D, kFmt>(k_lane + row * kRowBytes, v_lane + row * kRowBytes, s_lane + row * kGroups,
+                                  ring + copy_slot * kTile, base_k, base_v);
+          good |= 1;
+        } else {
+          record_error(kErrBadPage);
+        }
+        copy_tile += kAttnWarps;
+        if (copy_tile < tile_last) page = __ldg(table + (copy_tile >> tile_shift));
       }
-      return (((static_cast<long long>(page) * a.cache.heads + head) << a.cache.page_shift) +
-              ((tile & ((1 << tile_shift) - 1)) << 4));
+      copy_slot = copy_slot + 1 == kRing ? 0 : copy_slot + 1;
+      cp_async_commit();
     };
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) copy_next();
 
     // Q operand: head g of n-tile n, values 32 b + 8 t .. + 7, scaled into f16
     uint32_t q[NT][kGroups][4];
@@ -327,8 +386,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kerne
       for (int b = 0; b < kGroups; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const __half2 h = __floats2half2_rn(__uint_as_float(q[n][b][i] << 16) * two,
-                                              __uint_as_float(q[n][b][i] & 0xFFFF0000u) * two);
+          const __half2 h = __floats2half2_rn(bf16_lo(q[n][b][i]) * two, bf16_hi(q[n][b][i]) * two);
           q[n][b][i] = *reinterpret_cast<const uint32_t*>(&h);
         }
       const float back = a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
@@ -337,7 +395,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kerne
     }
 
     float acc[D / 16][NT][4];
-    float m[NT][2], lsum[NT][2];
+    float m[NT][2], sub[NT][2], lsum[NT][2];  // reference maximum, what p's exponent subtracts, sum of p
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -345,140 +403,148 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kerne
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
       m[n][0] = m[n][1] = -kInf;
+      sub[n][0] = sub[n][1] = -kCarry;
       lsum[n][0] = lsum[n][1] = 0.0f;
     }
 
-    T x[KT];
-    bool some[KT];
-    const int tile_first = first * kUnitTiles + warp * KT, tile_last = min(last * kUnitTiles, tiles);
-    long long row[KT];
-#pragma unroll
-    for (int i = 0; i < KT; ++i) {
-      row[i] = tile_row(tile_first + i);
-      some[i] = row[i] >= 0;
-      if (some[i]) {
-        load_k<D, kFmt>(a.cache, row[i], x[i]);
-        load_v<D, kFmt>(a.cache, row[i], x[i]);
-      }
-    }
-    for (int tile = tile_first; tile < tile_last; tile += kUnitTiles) {
-      const int next = tile + kUnitTiles;
-      bool more[KT];
-#pragma unroll
-      for (int i = 0; i < KT; ++i) {
-        row[i] = next < tile_last ? tile_row(next + i) : -1;
-        more[i] = row[i] >= 0;
-      }
-      // scores
-      float s[KT][NT][4];
-#pragma unroll
-      for (int i = 0; i < KT; ++i) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.0f;
-#pragma unroll
-        for (int b = 0; b < kGroups; ++b) {
-          uint32_t f[2][4];  // [key g / g+8][value pairs 8t + 2j]
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if constexpr (kFmt == kFmtE4M3) {
-              const uint32_t w0 = x[i].k[(h * kGroups + b) * 2], w1 = x[i].k[(h * kGroups + b) * 2 + 1];
-              const uint32_t p[4] = {w0 & 0xFFFFu, w0 >> 16, w1 & 0xFFFFu, w1 >> 16};
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f[h][j]) : "h"(static_cast<uint16_t>(p[j])));
-            } else {
-              e2m1x8_to_f16x2(x[i].k[h * kGroups + b], f[h]);
-            }
-          }
-          const float s0 = e8m0_value((x[i].ks[0][b / 4] >> (8 * (b & 3))) & 255u);
-          const float s1 = e8m0_value((x[i].ks[1][b / 4] >> (8 * (b & 3))) & 255u);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma_f16_16816(d, f[0][0], f[1][0], f[0][1], f[1][1], q[n][b][0], q[n][b][1]);
-            mma_f16_16816(d, f[0][2], f[1][2], f[0][3], f[1][3], q[n][b][2], q[n][b][3]);
-            s[i][n][0] = fmaf(d[0], s0, s[i][n][0]);
-            s[i][n][1] = fmaf(d[1], s0, s[i][n][1]);
-            s[i][n][2] = fmaf(d[2], s1, s[i][n][2]);
-            s[i][n][3] = fmaf(d[3], s1, s[i][n][3]);
-          }
-        }
-      }
-      // K registers are free: the next step's keys
-#pragma unroll
-      for (int i = 0; i < KT; ++i)
-        if (more[i]) load_k<D, kFmt>(a.cache, row[i], x[i]);
+    int slot = 0;
+    // One tile; `ragged`: the sequence ends inside it.
+    auto do_tile = [&](int tile, auto ragged) {
+      cp_async_wait<kRing - 2>();
+      __syncwarp();  // every lane's copies have landed, and all lanes have left the slot copied into next
+      copy_next();
+      const uint32_t at = ring + slot * kTile;
+      slot = slot + 1 == kRing ? 0 : slot + 1;
+      if (!((good >> (kRing - 1)) & 1)) return;
 
-      // masked scores, running maximum, p = 2^(s - m + kCarry)
-      uint32_t p[KT][NT][2];
+      // scores
+      float s[NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float top[2] = {m[n][0], m[n][1]};
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+      uint32_t two[2][kGroups / 2];  // the two keys' scales, a bf16x2 per pair of groups
 #pragma unroll
-        for (int i = 0; i < KT; ++i) {
-          const int key = (tile + i) * 16 + g;
-          const bool in0 = some[i] && key < len, in1 = some[i] && key + 8 < len;
-          s[i][n][0] = in0 ? s[i][n][0] * mult[n][0] : -kInf;
-          s[i][n][1] = in0 ? s[i][n][1] * mult[n][1] : -kInf;
-          s[i][n][2] = in1 ? s[i][n][2] * mult[n][0] : -kInf;
-          s[i][n][3] = in1 ? s[i][n][3] * mult[n][1] : -kInf;
-          top[0] = fmaxf(top[0], fmaxf(s[i][n][0], s[i][n][2]));
-          top[1] = fmaxf(top[1], fmaxf(s[i][n][1], s[i][n][3]));
-        }
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t sa = at + 32 * kRowBytes + (key_g + 8 * h) * kGroups;
+        uint32_t w[(kGroups + 3) / 4];
+        if constexpr (kGroups == 2) {
+          asm volatile("ld.shared.u16 %0, [%1];" : "=r"(w[0]) : "r"(sa));
+          two[h][0] = e8m0x2_bf16x2(w[0]);
+        } else {
+          lds_words<kGroups / 4>(sa, w);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 4));
-          top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 8));
-          top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 16));
-          const float base = top[j] == -kInf ? 0.0f : top[j];  // nothing seen yet
-          const float fade = exp2_approx(m[n][j] - base);
-          m[n][j] = top[j];
-          lsum[n][j] *= fade;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) acc[i][n][j] *= fade, acc[i][n][j + 2] *= fade;
-          top[j] = base - kCarry;
-        }
-#pragma unroll
-        for (int i = 0; i < KT; ++i) {
-          const float p0 = exp2_approx(s[i][n][0] - top[0]), p1 = exp2_approx(s[i][n][1] - top[1]);
-          const float p2 = exp2_approx(s[i][n][2] - top[0]), p3 = exp2_approx(s[i][n][3] - top[1]);
-          lsum[n][0] += p0 + p2;
-          lsum[n][1] += p1 + p3;
-          // p is rounded to bf16 for the product (relative 2^-9 each, of either sign); the sum is not
-          p[i][n][0] = transpose8x8(pack_bf16x2(p0, p1));
-          p[i][n][1] = transpose8x8(pack_bf16x2(p2, p3));
+          for (int b = 0; b < kGroups; b += 4) e8m0x4_bf16x2(w[b / 4], two[h][b / 2], two[h][b / 2 + 1]);
         }
       }
-      // output
 #pragma unroll
-      for (int i = 0; i < KT; ++i) {
-        if (!some[i]) continue;
-        constexpr int kW = T::kVWords / 4;
-        const int key = (tile + i) * 16;
-        if (key + 16 > len) {  // rows behind the sequence may hold anything
+      for (int b = 0; b < kGroups; ++b) {
+        uint32_t f[2][4];  // [key][value pairs 8t + 2j]
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = key_g + 8 * h;
+          const int byte = b * (kRowBytes / kGroups) + 4 * kKw * t;
+          uint32_t w[kKw];
+          lds_words<kKw>(at + key * kRowBytes + (byte ^ (16 * attn_swizzle<D, kFmt, false>(key))), w);
+          if constexpr (kFmt == kFmtE4M3) {
+            e4m3x4_to_f16x2(w[0], f[h][0], f[h][1]);
+            e4m3x4_to_f16x2(w[1], f[h][2], f[h][3]);
+          } else {
+            e2m1x8_to_f16x2(w[0], f[h]);
+          }
+        }
+        const float s0 = b & 1 ? bf16_hi(two[0][b / 2]) : bf16_lo(two[0][b / 2]);
+        const float s1 = b & 1 ? bf16_hi(two[1][b / 2]) : bf16_lo(two[1][b / 2]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma_f16_16816(d, f[0][0], f[1][0], f[0][1], f[1][1], q[n][b][0], q[n][b][1]);
+          mma_f16_16816(d, f[0][2], f[1][2], f[0][3], f[1][3], q[n][b][2], q[n][b][3]);
+          s[n][0] = fmaf(d[0], s0, s[n][0]);
+          s[n][1] = fmaf(d[1], s0, s[n][1]);
+          s[n][2] = fmaf(d[2], s1, s[n][2]);
+          s[n][3] = fmaf(d[3], s1, s[n][3]);
+        }
+      }
+      // in powers of two, those of no key at -inf
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] *= mult[n][j & 1];
+      if constexpr (decltype(ragged)::value) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (key + 2 * t + (j & 1) + 8 * (j >> 1) >= len) {
-              x[i].vs[j] = 0;
-#pragma unroll
-              for (int w = 0; w < kW; ++w) x[i].v[j * kW + w] = 0;
-            }
-        }
-        uint32_t va[D / 8], vb[D / 8];
-        v_pairs<D, kFmt>(x[i].v, x[i].v + kW, v_factor(x[i].vs[0]) | (v_factor(x[i].vs[1]) << 16), va);
-        v_pairs<D, kFmt>(x[i].v + 2 * kW, x[i].v + 3 * kW, v_factor(x[i].vs[2]) | (v_factor(x[i].vs[3]) << 16), vb);
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            mma_bf16_16816(acc[c][n], va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], p[i][n][0], p[i][n][1]);
+            if (tile * 16 + key_g + 8 * (j >> 1) >= len) s[n][j] = -kInf;
       }
+      // The reference m follows the running maximum only when a score passes it by kRise: p stays
+      // below 2^(kCarry + kRise), and most tiles need no exchange between lanes and no rescaling.
+      bool rise = false;
 #pragma unroll
-      for (int i = 0; i < KT; ++i) {
-        some[i] = more[i];
-        if (more[i]) load_v<D, kFmt>(a.cache, row[i], x[i]);
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) rise |= fmaxf(s[n][j], s[n][j + 2]) > m[n][j] + kRise;
+      if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = fmaxf(m[n][j], fmaxf(s[n][j], s[n][j + 2]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float base = top == -kInf ? 0.0f : top;  // no score yet
+            const float fade = exp2_approx(m[n][j] - base);
+            m[n][j] = top;
+            sub[n][j] = base - kCarry;
+            lsum[n][j] *= fade;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) acc[i][n][j] *= fade, acc[i][n][j + 2] *= fade;
+          }
       }
-    }
+      uint32_t p[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float p0 = exp2_approx(s[n][0] - sub[n][0]), p1 = exp2_approx(s[n][1] - sub[n][1]);
+        const float p2 = exp2_approx(s[n][2] - sub[n][0]), p3 = exp2_approx(s[n][3] - sub[n][1]);
+        lsum[n][0] += p0 + p2;
+        lsum[n][1] += p1 + p3;
+        // p is rounded to bf16 for the product (relative 2^-9 each, of either sign); the sum is not
+        p[n][0] = transpose8x8(pack_bf16x2(p0, p1));
+        p[n][1] = transpose8x8(pack_bf16x2(p2, p3));
+      }
+      // output
+      uint32_t w[4][kVw], vs[4];  // keys t, t + 4, t + 8, t + 12
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = t + 4 * j;
+        const uint32_t va = at + 16 * kRowBytes + key * kRowBytes;
+#pragma unroll
+        for (int i = 0; i < kVw; i += 4)
+          lds_words<(kVw < 4 ? kVw : 4)>(va + ((4 * kVw * g + 4 * i) ^ (16 * attn_swizzle<D, kFmt, true>(key))), w[j] + i);
+        vs[j] = lds_u8(at + 32 * kRowBytes + 16 * kGroups + key * kGroups + (g * D / 8) / 32);
+        if constexpr (decltype(ragged)::value)
+          if (tile * 16 + key >= len) {  // rows behind the sequence may hold anything
+            vs[j] = 0;
+#pragma unroll
+            for (int i = 0; i < kVw; ++i) w[j][i] = 0;
+          }
+      }
+      uint32_t va[D / 8], vb[D / 8];
+      v_pairs<D, kFmt>(w[0], w[1], v_factor(vs[0], vs[1]), va);
+      v_pairs<D, kFmt>(w[2], w[3], v_factor(vs[2], vs[3]), vb);
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          mma_bf16_16816(acc[c][n], va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], p[n][0], p[n][1]);
+    };
+    int tile = first * kAttnWarps + warp;
+    const int tile_full = min(tile_last, len >> 4);
+#pragma unroll 1
+    for (; tile < tile_full; tile += kAttnWarps) do_tile(tile, std::false_type{});
+    if (tile < tile_last) do_tile(tile, std::true_type{});
+    cp_async_wait<0>();
+    __syncthreads();  // the rings become the buffer of the parts
 
     // join the warps
 #pragma unroll
@@ -536,27 +602,29 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kerne
   }
 }
 
-// Joins the parts of the heads that lie in several blocks' shares, in the blocks' order, and
-// writes the rows of empty sequences.  One block per (sequence, kv head, chunk).
+// Joins the parts of the heads that lie in several blocks' shares, in a fixed order, and writes the
+// rows of empty sequences.  One block per (sequence, kv head, chunk) and query head; the parts are
+// dealt to its lanes, D / 4 of them to a part.
 template <int D, int NT>
-__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs a, int unit_keys) {
-  constexpr int kHeads = 8 * NT;
+__global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int kHeads = 8 * NT, kLanes = D / 4, kTeams = kAttnThreads / kLanes;
   constexpr float kInf = __builtin_huge_valf();
-  __shared__ long long red[8];
-  __shared__ float top_s[kHeads], sum_s[kHeads];
+  __shared__ long long red[2 * kAttnWarps];
+  __shared__ float4 sums[kTeams][kLanes];
+  __shared__ float ls[kTeams];
   const int per = a.cache.heads * a.chunks;
   const int seq = blockIdx.x / per, hc = blockIdx.x - seq * per;
-  const int head = hc / a.chunks, chunk = hc - head * a.chunks;
-  const int h0 = head * a.group + chunk * kHeads, nh = min(kHeads, a.group - chunk * kHeads);
+  const int head = hc / a.chunks, chunk = hc - head * a.chunks, h = blockIdx.y;
+  if (h >= a.group - chunk * kHeads) return;
+  const size_t at = static_cast<size_t>(seq) * a.q_heads + head * a.group + chunk * kHeads + h;
   long long total, ahead;
-  attn_count_units(a, unit_keys, seq, total, ahead, red);
-  const int units = (attn_length(a, seq) + unit_keys - 1) / unit_keys;
-  const size_t at0 = static_cast<size_t>(seq) * a.q_heads + h0;
+  attn_count_units(a, kAttnUnitKeys, seq, total, ahead, red);
+  const int units = (attn_length(a, seq) + kAttnUnitKeys - 1) / kAttnUnitKeys;
+  const int team = threadIdx.x / kLanes, d = 4 * (threadIdx.x - team * kLanes);
   griddep_wait();
   if (units == 0) {
-    for (int i = threadIdx.x; i < nh * (D / 4); i += 128)
-      *reinterpret_cast<uint2*>(a.out + at0 * D + 4 * static_cast<size_t>(i)) = make_uint2(0, 0);
-    if (a.lse && threadIdx.x < nh) a.lse[at0 + threadIdx.x] = -kInf;
+    if (team == 0) *reinterpret_cast<uint2*>(a.out + at * D + d) = make_uint2(0, 0);
+    if (a.lse && threadIdx.x == 0) a.lse[at] = -kInf;
     return;
   }
   const long long share = attn_share(total, a.blocks), u0 = ahead + static_cast<long long>(hc) * units;
@@ -564,42 +632,37 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
   if (c0 == c1) return;
   // the head begins in block c0 (its slot 1) and covers the start of the others (their slot 0)
   auto part_of = [&](int c) { return a.parts + (2 * static_cast<size_t>(c) + (c == c0 ? 1 : 0)) * kHeads * (D + 2); };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int h = warp; h < nh; h += 4) {
-    float top = -kInf;
-    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, part_of(c)[kHeads * D + 2 * h]);
+  float top = -kInf;
+  for (int c = c0 + static_cast<int>(threadIdx.x & 31); c <= c1; c += 32) top = fmaxf(top, part_of(c)[kHeads * D + 2 * h]);
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const float base = top == -kInf ? 0.0f : top;
-    float l = 0.0f;
-    for (int c = c0 + lane; c <= c1; c += 32) {
-      const float2 ml = *reinterpret_cast<const float2*>(part_of(c) + kHeads * D + 2 * h);
-      l = fmaf(ml.y, exp2_approx(ml.x - base), l);
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-    if (lane == 0) {
-      top_s[h] = base, sum_s[h] = l;
-      if (a.lse) a.lse[at0 + h] = l == 0.0f ? -kInf : (top + log2f(l)) * 0.6931471805599453f;
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < nh * (D / 4); i += 128) {
-    const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
-    const float base = top_s[h], l = sum_s[h];
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  const float base = top == -kInf ? 0.0f : top;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float l = 0.0f;
 #pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const float* part = part_of(c);
-      const float f = exp2_approx(part[kHeads * D + 2 * h] - base);
-      const float4 x4 = *reinterpret_cast<const float4*>(part + h * D + d);
-      o.x = fmaf(x4.x, f, o.x), o.y = fmaf(x4.y, f, o.y), o.z = fmaf(x4.z, f, o.z), o.w = fmaf(x4.w, f, o.w);
-    }
-    const float r = l == 0.0f ? 0.0f : 1.0f / l;
-    uint2 o2;
-    o2.x = pack_bf16x2(o.x * r, o.y * r), o2.y = pack_bf16x2(o.z * r, o.w * r);
-    *reinterpret_cast<uint2*>(a.out + (at0 + h) * D + d) = o2;
+  for (int c = c0 + team; c <= c1; c += kTeams) {
+    const float* part = part_of(c);
+    const float2 ml = *reinterpret_cast<const float2*>(part + kHeads * D + 2 * h);
+    const float4 x4 = *reinterpret_cast<const float4*>(part + h * D + d);
+    const float f = exp2_approx(ml.x - base);
+    l = fmaf(ml.y, f, l);
+    o.x = fmaf(x4.x, f, o.x), o.y = fmaf(x4.y, f, o.y), o.z = fmaf(x4.z, f, o.z), o.w = fmaf(x4.w, f, o.w);
   }
+  sums[team][threadIdx.x - team * kLanes] = o;
+  if (d == 0) ls[team] = l;
+  __syncthreads();
+  if (team != 0) return;
+#pragma unroll
+  for (int i = 1; i < kTeams; ++i) {
+    const float4 x4 = sums[i][threadIdx.x];
+    o.x += x4.x, o.y += x4.y, o.z += x4.z, o.w += x4.w;
+    l += ls[i];
+  }
+  const float r = l == 0.0f ? 0.0f : 1.0f / l;
+  uint2 o2;
+  o2.x = pack_bf16x2(o.x * r, o.y * r), o2.y = pack_bf16x2(o.z * r, o.w * r);
+  *reinterpret_cast<uint2*>(a.out + at * D + d) = o2;
+  if (a.lse && threadIdx.x == 0) a.lse[at] = l == 0.0f ? -kInf : (top + log2f(l)) * 0.6931471805599453f;
 }
 
 }  // namespace mxb
