@@ -15,7 +15,6 @@ word (:func:`mxfp4_b200.device_error`: 0x201 slot, 0x202 position, 0x203 page, 0
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
@@ -25,28 +24,36 @@ from . import _lib
 from .kernels import _check, _require_cuda
 
 KV_FORMATS = {"mxfp8": _lib.KV_MXFP8, "mxfp4": _lib.KV_MXFP4}
-_NOTHING = contextlib.nullcontext()
+_PAGE_SIZES = (16, 32, 64, 128, 256)
+
+# A decoding step calls these with GPU work of a few microseconds, so the checks are plain conditions
+# (a message is only made for a call that is refused) and the stream is asked for by device index.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_BF16, _F32, _I32, _Tensor = torch.bfloat16, torch.float32, torch.int32, torch.Tensor
 
 
-def _on(device: torch.device):
-    """Makes `device` the current one if it is not."""
-    return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _call(device: torch.device, what: str, fn, *args):
+    """One C entry on `device`'s current stream, with `device` current."""
+    i = device.index
+    if i == torch.cuda.current_device():
+        code = fn(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            code = fn(*args, _raw_stream(i))
+    if code:
+        _lib.check(code, what)
 
 
-def _stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _index(t, n: int, device, what: str) -> int:
+    """Address of an int32 vector of n on `device`."""
+    if not (isinstance(t, _Tensor) and t.dtype is _I32 and t.device == device and t.dim() == 1 and t.shape[0] == n
+            and (n < 2 or t.stride(0) == 1)):
+        raise RuntimeError(f"{what} must be a contiguous int32 vector of {n} on {device}")
+    return t.data_ptr()
 
 
-def _check_index(t, n: int, device, what: str):
-    _check(isinstance(t, torch.Tensor) and t.is_cuda and t.device == device, f"{what} must be on the GPU of the other tensors")
-    _check(t.dtype == torch.int32, f"{what} must be int32")
-    _check(t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1), f"{what} must be a contiguous vector of {n}")
-
-
-def _check_bf16(t, device, what: str):
-    _check(isinstance(t, torch.Tensor) and t.is_cuda and (device is None or t.device == device),
-           f"{what} must be on the GPU of the other tensors")
-    _check(t.dtype == torch.bfloat16, f"{what} must be bfloat16")
+def _is_bf16(t, device=None) -> bool:
+    return isinstance(t, _Tensor) and t.dtype is _BF16 and (t.is_cuda if device is None else t.device == device)
 
 
 class MXKVCache:
@@ -71,7 +78,7 @@ class MXKVCache:
         dim = width * (1 if format == "mxfp8" else 2)
         _check(v_codes.shape == k_codes.shape, "v_codes shape")
         _check(dim in (64, 128, 256), "head_dim must be 64, 128 or 256")
-        _check(size in (16, 32, 64, 128, 256), "page_size must be 16, 32, 64, 128 or 256")
+        _check(size in _PAGE_SIZES, "page_size must be 16, 32, 64, 128 or 256")
         _check(pages > 0 and heads > 0 and pages * size < 2**31, "num_pages * page_size must be in 1 .. 2**31 - 1")
         for t in (k_scales, v_scales):
             _check(tuple(t.shape) == (pages, heads, size, dim // 32), "scales shape")
@@ -97,38 +104,41 @@ def new_kv_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: in
                        for n in (width, width, head_dim // 32, head_dim // 32)), format=format)
 
 
-def _rope_arguments(qkv, num_heads, num_kv_heads, dim, cos, sin, positions, q_weight, k_weight, eps):
-    _check_bf16(qkv, None, "qkv")
-    _check(qkv.dim() == 2 and qkv.stride(1) == 1, "qkv must be [tokens, width] with contiguous rows")
-    T, dev = qkv.shape[0], qkv.device
-    _check(num_heads > 0 and num_kv_heads > 0 and qkv.shape[1] == (num_heads + 2 * num_kv_heads) * dim,
-           "qkv's width must be (num_heads + 2 * num_kv_heads) * head_dim")
-    rows = rot = cp = sp = 0
+def _rope_arguments(qkv, heads, kv_heads, dim, cos, sin, positions, q_weight, k_weight):
+    """Checks what the two norm-and-rotation calls share; the arguments of the C entry from cos to
+    weight_dtype, with the interleaved flag left out, and qkv's row stride."""
+    if not (_is_bf16(qkv) and qkv.dim() == 2 and qkv.stride(1) == 1):
+        raise RuntimeError("qkv must be bfloat16 [tokens, width] on the GPU with contiguous rows")
+    tokens, width = qkv.shape
+    if not (heads > 0 and kv_heads > 0 and width == (heads + 2 * kv_heads) * dim):
+        raise RuntimeError("qkv's width must be (num_heads + 2 * num_kv_heads) * head_dim")
+    dev = qkv.device
+    rows = rot = cp = sp = pos = qw = kw = 0
+    wt = _lib.DTYPE_BF16
     if cos is not None or sin is not None:
-        for t in (cos, sin):
-            _check(isinstance(t, torch.Tensor) and t.is_cuda and t.device == dev, "cos and sin must be on qkv's GPU")
-            _check(t.dtype == torch.float32 and t.dim() == 2 and t.is_contiguous(), "cos and sin must be contiguous 2-D float32")
-        _check(cos.shape == sin.shape, "cos and sin must have one shape")
-        rows, rot = cos.shape[0], 2 * cos.shape[1]
-        _check(rows > 0 and rot > 0, "cos and sin must not be empty")
+        if not (isinstance(cos, _Tensor) and isinstance(sin, _Tensor) and cos.dtype is _F32 and sin.dtype is _F32
+                and cos.device == dev and sin.device == dev and cos.dim() == 2 and cos.shape == sin.shape
+                and cos.is_contiguous() and sin.is_contiguous() and cos.numel() > 0):
+            raise RuntimeError(f"cos and sin must be contiguous float32 [rows, rot / 2] of one shape on {dev}")
+        rows, rot = cos.shape
+        rot *= 2
         cp, sp = cos.data_ptr(), sin.data_ptr()
     if positions is not None:
-        _check(rot > 0, "positions without cos and sin")
-        _check_index(positions, T, dev, "positions")
-    else:
-        _check(rot == 0 or rows >= T, "cos and sin need a row per token when no positions are given")
-    _check((q_weight is None) == (k_weight is None), "q_weight and k_weight come together")
-    qw = kw = 0
-    wt = _lib.DTYPE_BF16
-    if q_weight is not None:
+        if not rot:
+            raise RuntimeError("positions without cos and sin")
+        pos = _index(positions, tokens, dev, "positions")
+    elif rows < tokens and rot:
+        raise RuntimeError("cos and sin need a row per token when no positions are given")
+    if q_weight is not None or k_weight is not None:
         for w in (q_weight, k_weight):
-            _check(isinstance(w, torch.Tensor) and w.is_cuda and w.device == dev, "weights must be on qkv's GPU")
-            _check(w.dtype in (torch.bfloat16, torch.float32) and w.dtype == q_weight.dtype, "weights must be bfloat16 or float32")
-            _check(tuple(w.shape) == (dim,) and w.is_contiguous(), "weights must be vectors of head_dim")
+            if not (isinstance(w, _Tensor) and w.device == dev and w.dtype in (_BF16, _F32) and w.shape == (dim,) and w.is_contiguous()):
+                raise RuntimeError(f"q_weight and k_weight come together, contiguous bfloat16 or float32 [head_dim] on {dev}")
+        if q_weight.dtype is not k_weight.dtype:
+            raise RuntimeError("q_weight and k_weight must have one type")
         qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
-        wt = _lib.DTYPE_F32 if q_weight.dtype == torch.float32 else _lib.DTYPE_BF16
-    stride = qkv.stride(0) if T > 1 else qkv.shape[1]
-    return T, dev, stride, cp, sp, rows, rot, positions.data_ptr() if positions is not None else 0, qw, kw, wt, float(eps)
+        if q_weight.dtype is _F32:
+            wt = _lib.DTYPE_F32
+    return tokens, dev, qkv.stride(0) if tokens > 1 else width, (cp, sp, rows, rot), (pos, qw, kw, wt)
 
 
 def qk_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos=None, sin=None, positions=None, q_weight=None,
@@ -144,20 +154,13 @@ def qk_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos=None, sin=None, pos
     Returns new ``(q [tokens, num_heads, head_dim], k [tokens, num_kv_heads, head_dim])`` in bf16, each
     value computed in fp32 and rounded once.
     """
-    _check(isinstance(qkv, torch.Tensor) and qkv.dim() == 2 and num_heads > 0 and num_kv_heads > 0,
-           "qkv must be [tokens, width] with contiguous rows")
+    if not (isinstance(qkv, _Tensor) and qkv.dim() == 2 and num_heads > 0 and num_kv_heads > 0):
+        raise RuntimeError("qkv must be bfloat16 [tokens, width] on the GPU with contiguous rows")
     dim = qkv.shape[1] // (num_heads + 2 * num_kv_heads)
-    T, dev, stride, cp, sp, rows, rot, pos, qw, kw, wt, eps = _rope_arguments(
-        qkv, num_heads, num_kv_heads, dim, cos, sin, positions, q_weight, k_weight, eps)
-    with _on(dev):
-        q = torch.empty((T, num_heads, dim), dtype=torch.bfloat16, device=dev)
-        k = torch.empty((T, num_kv_heads, dim), dtype=torch.bfloat16, device=dev)
-        _lib.check(
-            _lib.lib().mxfp4_qk_norm_rope(qkv.data_ptr(), stride, T, num_heads, num_kv_heads, dim, cp, sp, rows, rot,
-                                          int(interleaved), pos, qw, kw, wt, eps, q.data_ptr(), k.data_ptr(),
-                                          _stream_of(dev)),
-            "mxfp4_qk_norm_rope",
-        )
+    tokens, dev, stride, table, rest = _rope_arguments(qkv, num_heads, num_kv_heads, dim, cos, sin, positions, q_weight, k_weight)
+    q, k = qkv.new_empty((tokens, num_heads, dim)), qkv.new_empty((tokens, num_kv_heads, dim))
+    _call(dev, "mxfp4_qk_norm_rope", _lib.lib().mxfp4_qk_norm_rope, qkv.data_ptr(), stride, tokens, num_heads, num_kv_heads,
+          dim, *table, bool(interleaved), *rest, eps, q.data_ptr(), k.data_ptr())
     return q, k
 
 
@@ -170,28 +173,25 @@ def qk_norm_rope_cache(qkv, num_heads: int, num_kv_heads: int, cos, sin, cache: 
     later is stored.  Keys are coded from the unrounded rotated value, values from ``qkv`` as they
     are.  ``cos`` and ``sin`` may be None (no rotation).  Returns q.
     """
-    _check(isinstance(cache, MXKVCache), "cache must be an MXKVCache")
-    _check(num_kv_heads == cache.num_kv_heads, "num_kv_heads differs from the cache's")
-    T, dev, stride, cp, sp, rows, rot, pos, qw, kw, wt, eps = _rope_arguments(
-        qkv, num_heads, num_kv_heads, cache.head_dim, cos, sin, positions, q_weight, k_weight, eps)
-    _check(dev == cache.device, "qkv must be on the cache's GPU")
-    _check_index(slots, T, dev, "slots")
-    with _on(dev):
-        q = torch.empty((T, num_heads, cache.head_dim), dtype=torch.bfloat16, device=dev)
-        _lib.check(
-            _lib.lib().mxfp4_qk_norm_rope_cache(qkv.data_ptr(), stride, T, num_heads, cp, sp, rows, rot, int(interleaved),
-                                                pos, qw, kw, wt, eps, q.data_ptr(), cache._ref, slots.data_ptr(),
-                                                _stream_of(dev)),
-            "mxfp4_qk_norm_rope_cache",
-        )
+    if not (isinstance(cache, MXKVCache) and num_kv_heads == cache.num_kv_heads):
+        raise RuntimeError("cache must be an MXKVCache of num_kv_heads heads")
+    dim = cache.head_dim
+    tokens, dev, stride, table, rest = _rope_arguments(qkv, num_heads, num_kv_heads, dim, cos, sin, positions, q_weight, k_weight)
+    if dev != cache.device:
+        raise RuntimeError("qkv must be on the cache's GPU")
+    at = _index(slots, tokens, dev, "slots")
+    q = qkv.new_empty((tokens, num_heads, dim))
+    _call(dev, "mxfp4_qk_norm_rope_cache", _lib.lib().mxfp4_qk_norm_rope_cache, qkv.data_ptr(), stride, tokens, num_heads,
+          *table, bool(interleaved), *rest, eps, q.data_ptr(), cache._ref, at)
     return q
 
 
-def _row_stride(t, cache, T, what):
-    _check_bf16(t, cache.device, what)
-    _check(tuple(t.shape) == (T, cache.num_kv_heads, cache.head_dim), f"{what} must be [tokens, num_kv_heads, head_dim]")
-    _check(t.stride(2) == 1 and (cache.num_kv_heads == 1 or t.stride(1) == cache.head_dim), f"{what}: a token's heads must be contiguous")
-    return t.stride(0) if T > 1 else cache.num_kv_heads * cache.head_dim
+def _row_stride(t, cache, tokens, what):
+    heads, dim = cache.num_kv_heads, cache.head_dim
+    if not (_is_bf16(t, cache.device) and t.shape == (tokens, heads, dim) and t.stride(2) == 1
+            and (heads == 1 or t.stride(1) == dim)):
+        raise RuntimeError(f"{what} must be bfloat16 [tokens, num_kv_heads, head_dim] on the cache's GPU, a token's heads contiguous")
+    return t.stride(0) if tokens > 1 else heads * dim
 
 
 def kv_cache_write(cache: MXKVCache, k, v, slots) -> None:
@@ -199,33 +199,25 @@ def kv_cache_write(cache: MXKVCache, k, v, slots) -> None:
     row stride that is a multiple of 8) into the cache rows ``slots`` names, as
     :func:`qk_norm_rope_cache` does: the OCP MX rule, the counterpart of
     ``quantize_mxfp4(..., rule="ocp")`` and :func:`quantize_act_mx8`."""
-    _check(isinstance(cache, MXKVCache), "cache must be an MXKVCache")
-    _check(isinstance(k, torch.Tensor) and k.dim() == 3, "k must be [tokens, num_kv_heads, head_dim]")
-    T = k.shape[0]
-    ks, vs = _row_stride(k, cache, T, "k"), _row_stride(v, cache, T, "v")
-    _check_index(slots, T, cache.device, "slots")
-    with _on(cache.device):
-        _lib.check(
-            _lib.lib().mxfp4_kv_cache_write(cache._ref, k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(), T,
-                                            _stream_of(cache.device)),
-            "mxfp4_kv_cache_write",
-        )
+    if not (isinstance(cache, MXKVCache) and isinstance(k, _Tensor) and k.dim() == 3):
+        raise RuntimeError("cache must be an MXKVCache, k [tokens, num_kv_heads, head_dim]")
+    tokens = k.shape[0]
+    ks, vs = _row_stride(k, cache, tokens, "k"), _row_stride(v, cache, tokens, "v")
+    at = _index(slots, tokens, cache.device, "slots")
+    _call(cache.device, "mxfp4_kv_cache_write", _lib.lib().mxfp4_kv_cache_write, cache._ref, k.data_ptr(), ks, v.data_ptr(), vs,
+          at, tokens)
 
 
 def kv_cache_read(cache: MXKVCache, slots):
     """The rows ``slots`` (int32 ``[tokens]``) names, as new bf16 ``(k, v)`` of ``[tokens, num_kv_heads,
     head_dim]``; a negative slot reads zeros, the scale byte 255 NaN."""
-    _check(isinstance(cache, MXKVCache), "cache must be an MXKVCache")
-    _check(isinstance(slots, torch.Tensor) and slots.dim() == 1, "slots must be a vector")
-    T, dev = slots.shape[0], cache.device
-    _check_index(slots, T, dev, "slots")
-    with _on(dev):
-        k = torch.empty((T, cache.num_kv_heads, cache.head_dim), dtype=torch.bfloat16, device=dev)
-        v = torch.empty_like(k)
-        _lib.check(
-            _lib.lib().mxfp4_kv_cache_read(cache._ref, slots.data_ptr(), T, k.data_ptr(), v.data_ptr(), _stream_of(dev)),
-            "mxfp4_kv_cache_read",
-        )
+    if not (isinstance(cache, MXKVCache) and isinstance(slots, _Tensor) and slots.dim() == 1):
+        raise RuntimeError("cache must be an MXKVCache, slots a vector")
+    tokens, dev = slots.shape[0], cache.device
+    at = _index(slots, tokens, dev, "slots")
+    shape = (tokens, cache.num_kv_heads, cache.head_dim)
+    k, v = slots.new_empty(shape, dtype=_BF16), slots.new_empty(shape, dtype=_BF16)
+    _call(dev, "mxfp4_kv_cache_read", _lib.lib().mxfp4_kv_cache_read, cache._ref, at, tokens, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -242,36 +234,32 @@ def paged_attention(q, cache: MXKVCache, page_table, lengths, scale: float | Non
     ``return_lse`` also fp32 ``[seqs, num_heads]``: the natural log of the sum of exp(scale * q . k), -inf
     for an empty sequence.  The same call gives the same bits.
     """
-    _check(isinstance(cache, MXKVCache), "cache must be an MXKVCache")
-    dev, D = cache.device, cache.head_dim
-    _check_bf16(q, dev, "q")
-    _check(q.dim() == 3 and q.shape[2] == D and q.shape[1] > 0, "q must be [seqs, num_heads, head_dim]")
-    B, H = q.shape[0], q.shape[1]
-    _check(H % cache.num_kv_heads == 0, "num_heads must be a multiple of num_kv_heads")
-    _check(q.stride(2) == 1 and (H == 1 or q.stride(1) == D), "q: a sequence's heads must be contiguous")
-    _check(isinstance(page_table, torch.Tensor) and page_table.is_cuda and page_table.device == dev
-           and page_table.dtype == torch.int32, "page_table must be int32 on the cache's GPU")
-    _check(page_table.dim() == 2 and page_table.shape[0] == B and page_table.shape[1] > 0
-           and (page_table.shape[1] == 1 or page_table.stride(1) == 1), "page_table must be [seqs, max_pages] with contiguous rows")
-    _check_index(lengths, B, dev, "lengths")
-    P = page_table.shape[1]
-    scale = D ** -0.5 if scale is None else float(scale)
-    _check(math.isfinite(scale), "scale must be finite")
-    with _on(dev):
-        if out is None:
-            out = torch.empty((B, H, D), dtype=torch.bfloat16, device=dev)
-        else:
-            _check_bf16(out, dev, "out")
-            _check(tuple(out.shape) == (B, H, D) and out.is_contiguous(), "out shape/contig")
-        lse = torch.empty((B, H), dtype=torch.float32, device=dev) if return_lse else None
-        L = _lib.lib()
-        nws = L.mxfp4_paged_attention_workspace_bytes(cache._ref, B, H, P)
-        ws = torch.empty(nws, dtype=torch.uint8, device=dev)
-        _lib.check(
-            L.mxfp4_paged_attention(q.data_ptr(), q.stride(0) if B > 1 else H * D, cache._ref, page_table.data_ptr(),
-                                    page_table.stride(0) if B > 1 else P, P, lengths.data_ptr(), B, H, scale,
-                                    out.data_ptr(), lse.data_ptr() if return_lse else 0, ws.data_ptr(), nws,
-                                    _stream_of(dev)),
-            "mxfp4_paged_attention",
-        )
+    if not isinstance(cache, MXKVCache):
+        raise RuntimeError("cache must be an MXKVCache")
+    dev, dim, kv_heads = cache.device, cache.head_dim, cache.num_kv_heads
+    if not (_is_bf16(q, dev) and q.dim() == 3 and q.shape[2] == dim and q.stride(2) == 1):
+        raise RuntimeError("q must be bfloat16 [seqs, num_heads, head_dim] on the cache's GPU")
+    seqs, heads, _ = q.shape
+    if heads == 0 or heads % kv_heads or (heads > 1 and q.stride(1) != dim):
+        raise RuntimeError("q: num_heads must be a multiple of num_kv_heads, a sequence's heads contiguous")
+    if not (isinstance(page_table, _Tensor) and page_table.dtype is _I32 and page_table.device == dev and page_table.dim() == 2):
+        raise RuntimeError("page_table must be int32 [seqs, max_pages] on the cache's GPU")
+    rows, pages = page_table.shape
+    if rows != seqs or pages == 0 or (pages > 1 and page_table.stride(1) != 1):
+        raise RuntimeError("page_table must be [seqs, max_pages] with contiguous rows")
+    lens = _index(lengths, seqs, dev, "lengths")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise RuntimeError("scale must be finite")
+    if out is None:
+        out = q.new_empty((seqs, heads, dim))
+    elif not (_is_bf16(out, dev) and out.shape == (seqs, heads, dim) and out.is_contiguous()):
+        raise RuntimeError("out must be contiguous bfloat16 [seqs, num_heads, head_dim] on the cache's GPU")
+    lse = q.new_empty((seqs, heads), dtype=_F32) if return_lse else None
+    L = _lib.lib()
+    nws = L.mxfp4_paged_attention_workspace_bytes(cache._ref, seqs, heads, pages)
+    ws = q.new_empty(nws // 2)
+    _call(dev, "mxfp4_paged_attention", L.mxfp4_paged_attention, q.data_ptr(), q.stride(0) if seqs > 1 else heads * dim, cache._ref,
+          page_table.data_ptr(), page_table.stride(0) if seqs > 1 else pages, pages, lens, seqs, heads, scale, out.data_ptr(),
+          lse.data_ptr() if return_lse else 0, ws.data_ptr(), nws)
     return (out, lse) if return_lse else out
