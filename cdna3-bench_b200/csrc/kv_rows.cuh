@@ -1,9 +1,9 @@
 // Head rows between the QKV GEMM and the attention: per-head RMS norm, rotation, and the MX
 // key-value cache those rows are coded into and read back from.
 //
-// A row is one head of one token, D bf16 values (D % 32 == 0, D <= 256).  A lane holds 8
-// neighbouring values (one 16-byte load), so a row takes LPR = 4, 8, 16 or 32 lanes and a warp
-// works on 32 / LPR rows of one kind (q, k or v) at a time.
+// A row is one head of one token, D bf16 values (D % 32 == 0, D <= 256).  For the rows to be coded a
+// lane holds 8 neighbouring values (one 16-byte load), so a row takes LPR = 4, 8, 16 or 32 lanes and
+// a warp works on 32 / LPR rows of one kind at a time; for those that stay bf16 it holds 16.
 //
 //   norm      y_i = x_i * w_i / sqrt(mean(x^2) + eps)
 //   rotation  of the first R values with c = cos[p][i], s = sin[p][i], i < R/2:
@@ -42,19 +42,18 @@ struct RowArgs {
   long long q_stride, k_stride, v_stride;    // elements from one token to the next
   int tokens, q_heads, kv_heads, dim;
   const float *cos, *sin;                    // [table_rows][rot / 2]; rot == 0: no rotation
-  int table_rows, rot, interleaved;
+  int table_rows, rot;
   const int* positions;                      // table row of each token; null: the token's index
   const void *q_weight, *k_weight;           // [dim]; null: no norm
   int weight_f32;
-  double eps;
+  double eps, inv_dim;
   __nv_bfloat16 *q_out, *k_out;              // [tokens][heads][dim]
   KvCacheView cache;
   const int* slots;                          // cache row of each token; negative: not stored
 };
 
 // Eight values of a 16-byte load of bf16.
-template <typename Real>
-__device__ __forceinline__ void unpack_bf16x8(const uint4& u, Real (&v)[8]) {
+__device__ __forceinline__ void unpack_bf16x8(const uint4& u, float (&v)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -63,79 +62,220 @@ __device__ __forceinline__ void unpack_bf16x8(const uint4& u, Real (&v)[8]) {
   }
 }
 
-template <typename Real>
-__device__ __forceinline__ void load_weight8(const void* w, int f32, int at, Real (&v)[8]) {
-  if (f32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w) + at);
-    const float4 a = __ldg(p), b = __ldg(p + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w) + at)), v);
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void load_weight8(const void* w, int f32, int at, float (&v)[8]) {
+  if (f32) load8(static_cast<const float*>(w) + at, v);
+  else unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w) + at)), v);
+}
+
+// What the lane's 8 values are multiplied by: value i of a row becomes
+//   r (x_i w_i c_i + xp_i wp_i s_i),
+// xp and wp the values and weights of the partners (s carries the sign; past the rotated part c = 1,
+// s = 0; r = 1 and w = 1 without a norm).
+struct LaneTurn {
+  float c[8], s[8], w[8], wp[8];
+};
+template <int LPR, bool kInter>
+__device__ __forceinline__ void load_turn(const RowArgs& a, int p, const void* weight, LaneTurn& q) {
+  const int at = 8 * (threadIdx.x & (LPR - 1)), half = a.rot >> 1;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q.c[i] = 1.0f, q.s[i] = 0.0f, q.w[i] = 1.0f, q.wp[i] = 1.0f;
+  int partner = at;
+  if (at < a.rot) {
+    if constexpr (kInter) {
+      const size_t i0 = static_cast<size_t>(p) * half + (at >> 1);
+      const float4 c = __ldg(reinterpret_cast<const float4*>(a.cos + i0)), s = __ldg(reinterpret_cast<const float4*>(a.sin + i0));
+      q.c[0] = q.c[1] = c.x, q.c[2] = q.c[3] = c.y, q.c[4] = q.c[5] = c.z, q.c[6] = q.c[7] = c.w;
+      q.s[0] = -s.x, q.s[1] = s.x, q.s[2] = -s.y, q.s[3] = s.y, q.s[4] = -s.z, q.s[5] = s.z, q.s[6] = -s.w, q.s[7] = s.w;
+    } else {
+      const bool low = at < half;
+      const size_t i0 = static_cast<size_t>(p) * half + (low ? at : at - half);
+      load8(a.cos + i0, q.c);
+      load8(a.sin + i0, q.s);
+      if (low) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q.s[i] = -q.s[i];
+      }
+      partner = low ? at + half : at - half;
+    }
+  }
+  if (weight && at < a.dim) {
+    load_weight8(weight, a.weight_f32, at, q.w);
+    float v[8];
+    load_weight8(weight, a.weight_f32, partner, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q.wp[i] = v[kInter ? i ^ 1 : i];
   }
 }
 
-__device__ __forceinline__ float inv_sqrt(float x) { return rsqrtf(x); }
-__device__ __forceinline__ double inv_sqrt(double x) { return rsqrt(x); }
+// The partners' values: the neighbours' (interleaved) or another lane's (halves); zeros past the
+// rotated part (a value there times s = 0 would be lost to an infinity).  v: x unpacked.  The whole warp.
+template <int LPR, bool kInter>
+__device__ __forceinline__ void partner_values(const RowArgs& a, const uint4& x, const float (&v)[8], float (&z)[8]) {
+  const int at = 8 * (threadIdx.x & (LPR - 1)), half = a.rot >> 1, lane = threadIdx.x & 31;
+  if constexpr (kInter) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = v[i ^ 1];
+  } else {
+    const int src = at >= a.rot ? lane : (at < half ? lane + (half >> 3) : lane - (half >> 3));
+    uint4 px;
+    px.x = __shfl_sync(0xffffffffu, x.x, src);
+    px.y = __shfl_sync(0xffffffffu, x.y, src);
+    px.z = __shfl_sync(0xffffffffu, x.z, src);
+    px.w = __shfl_sync(0xffffffffu, x.w, src);
+    unpack_bf16x8(px, z);
+  }
+  if (a.rot < a.dim && at >= a.rot) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = 0.0f;
+  }
+}
 
-// Norm and rotation of one row in the precision of Real: x are the lane's 8 values, c and s its
-// cos / sin (8 of them for the halves form, the first 4 for the interleaved one).  Every lane of
-// the warp takes part (shuffles); lanes past the row hold zeros.
-template <int LPR, typename Real>
-__device__ __forceinline__ void norm_rotate(const RowArgs& a, const uint4& x, const void* weight, const float (&c)[8],
-                                            const float (&s)[8], Real (&y)[8]) {
-  const int l = threadIdx.x & (LPR - 1), at = 8 * l;
-  const bool live = at < a.dim;
-  unpack_bf16x8(x, y);
-  Real r = 1;
-  if (weight) {
-    Real ss = 0;
+// Pairs of fp32 values in one 64-bit register: sm_100 multiplies and adds both in one instruction.
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 1 / sqrt(mean(x^2) + eps) of the row the lane's 8 values belong to.  The whole warp.
+template <int LPR>
+__device__ __forceinline__ float inverse_rms(const RowArgs& a, const float (&v)[8]) {
+  uint64_t s2 = mul_f32x2(pack_f32x2(v[0], v[1]), pack_f32x2(v[0], v[1]));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += y[i] * y[i];
+  for (int i = 2; i < 8; i += 2) s2 = fma_f32x2(pack_f32x2(v[i], v[i + 1]), pack_f32x2(v[i], v[i + 1]), s2);
+  float ss, s1;
+  unpack_f32x2(s2, ss, s1);
+  ss += s1;
 #pragma unroll
-    for (int m = LPR / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-    r = inv_sqrt(ss / static_cast<Real>(a.dim) + static_cast<Real>(a.eps));
-    if (live) {
-      Real w[8];
-      load_weight8(weight, a.weight_f32, at, w);
+  for (int m = LPR / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+  return rsqrtf(fmaf(ss, static_cast<float>(a.inv_dim), static_cast<float>(a.eps)));
+}
+
+// ---- rows that stay bf16 ----
+// Here a lane holds 16 values, two pieces of 8 that a halves rotation pairs with each other, so that
+// nothing but the norm's sum crosses lanes and a warp works on 64 / LPR rows: lanes l < R / 16 hold
+// the pieces at 8 l and R/2 + 8 l, the lanes behind them the same of what follows R.
+struct LanePieces {
+  int a, b;  // their places; b >= dim: none
+};
+__device__ __forceinline__ LanePieces lane_pieces(const RowArgs& a, int l) {
+  const int turned = a.rot >> 4;
+  if (l < turned) return {8 * l, (a.rot >> 1) + 8 * l};
+  const int at = a.rot + 8 * (l - turned);
+  return {at, at + ((a.dim - a.rot) >> 1)};
+}
+// Value i becomes r (x_i cw_i + xp_i sw_i), xp the partner's: i ^ 1 (interleaved) or i ^ 8 (halves).
+struct LaneTurn16 {
+  float cw[16], sw[16];
+};
+template <bool kInter>
+__device__ __forceinline__ void load_turn16(const RowArgs& a, int p, const void* weight, int l, LaneTurn16& q) {
+  const LanePieces at = lane_pieces(a, l);
+  const bool rotated = l < (a.rot >> 4);
+  float w[16], c[8], s[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * r * w[i];
+  for (int i = 0; i < 16; ++i) w[i] = 1.0f;
+  if (weight && at.b < a.dim) {
+    float u[8], v[8];
+    load_weight8(weight, a.weight_f32, at.a, u);
+    load_weight8(weight, a.weight_f32, at.b, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = u[i], w[8 + i] = v[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = 1.0f, s[i] = 0.0f;
+  if (rotated) {
+    const size_t row = static_cast<size_t>(p) * (a.rot >> 1);
+    if constexpr (kInter) {  // four angles for each piece
+      const float4 c0 = __ldg(reinterpret_cast<const float4*>(a.cos + row + (at.a >> 1)));
+      const float4 c1 = __ldg(reinterpret_cast<const float4*>(a.cos + row + (at.b >> 1)));
+      const float4 s0 = __ldg(reinterpret_cast<const float4*>(a.sin + row + (at.a >> 1)));
+      const float4 s1 = __ldg(reinterpret_cast<const float4*>(a.sin + row + (at.b >> 1)));
+      c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+      s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+    } else {  // eight for the pairs of the two
+      load8(a.cos + row + at.a, c);
+      load8(a.sin + row + at.a, s);
     }
   }
-  if (a.rot == 0) return;
-  if (a.interleaved) {
-    if (at < a.rot) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const Real u = y[2 * i], v = y[2 * i + 1];
-        y[2 * i] = u * static_cast<Real>(c[i]) - v * static_cast<Real>(s[i]);
-        y[2 * i + 1] = v * static_cast<Real>(c[i]) + u * static_cast<Real>(s[i]);
+  for (int i = 0; i < 16; ++i) {
+    const int j = kInter ? i >> 1 : i & 7;         // the angle
+    const bool first = kInter ? !(i & 1) : i < 8;  // of its pair
+    q.cw[i] = c[j] * w[i];
+    q.sw[i] = (first ? -s[j] : s[j]) * w[kInter ? i ^ 1 : i ^ 8];
+  }
+}
+// One row per LPR / 2 lanes: the lane's pieces x[0], x[1] in, packed bf16 out.  The whole warp.
+template <int LPR, bool kInter>
+__device__ __forceinline__ void turn_row16(const RowArgs& a, uint4 (&x)[2], const LaneTurn16& q, bool norm, bool rotated) {
+  float v[16];
+  {
+    float u[8];
+    unpack_bf16x8(x[0], u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = u[i];
+    unpack_bf16x8(x[1], u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[8 + i] = u[i];
+  }
+  uint64_t v2[8], y2[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v2[i] = pack_f32x2(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y2[i] = mul_f32x2(v2[i], pack_f32x2(q.cw[2 * i], q.cw[2 * i + 1]));
+  if (rotated) {  // past the rotated part an infinity times s = 0 would be a NaN
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (kInter) {
+        float lo, hi;
+        unpack_f32x2(y2[i], lo, hi);
+        y2[i] = pack_f32x2(fmaf(v[2 * i + 1], q.sw[2 * i], lo), fmaf(v[2 * i], q.sw[2 * i + 1], hi));
+      } else {
+        y2[i] = fma_f32x2(v2[i ^ 4], pack_f32x2(q.sw[2 * i], q.sw[2 * i + 1]), y2[i]);
       }
     }
-    return;
   }
-  // halves: the partner's values come as the packed input (4 shuffles) and are normed here too
-  const int half = a.rot >> 1, lane = threadIdx.x & 31;
-  const bool rotated = at < a.rot, low = at < half;
-  const int src = rotated ? (low ? lane + (half >> 3) : lane - (half >> 3)) : lane;
-  uint4 px;
-  px.x = __shfl_sync(0xffffffffu, x.x, src);
-  px.y = __shfl_sync(0xffffffffu, x.y, src);
-  px.z = __shfl_sync(0xffffffffu, x.z, src);
-  px.w = __shfl_sync(0xffffffffu, x.w, src);
-  if (!rotated) return;
-  Real z[8];
-  unpack_bf16x8(px, z);
-  if (weight) {
-    Real w[8];
-    load_weight8(weight, a.weight_f32, low ? at + half : at - half, w);
+  if (norm) {
+    uint64_t s2 = mul_f32x2(v2[0], v2[0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] = z[i] * r * w[i];
+    for (int i = 1; i < 8; ++i) s2 = fma_f32x2(v2[i], v2[i], s2);
+    float ss, s1;
+    unpack_f32x2(s2, ss, s1);
+    ss += s1;
+#pragma unroll
+    for (int m = LPR / 4; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+    const float r = rsqrtf(fmaf(ss, static_cast<float>(a.inv_dim), static_cast<float>(a.eps)));
+    const uint64_t r2 = pack_f32x2(r, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y2[i] = mul_f32x2(y2[i], r2);
   }
+  uint32_t o[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const Real sn = low ? -static_cast<Real>(s[i]) : static_cast<Real>(s[i]);
-    y[i] = y[i] * static_cast<Real>(c[i]) + z[i] * sn;
+    float lo, hi;
+    unpack_f32x2(y2[i], lo, hi);
+    o[i] = pack_bf16x2(lo, hi);
   }
+  x[0] = make_uint4(o[0], o[1], o[2], o[3]);
+  x[1] = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
 // A double as a float rounded to odd: truncated, the last bit set when anything was cut off.  A
@@ -144,8 +284,6 @@ __device__ __forceinline__ float round_odd(double d) {
   const float f = __double2float_rz(d);
   return static_cast<double>(f) == d ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
-__device__ __forceinline__ float round_odd(float f) { return f; }
-
 __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
   uint32_t r;
   asm("{\n\t.reg .b8 t;\n\t"
@@ -156,82 +294,219 @@ __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
   return r;
 }
 
-// Codes the lane's 8 values as part of their 32-value group (4 lanes) and writes codes and scale.
-template <int kFmt, typename Real>
-__device__ __forceinline__ void code_and_store(const Real (&y)[8], bool live, size_t row, int dim, int at,
-                                               uint8_t* codes, uint8_t* scales) {
-  float f[8];
-  uint32_t amax = 0;  // of the magnitudes' bits: a NaN sorts above infinity
+// Scale byte of a group whose largest magnitude has these bits (a NaN sorts above infinity): the
+// biased exponent field is floor(log2(amax)) + 127, and 0 for zero and subnormals, which clip anyway.
+template <int kFmt>
+__device__ __forceinline__ int scale_byte(uint32_t amax) {
+  return amax > 0x7F800000u ? 255 : max(static_cast<int>(amax >> 23) - (kFmt == kFmtE4M3 ? 8 : 2), 0);
+}
+// The lane's 8 codes, packed: two words of E4M3 or one of E2M1.
+template <int kFmt>
+__device__ __forceinline__ uint2 code8(const float (&f)[8], float inv) {
+  if constexpr (kFmt == kFmtE4M3)
+    return make_uint2(e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16),
+                      e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16));
+  // + 0.0f: a negative zero is coded as zero, as mxfp4_quantize does
+  uint32_t o = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    f[i] = round_odd(y[i]);
-    amax = max(amax, __float_as_uint(f[i]) & 0x7FFFFFFFu);
-  }
-  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  const bool nan = amax > 0x7F800000u;
-  // biased exponent field = floor(log2(amax)) + 127 (0 for zero and subnormals, which clip anyway)
-  const int byte = max(static_cast<int>(amax >> 23) - (kFmt == kFmtE4M3 ? 8 : 2), 0);
-  const float inv = nan ? 0.0f : exp2_neg(byte - 127);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = nan ? 0.0f : f[i] * inv;
-  if (!live) return;
-  if (kFmt == kFmtE4M3) {
-    uint2 o;
-    o.x = e4m3x2(f[0], f[1]) | (e4m3x2(f[2], f[3]) << 16);
-    o.y = e4m3x2(f[4], f[5]) | (e4m3x2(f[6], f[7]) << 16);
-    *reinterpret_cast<uint2*>(codes + row * dim + at) = o;
-  } else {
-    // + 0.0f: a negative zero is coded as zero, as mxfp4_quantize does
-    uint32_t o = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o |= e2m1x2(f[2 * i] + 0.0f, f[2 * i + 1] + 0.0f) << (8 * i);
-    *reinterpret_cast<uint32_t*>(codes + row * (dim / 2) + at / 2) = o;
-  }
-  if ((at & 31) == 0) scales[row * (dim / 32) + at / 32] = static_cast<uint8_t>(nan ? 255 : byte);
+  for (int i = 0; i < 4; ++i) o |= e2m1x2(fmaf(f[2 * i], inv, 0.0f), fmaf(f[2 * i + 1], inv, 0.0f)) << (8 * i);
+  return make_uint2(o, 0);
+}
+template <int kFmt>
+__device__ __forceinline__ void store_codes(const KvCacheView& c, bool key, size_t row, int at, const uint2& o, int byte) {
+  uint8_t* codes = key ? c.k_codes : c.v_codes;
+  if constexpr (kFmt == kFmtE4M3) *reinterpret_cast<uint2*>(codes + row * c.dim + at) = o;
+  else *reinterpret_cast<uint32_t*>(codes + row * (c.dim / 2) + at / 2) = o.x;
+  if ((at & 31) == 0) (key ? c.k_scales : c.v_scales)[row * (c.dim / 32) + at / 32] = static_cast<uint8_t>(byte);
 }
 
-constexpr int kRowThreads = 128;
+__device__ __forceinline__ uint32_t magnitude_bits(const float (&f)[8]) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+  return amax;
+}
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {  // over the 4 lanes of a group of 32 values
+  v = max(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return max(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
 
-// One token per blockIdx.x, a share of its head rows per blockIdx.y.
+// Codes 8 values per lane as they are (or rounded to odd) and stores them.  The whole warp.
+template <int kFmt>
+__device__ __forceinline__ void code_and_store(const KvCacheView& c, bool key, const float (&f)[8], bool here, size_t row,
+                                               int at) {
+  const int byte = scale_byte<kFmt>(group_max(magnitude_bits(f)));
+  uint2 o = make_uint2(0, 0);
+  if (byte != 255) o = code8<kFmt>(f, exp2_neg(byte - 127));
+  if (here) store_codes<kFmt>(c, key, row, at, o, byte);
+}
+
+constexpr int kRowThreads = 64;
+constexpr int kRowBlocks = 10;  // resident per SM
+
+// One row in 64 bits, each value rounded to odd.  The whole warp.
+template <int LPR, bool kInter>
+__device__ __forceinline__ void turn_row_exact(const RowArgs& a, const uint4& x, const LaneTurn& q, bool norm, float (&f)[8]) {
+  float v[8], z[8];
+  unpack_bf16x8(x, v);
+  double r = 1.0;
+  if (norm) {
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), ss);
+#pragma unroll
+    for (int m = LPR / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+    r = rsqrt(fma(ss, a.inv_dim, a.eps));
+  }
+  partner_values<LPR, kInter>(a, x, v, z);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // value * weight and weight * cos are exact in 64 bits
+    const double u = static_cast<double>(v[i]) * q.w[i], t = static_cast<double>(z[i]) * q.wp[i];
+    f[i] = round_odd(r * fma(u, static_cast<double>(q.c[i]), t * q.s[i]));
+  }
+}
+
+
+// Keys h .. of token t (head h + sub per lane), normed, rotated and coded in 64 bits.  The whole warp.
+template <int LPR, int kFmt, bool kInter>
+__device__ __noinline__ void store_keys_exact(const RowArgs* ap, int t, int p, int slot, int h0) {
+  const RowArgs& a = *ap;
+  const int lane = threadIdx.x & 31, at = 8 * (lane & (LPR - 1)), h = h0 + lane / LPR;
+  const bool here = at < a.dim && h < a.kv_heads;
+  uint4 x = make_uint4(0, 0, 0, 0);
+  if (here) x = *reinterpret_cast<const uint4*>(a.k + a.k_stride * t + h * a.dim + at);
+  LaneTurn q;
+  load_turn<LPR, kInter>(a, p, a.k_weight, q);
+  float f[8];
+  turn_row_exact<LPR, kInter>(a, x, q, a.k_weight != nullptr, f);
+  code_and_store<kFmt>(a.cache, true, f, here, here ? a.cache.row(slot, h) : 0, at);
+}
+
+// The same keys in 32 bits, kept where that settles every code.  With T_i = |x_i c w| + |xp_i s wp|
+// the 32-bit value is off by less than 2^-19 r T_i: 2^-24 each for the products c w and s wp, the
+// product, the sum and the factor r; in r 2^-22 for rsqrtf and half of 16 * 2^-24 for the sum of
+// squares (13 roundings), the mean and eps; 1.1 * 2^-20 in all, the interval's ends included.
+// Where the group's exponent and all codes are the same at both
+// ends of that interval they are the 64-bit ones.  Returns false otherwise (about one call in
+// a hundred: 256 values, 2^-14 each), with nothing stored.  The whole warp.
+template <int LPR, int kFmt, bool kInter>
+__device__ __forceinline__ bool store_keys(const RowArgs& a, const uint4& x, const float (&cw)[8], const float (&sw)[8], bool here,
+                                           size_t row, int at) {
+  float v[8], z[8], lo[8], hi[8];
+  unpack_bf16x8(x, v);
+  const float r = a.k_weight ? inverse_rms<LPR>(a, v) : 1.0f;
+  partner_values<LPR, kInter>(a, x, v, z);
+  // values that no rounding touches (past the rotated part, without a norm) are their own interval
+  const float off = a.k_weight || at < a.rot ? r * 1.9073486328125e-6f : 0.0f;
+  float top_lo = 0.0f, top_hi = 0.0f;
+  bool ok = true;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float u = z[i] * sw[i], y = fmaf(v[i], cw[i], u) * r, e = fmaf(fabsf(v[i]), fabsf(cw[i]), fabsf(u)) * off;
+    lo[i] = y - e, hi[i] = y + e;
+    top_lo = fmaxf(top_lo, fabsf(y) - e);
+    top_hi = fmaxf(top_hi, fabsf(y) + e);
+    ok &= fabsf(y) + e < 3.0e38f;  // infinities and NaN are left to the exact path
+  }
+  const uint32_t b0 = group_max(__float_as_uint(top_lo)), b1 = group_max(__float_as_uint(top_hi));
+  const int byte = scale_byte<kFmt>(b1);
+  const float inv = exp2_neg(byte - 127);
+  const uint2 c0 = code8<kFmt>(lo, inv), c1 = code8<kFmt>(hi, inv);
+  ok &= scale_byte<kFmt>(b0) == byte && c0.x == c1.x && c0.y == c1.y;
+  if (!__all_sync(0xffffffffu, ok || !here)) return false;
+  if (here) store_codes<kFmt>(a.cache, true, row, at, c1, byte);
+  return true;
+}
+
+constexpr int kRowStage = 3;  // sets of rows of each kind a warp has on their way at once, 1024 bytes each
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// One token per blockIdx.x, a share of its head rows per warp of blockIdx.y's blocks.
 //
-// Bound by HBM: each row is read once and written once.  q is computed in 32 bits and rounded to
-// bf16 once.  A key on its way into the cache is computed in 64 bits: next to a rounding border
-// an error in the 24th bit would pick the neighbouring code, and with it the stored byte would
-// depend on how the norm's sum was ordered.  Its few rows (kv_heads of q_heads + 2 kv_heads) hide
-// behind the loads.
+// Bound by HBM: each row is read once and written once.  A warp first sends for its rows (up to
+// kRowStage sets of each kind) with asynchronous copies to shared memory, each lane's bytes to a
+// place of its own, so that bytes in flight cost no registers.  q is computed in 32 bits and rounded
+// to bf16 once, with cos, sin and the weight multiplied together once per warp.  A key on its
+// way into the cache has the codes of the 64-bit value: next to a rounding border an error in the
+// 24th bit would pick the neighbouring code, and with it the stored byte would depend on how
+// the norm's sum was ordered.  store_keys settles almost all of them in 32 bits.
 //
 // Two tokens of one launch that name the same slot: the later one is stored (every block looks
 // through the slots behind its own; the caller keeps a launch to 4096 tokens).
-template <int LPR, int kFmt>
-__global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_constant__ RowArgs a, int first) {
-  constexpr int kRows = 32 / LPR;  // rows a warp works on at a time
-  const int t = first + blockIdx.x;
-  const int warp = (blockIdx.y * kRowThreads + threadIdx.x) >> 5, warps = gridDim.y * (kRowThreads / 32);
-  const int lane = threadIdx.x & 31, l = lane & (LPR - 1), sub = lane / LPR, at = 8 * l;
+template <int LPR, int kFmt, bool kInter>
+__global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(const __grid_constant__ RowArgs a, int first) {
+  constexpr int kRows = 32 / LPR;  // rows to be coded a warp works on at a time
+  __shared__ __align__(16) uint8_t stage_s[kRowThreads / 32][2 * kRowStage * 1024];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, at = 8 * (lane & (LPR - 1)), sub = lane / LPR;
   const bool live = at < a.dim;
+  const int t = first + blockIdx.x, part = blockIdx.y * (kRowThreads / 32) + warp, parts = gridDim.y * (kRowThreads / 32);
 
-  bool good = true;
-  float c[8], s[8];
-  if (a.rot) {
-    const int p = a.positions ? __ldg(a.positions + t) : t;
-    good = p >= 0 && p < a.table_rows;
-    if (!good && threadIdx.x == 0) record_error(kErrBadPosition);
-    if (good && at < a.rot) {
-      const int half = a.rot >> 1;
-      const int i0 = a.interleaved ? at >> 1 : (at < half ? at : at - half);
-      const float4* pc = reinterpret_cast<const float4*>(a.cos + static_cast<size_t>(p) * half + i0);
-      const float4* ps = reinterpret_cast<const float4*>(a.sin + static_cast<size_t>(p) * half + i0);
-      const float4 c0 = __ldg(pc), s0 = __ldg(ps);
-      c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w;
-      if (!a.interleaved) {
-        const float4 c1 = __ldg(pc + 1), s1 = __ldg(ps + 1);
-        c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+  // q rows (and k rows that stay bf16): the warp's sets are part, part + parts, ... of 2 * kRows rows;
+  // k's from the other end, so that a warp with a q set less comes first.
+  const int back = parts - 1 - part;
+  const int l16 = lane & (LPR / 2 - 1), sub16 = lane / (LPR / 2);
+  const LanePieces piece = lane_pieces(a, l16);
+  const bool live16 = piece.b < a.dim, rotated = l16 < (a.rot >> 4);
+  const uint32_t stage1 = smem_u32(stage_s[warp]) + 16 * lane, stage2 = stage1 + 1024 * kRowStage;
+  const int step = parts * 2 * kRows;  // heads from set to set
+  auto stage_rows = [&](uint32_t st, const __nv_bfloat16* src, int h, int heads) {
+#pragma unroll
+    for (int i = 0; i < kRowStage; ++i, h += step)
+      if (live16 && h < heads) {
+        cp_async16(st + 1024 * i, src + h * a.dim + piece.a);
+        cp_async16(st + 1024 * i + 512, src + h * a.dim + piece.b);
+      }
+  };
+  auto turn_rows = [&](uint32_t st, __nv_bfloat16* dst, int h, int heads, const LaneTurn16& turn, bool norm, bool good) {
+#pragma unroll 1
+    for (int i = 0; i < kRowStage && h - sub16 < heads; ++i, h += step) {
+      const bool here = live16 && h < heads;
+      uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+      if (here && good) x[0] = lds128(st + 1024 * i), x[1] = lds128(st + 1024 * i + 512);
+      if (good) turn_row16<LPR, kInter>(a, x, turn, norm, rotated);
+      if (here) {
+        *reinterpret_cast<uint4*>(dst + h * a.dim + piece.a) = x[0];
+        *reinterpret_cast<uint4*>(dst + h * a.dim + piece.b) = x[1];
       }
     }
-  }
+  };
+  const __nv_bfloat16* q_src = a.q + a.q_stride * t;
+  const __nv_bfloat16* k_src = a.k + a.k_stride * t;
+  const __nv_bfloat16* v_src = a.v + a.v_stride * t;
+  const int q0 = part * 2 * kRows, k0 = back * 2 * kRows;  // first heads of the first sets
+  // for a cache: sets of kRows rows, k's and then v's
+  const int kv_sets = ceil_div(a.kv_heads, kRows);
+  auto coded = [&](int g, bool& value) {
+    value = g >= kv_sets;
+    return (value ? g - kv_sets : g) * kRows + sub;
+  };
+  auto stage_coded = [&](int g) {
+#pragma unroll
+    for (int i = 0; i < kRowStage; ++i, g += parts) {
+      bool value;
+      const int h = coded(g, value);
+      if (live && g < 2 * kv_sets && h < a.kv_heads) cp_async16(stage2 + 1024 * i, (value ? v_src : k_src) + h * a.dim + at);
+    }
+  };
+  stage_rows(stage1, q_src, q0 + sub16, a.q_heads);
+  if constexpr (kFmt == kFmtNone) stage_rows(stage2, k_src, k0 + sub16, a.kv_heads);
+  else stage_coded(back);
+  cp_async_commit();
+
+  const int p = a.rot && a.positions ? __ldg(a.positions + t) : t;
+  const bool good = !a.rot || (p >= 0 && p < a.table_rows);
+  if (!good && threadIdx.x == 0) record_error(kErrBadPosition);
   int slot = -1;
-  if (kFmt != kFmtNone) {
+  if constexpr (kFmt != kFmtNone) {
     slot = __ldg(a.slots + t);
     if (slot >= a.cache.slots()) {
       if (threadIdx.x == 0) record_error(kErrBadSlot);
@@ -239,45 +514,77 @@ __global__ void __launch_bounds__(kRowThreads) head_rows_kernel(const __grid_con
     }
     if (!good) slot = -1;
     bool later = false;
-    if (slot >= 0)
-      for (int u = blockIdx.x + 1 + threadIdx.x; u < gridDim.x; u += kRowThreads) later |= __ldg(a.slots + first + u) == slot;
+    if (slot >= 0) {
+#pragma unroll 4
+      for (int u = t + 1 + threadIdx.x; u < first + static_cast<int>(gridDim.x); u += kRowThreads) later |= __ldg(a.slots + u) == slot;
+    }
     if (__syncthreads_or(later)) slot = -1;
   }
-
-  const int q_groups = ceil_div(a.q_heads, kRows), kv_groups = ceil_div(a.kv_heads, kRows);
-  const int groups = q_groups + kv_groups * (kFmt != kFmtNone ? 2 : 1);
-  for (int g = warp; g < groups; g += warps) {
-    const int kind = g < q_groups ? 0 : (g < q_groups + kv_groups ? 1 : 2);
-    const int h = (kind == 0 ? g : kind == 1 ? g - q_groups : g - q_groups - kv_groups) * kRows + sub;
-    const int heads = kind == 0 ? a.q_heads : a.kv_heads;
-    const bool here = live && h < heads;
-    if (kFmt != kFmtNone && kind != 0 && slot < 0) continue;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (here) {
-      const __nv_bfloat16* src = kind == 0 ? a.q + a.q_stride * t : kind == 1 ? a.k + a.k_stride * t : a.v + a.v_stride * t;
-      x = *reinterpret_cast<const uint4*>(src + static_cast<size_t>(h) * a.dim + at);
-    }
-    if (kind == 0 || (kind == 1 && kFmt == kFmtNone)) {
-      float y[8];
-      norm_rotate<LPR, float>(a, x, kind == 0 ? a.q_weight : a.k_weight, c, s, y);
-      if (here) {
-        uint4 o = make_uint4(0, 0, 0, 0);
-        if (good)
-          o = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                         pack_bf16x2(y[6], y[7]));
-        __nv_bfloat16* dst = kind == 0 ? a.q_out : a.k_out;
-        *reinterpret_cast<uint4*>(dst + (static_cast<size_t>(t) * heads + h) * a.dim + at) = o;
+  if (q0 < a.q_heads) {
+    LaneTurn16 turn;
+    if (good) load_turn16<kInter>(a, p, a.q_weight, l16, turn);
+    cp_async_wait<0>();
+    __nv_bfloat16* dst = a.q_out + static_cast<size_t>(t) * a.q_heads * a.dim;
+    for (int h = q0; h < a.q_heads; h += kRowStage * step) {
+      if (h != q0) {
+        stage_rows(stage1, q_src, h + sub16, a.q_heads);
+        cp_async_commit();
+        cp_async_wait<0>();
       }
-    } else if (kFmt != kFmtNone) {
-      const size_t row = here ? a.cache.row(slot, h) : 0;
-      if (kind == 1) {
-        double y[8];
-        norm_rotate<LPR, double>(a, x, a.k_weight, c, s, y);
-        code_and_store<kFmt>(y, here, row, a.dim, at, a.cache.k_codes, a.cache.k_scales);
-      } else {
-        float y[8];
-        unpack_bf16x8(x, y);
-        code_and_store<kFmt>(y, here, row, a.dim, at, a.cache.v_codes, a.cache.v_scales);
+      turn_rows(stage1, dst, h + sub16, a.q_heads, turn, a.q_weight != nullptr, good);
+    }
+  }
+  cp_async_wait<0>();
+  if constexpr (kFmt == kFmtNone) {
+    if (k0 >= a.kv_heads) return;
+    LaneTurn16 turn;
+    if (good) load_turn16<kInter>(a, p, a.k_weight, l16, turn);
+    __nv_bfloat16* dst = a.k_out + static_cast<size_t>(t) * a.kv_heads * a.dim;
+    for (int h = k0; h < a.kv_heads; h += kRowStage * step) {
+      if (h != k0) {
+        stage_rows(stage2, k_src, h + sub16, a.kv_heads);
+        cp_async_commit();
+        cp_async_wait<0>();
+      }
+      turn_rows(stage2, dst, h + sub16, a.kv_heads, turn, a.k_weight != nullptr, good);
+    }
+  } else {
+    if (slot < 0) return;
+    const bool turned = a.rot || a.k_weight;
+    for (int g0 = back; g0 < 2 * kv_sets; g0 += kRowStage * parts) {
+      if (g0 != back) {
+        stage_coded(g0);
+        cp_async_commit();
+        cp_async_wait<0>();
+      }
+      float cw[8], sw[8];
+      if (turned && g0 < kv_sets) {
+        LaneTurn q;
+        load_turn<LPR, kInter>(a, p, a.k_weight, q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) cw[j] = q.c[j] * q.w[j], sw[j] = q.s[j] * q.wp[j];
+      }
+      uint32_t open = 0;  // sets whose codes 32 bits did not settle
+#pragma unroll 1
+      for (int i = 0, g = g0; i < kRowStage && g < 2 * kv_sets; ++i, g += parts) {
+        bool value;
+        const int h = coded(g, value);
+        const bool here = live && h < a.kv_heads;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (here) x = lds128(stage2 + 1024 * i);
+        const size_t row = here ? a.cache.row(slot, h) : 0;
+        if (!value && turned) {
+          if (!store_keys<LPR, kFmt, kInter>(a, x, cw, sw, here, row, at)) open |= 1u << i;
+        } else {
+          float f[8];
+          unpack_bf16x8(x, f);
+          code_and_store<kFmt>(a.cache, !value, f, here, row, at);
+        }
+      }
+      while (open) {  // nothing is kept over the call
+        const int i = __ffs(open) - 1;
+        open &= open - 1;
+        store_keys_exact<LPR, kFmt, kInter>(&a, t, p, slot, (g0 + i * parts) * kRows);
       }
     }
   }

@@ -689,37 +689,42 @@ int cache_view(const mxfp4_kv_cache* c, KvCacheView* v, int* fmt) {
 // Tokens per launch of a storing pass: every block looks through the slots behind its own.
 constexpr int kStoreTokens = 4096;
 
-template <int LPR, int kFmt>
+template <int LPR, int kFmt, bool kInter>
 int launch_head_rows(const RowArgs& a, cudaStream_t s, const DeviceState* d) {
   constexpr int rows = 32 / LPR;
-  const int groups = ceil_div(a.q_heads, rows) + ceil_div(a.kv_heads, rows) * (kFmt == kFmtNone ? 1 : 2);
+  const int sets = ceil_div(a.q_heads, 2 * rows) + (kFmt == kFmtNone ? ceil_div(a.kv_heads, 2 * rows) : 2 * ceil_div(a.kv_heads, rows));
   const int most = kFmt == kFmtNone ? a.tokens : kStoreTokens;
   for (int first = 0; first < a.tokens; first += most) {
     const int n = std::min(most, a.tokens - first);
     // few tokens: their rows are spread over blocks until the SMs have eight each
-    const int per_block = kRowThreads / 32;
-    const int y = std::max(1, std::min(ceil_div(groups, per_block), ceil_div(8 * d->sm_count, n)));
-    head_rows_kernel<LPR, kFmt><<<dim3(n, y), kRowThreads, 0, s>>>(a, first);
+    const int y = std::max(1, std::min(ceil_div(sets, kRowThreads / 32), 8 * d->sm_count / n));
+    head_rows_kernel<LPR, kFmt, kInter><<<dim3(n, y), kRowThreads, 0, s>>>(a, first);
     const int rc = launch_status();
     if (rc) return rc;
+    if (a.tokens - first <= most) break;  // first + most may pass the int range
   }
   return 0;
 }
 
-template <int kFmt>
+template <int kFmt, bool kInter>
 int launch_head_rows_dim(const RowArgs& a, cudaStream_t s) {
   DeviceState* d = nullptr;
   const int rc = current_device(&d);
   if (rc) return rc;
-  if (a.dim <= 32) return launch_head_rows<4, kFmt>(a, s, d);
-  if (a.dim <= 64) return launch_head_rows<8, kFmt>(a, s, d);
-  if (a.dim <= 128) return launch_head_rows<16, kFmt>(a, s, d);
-  return launch_head_rows<32, kFmt>(a, s, d);
+  if (a.dim <= 32) return launch_head_rows<4, kFmt, kInter>(a, s, d);
+  if (a.dim <= 64) return launch_head_rows<8, kFmt, kInter>(a, s, d);
+  if (a.dim <= 128) return launch_head_rows<16, kFmt, kInter>(a, s, d);
+  return launch_head_rows<32, kFmt, kInter>(a, s, d);
+}
+int launch_head_rows_any(const RowArgs& a, int fmt, int interleaved, cudaStream_t s) {
+  if (fmt == kFmtNone) return interleaved ? launch_head_rows_dim<kFmtNone, true>(a, s) : launch_head_rows_dim<kFmtNone, false>(a, s);
+  if (fmt == kFmtE4M3) return interleaved ? launch_head_rows_dim<kFmtE4M3, true>(a, s) : launch_head_rows_dim<kFmtE4M3, false>(a, s);
+  return interleaved ? launch_head_rows_dim<kFmtE2M1, true>(a, s) : launch_head_rows_dim<kFmtE2M1, false>(a, s);
 }
 
 // Checks what the two norm-and-rotation entry points share and fills the arguments.
 int rope_args(RowArgs* a, const void* qkv, long long row_stride, int tokens, int q_heads, int kv_heads, int dim,
-              const float* cos, const float* sin, int table_rows, int rot, int interleaved, const int* positions,
+              const float* cos, const float* sin, int table_rows, int rot, const int* positions,
               const void* q_weight, const void* k_weight, int weight_dtype, double eps, void* q_out) {
   if (tokens < 0 || q_heads <= 0 || kv_heads <= 0 || dim <= 0 || rot < 0) return MXFP4_ERR_INVALID_ARGUMENT;
   if (tokens > 0 && (!qkv || !q_out)) return MXFP4_ERR_INVALID_ARGUMENT;
@@ -739,9 +744,9 @@ int rope_args(RowArgs* a, const void* qkv, long long row_stride, int tokens, int
   a->v = a->k + static_cast<size_t>(kv_heads) * dim;
   a->q_stride = a->k_stride = a->v_stride = row_stride;
   a->tokens = tokens, a->q_heads = q_heads, a->kv_heads = kv_heads, a->dim = dim;
-  a->cos = cos, a->sin = sin, a->table_rows = table_rows, a->rot = rot, a->interleaved = interleaved != 0;
+  a->cos = cos, a->sin = sin, a->table_rows = table_rows, a->rot = rot;
   a->positions = positions, a->q_weight = q_weight, a->k_weight = k_weight;
-  a->weight_f32 = weight_dtype == MXFP4_DTYPE_F32, a->eps = eps;
+  a->weight_f32 = weight_dtype == MXFP4_DTYPE_F32, a->eps = eps, a->inv_dim = 1.0 / dim;
   a->q_out = static_cast<__nv_bfloat16*>(q_out);
   return 0;
 }
@@ -1042,13 +1047,13 @@ int mxfp4_qk_norm_rope(const void* qkv, long long row_stride, int tokens, int nu
                        double eps, void* q_out, void* k_out, void* stream) {
   RowArgs a;
   const int rc = rope_args(&a, qkv, row_stride, tokens, num_heads, num_kv_heads, head_dim, cos, sin, table_rows, rot,
-                           interleaved, positions, q_weight, k_weight, weight_dtype, eps, q_out);
+                           positions, q_weight, k_weight, weight_dtype, eps, q_out);
   if (rc) return rc;
   if (tokens == 0) return 0;
   if (!k_out) return MXFP4_ERR_INVALID_ARGUMENT;
   if (!aligned16(k_out)) return MXFP4_ERR_MISALIGNED;
   a.k_out = static_cast<__nv_bfloat16*>(k_out);
-  return launch_head_rows_dim<kFmtNone>(a, static_cast<cudaStream_t>(stream));
+  return launch_head_rows_any(a, kFmtNone, interleaved, static_cast<cudaStream_t>(stream));
 }
 
 int mxfp4_qk_norm_rope_cache(const void* qkv, long long row_stride, int tokens, int num_heads, const float* cos,
@@ -1060,15 +1065,14 @@ int mxfp4_qk_norm_rope_cache(const void* qkv, long long row_stride, int tokens, 
   int rc = cache_view(cache, &c, &fmt);
   if (rc) return rc;
   RowArgs a;
-  rc = rope_args(&a, qkv, row_stride, tokens, num_heads, c.heads, c.dim, cos, sin, table_rows, rot, interleaved,
-                 positions, q_weight, k_weight, weight_dtype, eps, q_out);
+  rc = rope_args(&a, qkv, row_stride, tokens, num_heads, c.heads, c.dim, cos, sin, table_rows, rot, positions,
+                 q_weight, k_weight, weight_dtype, eps, q_out);
   if (rc) return rc;
   if (tokens == 0) return 0;
   if (!slots) return MXFP4_ERR_INVALID_ARGUMENT;
   a.cache = c;
   a.slots = slots;
-  auto s = static_cast<cudaStream_t>(stream);
-  return fmt == kFmtE4M3 ? launch_head_rows_dim<kFmtE4M3>(a, s) : launch_head_rows_dim<kFmtE2M1>(a, s);
+  return launch_head_rows_any(a, fmt, interleaved, static_cast<cudaStream_t>(stream));
 }
 
 int mxfp4_kv_cache_write(const mxfp4_kv_cache* cache, const void* k, long long k_stride, const void* v,
@@ -1087,8 +1091,7 @@ int mxfp4_kv_cache_write(const mxfp4_kv_cache* cache, const void* k, long long k
   a.k_stride = k_stride, a.v_stride = v_stride;
   a.tokens = tokens, a.kv_heads = a.cache.heads, a.dim = a.cache.dim;
   a.slots = slots;
-  auto s = static_cast<cudaStream_t>(stream);
-  return fmt == kFmtE4M3 ? launch_head_rows_dim<kFmtE4M3>(a, s) : launch_head_rows_dim<kFmtE2M1>(a, s);
+  return launch_head_rows_any(a, fmt, 0, static_cast<cudaStream_t>(stream));
 }
 
 int mxfp4_kv_cache_read(const mxfp4_kv_cache* cache, const int* slots, int tokens, void* k, void* v, void* stream) {

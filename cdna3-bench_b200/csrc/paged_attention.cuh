@@ -178,15 +178,6 @@ __device__ __forceinline__ constexpr int attn_swizzle(int r) {
   }
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Copies the 16 keys of a tile into shared memory at dst (one warp): codes from k and v, scales
 // from sc, each with the lane's own offset already in it.  base_k and base_v: the lane's first
 // place in the tile; a later one differs by whole rows and, as the swizzle is linear over xor in

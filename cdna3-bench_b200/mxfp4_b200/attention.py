@@ -27,33 +27,25 @@ KV_FORMATS = {"mxfp8": _lib.KV_MXFP8, "mxfp4": _lib.KV_MXFP4}
 _PAGE_SIZES = (16, 32, 64, 128, 256)
 
 # A decoding step calls these with GPU work of a few microseconds, so the checks are plain conditions
-# (a message is only made for a call that is refused) and the stream is asked for by device index.
+# (a message is only made for a call that is refused), devices are compared by index (-1: the CPU)
+# and the current stream is asked for by index.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_device = torch.cuda.current_device
 _BF16, _F32, _I32, _Tensor = torch.bfloat16, torch.float32, torch.int32, torch.Tensor
 
 
-def _call(device: torch.device, what: str, fn, *args):
-    """One C entry on `device`'s current stream, with `device` current."""
-    i = device.index
-    if i == torch.cuda.current_device():
-        code = fn(*args, _raw_stream(i))
-    else:
-        with torch.cuda.device(i):
-            code = fn(*args, _raw_stream(i))
-    if code:
-        _lib.check(code, what)
+def _on_device(index: int, fn, *args) -> int:
+    """fn(*args, stream) with device `index`, which is not the current one, made current."""
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
 
 
-def _index(t, n: int, device, what: str) -> int:
-    """Address of an int32 vector of n on `device`."""
-    if not (isinstance(t, _Tensor) and t.dtype is _I32 and t.device == device and t.dim() == 1 and t.shape[0] == n
+def _index(t, n: int, dev: int, what: str) -> int:
+    """Address of an int32 vector of n on device `dev`."""
+    if not (isinstance(t, _Tensor) and t.dtype is _I32 and t.get_device() == dev and t.dim() == 1 and t.shape[0] == n
             and (n < 2 or t.stride(0) == 1)):
-        raise RuntimeError(f"{what} must be a contiguous int32 vector of {n} on {device}")
+        raise RuntimeError(f"{what} must be a contiguous int32 vector of {n} on cuda:{dev}")
     return t.data_ptr()
-
-
-def _is_bf16(t, device=None) -> bool:
-    return isinstance(t, _Tensor) and t.dtype is _BF16 and (t.is_cuda if device is None else t.device == device)
 
 
 class MXKVCache:
@@ -67,7 +59,7 @@ class MXKVCache:
     """
 
     __slots__ = ("k_codes", "v_codes", "k_scales", "v_scales", "format", "num_pages", "num_kv_heads", "page_size",
-                 "head_dim", "device", "_struct", "_ref")
+                 "head_dim", "device", "_index", "_struct", "_ref")
 
     def __init__(self, k_codes, v_codes, k_scales, v_scales, format: str = "mxfp8"):
         _check(format in KV_FORMATS, "format must be 'mxfp8' or 'mxfp4'")
@@ -85,6 +77,7 @@ class MXKVCache:
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
         self.format, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = format, pages, heads, size, dim
         self.device = k_codes.device
+        self._index = k_codes.get_device()
         self._struct = _lib.KVCache(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                                     pages, heads, size, dim, KV_FORMATS[format])
         self._ref = ctypes.byref(self._struct)
@@ -105,23 +98,25 @@ def new_kv_cache(num_pages: int, num_kv_heads: int, head_dim: int, page_size: in
 
 
 def _rope_arguments(qkv, heads, kv_heads, dim, cos, sin, positions, q_weight, k_weight):
-    """Checks what the two norm-and-rotation calls share; the arguments of the C entry from cos to
-    weight_dtype, with the interleaved flag left out, and qkv's row stride."""
-    if not (_is_bf16(qkv) and qkv.dim() == 2 and qkv.stride(1) == 1):
+    """Checks what the two norm-and-rotation calls share.  Returns tokens, the device's index, qkv's row
+    stride, and the C entry's cos, sin, table_rows, rot, positions, q_weight, k_weight, weight_dtype."""
+    if not (isinstance(qkv, _Tensor) and qkv.dtype is _BF16 and qkv.dim() == 2 and qkv.stride(1) == 1):
         raise RuntimeError("qkv must be bfloat16 [tokens, width] on the GPU with contiguous rows")
     tokens, width = qkv.shape
-    if not (heads > 0 and kv_heads > 0 and width == (heads + 2 * kv_heads) * dim):
-        raise RuntimeError("qkv's width must be (num_heads + 2 * num_kv_heads) * head_dim")
-    dev = qkv.device
+    dev = qkv.get_device()
+    if dev < 0 or heads <= 0 or kv_heads <= 0 or width != (heads + 2 * kv_heads) * dim:
+        raise RuntimeError("qkv must be on the GPU, its width (num_heads + 2 * num_kv_heads) * head_dim")
     rows = rot = cp = sp = pos = qw = kw = 0
     wt = _lib.DTYPE_BF16
     if cos is not None or sin is not None:
         if not (isinstance(cos, _Tensor) and isinstance(sin, _Tensor) and cos.dtype is _F32 and sin.dtype is _F32
-                and cos.device == dev and sin.device == dev and cos.dim() == 2 and cos.shape == sin.shape
-                and cos.is_contiguous() and sin.is_contiguous() and cos.numel() > 0):
-            raise RuntimeError(f"cos and sin must be contiguous float32 [rows, rot / 2] of one shape on {dev}")
+                and cos.get_device() == dev and sin.get_device() == dev and cos.dim() == 2 and cos.shape == sin.shape
+                and cos.is_contiguous() and sin.is_contiguous()):
+            raise RuntimeError(f"cos and sin must be contiguous float32 [rows, rot / 2] of one shape on cuda:{dev}")
         rows, rot = cos.shape
         rot *= 2
+        if rows == 0 or rot == 0:
+            raise RuntimeError("cos and sin must not be empty")
         cp, sp = cos.data_ptr(), sin.data_ptr()
     if positions is not None:
         if not rot:
@@ -131,14 +126,15 @@ def _rope_arguments(qkv, heads, kv_heads, dim, cos, sin, positions, q_weight, k_
         raise RuntimeError("cos and sin need a row per token when no positions are given")
     if q_weight is not None or k_weight is not None:
         for w in (q_weight, k_weight):
-            if not (isinstance(w, _Tensor) and w.device == dev and w.dtype in (_BF16, _F32) and w.shape == (dim,) and w.is_contiguous()):
-                raise RuntimeError(f"q_weight and k_weight come together, contiguous bfloat16 or float32 [head_dim] on {dev}")
+            if not (isinstance(w, _Tensor) and w.get_device() == dev and w.dtype in (_BF16, _F32) and w.dim() == 1
+                    and w.shape[0] == dim and w.is_contiguous()):
+                raise RuntimeError(f"q_weight and k_weight come together, contiguous bfloat16 or float32 [head_dim] on cuda:{dev}")
         if q_weight.dtype is not k_weight.dtype:
             raise RuntimeError("q_weight and k_weight must have one type")
         qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
         if q_weight.dtype is _F32:
             wt = _lib.DTYPE_F32
-    return tokens, dev, qkv.stride(0) if tokens > 1 else width, (cp, sp, rows, rot), (pos, qw, kw, wt)
+    return tokens, dev, qkv.stride(0) if tokens > 1 else width, cp, sp, rows, rot, pos, qw, kw, wt
 
 
 def qk_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos=None, sin=None, positions=None, q_weight=None,
@@ -157,10 +153,15 @@ def qk_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos=None, sin=None, pos
     if not (isinstance(qkv, _Tensor) and qkv.dim() == 2 and num_heads > 0 and num_kv_heads > 0):
         raise RuntimeError("qkv must be bfloat16 [tokens, width] on the GPU with contiguous rows")
     dim = qkv.shape[1] // (num_heads + 2 * num_kv_heads)
-    tokens, dev, stride, table, rest = _rope_arguments(qkv, num_heads, num_kv_heads, dim, cos, sin, positions, q_weight, k_weight)
+    tokens, dev, stride, cp, sp, rows, rot, pos, qw, kw, wt = _rope_arguments(
+        qkv, num_heads, num_kv_heads, dim, cos, sin, positions, q_weight, k_weight)
     q, k = qkv.new_empty((tokens, num_heads, dim)), qkv.new_empty((tokens, num_kv_heads, dim))
-    _call(dev, "mxfp4_qk_norm_rope", _lib.lib().mxfp4_qk_norm_rope, qkv.data_ptr(), stride, tokens, num_heads, num_kv_heads,
-          dim, *table, bool(interleaved), *rest, eps, q.data_ptr(), k.data_ptr())
+    fn = _lib.lib().mxfp4_qk_norm_rope
+    args = (qkv.data_ptr(), stride, tokens, num_heads, num_kv_heads, dim, cp, sp, rows, rot, interleaved, pos, qw, kw, wt, eps,
+            q.data_ptr(), k.data_ptr())
+    code = fn(*args, _raw_stream(dev)) if dev == _device() else _on_device(dev, fn, *args)
+    if code:
+        _lib.check(code, "mxfp4_qk_norm_rope")
     return q, k
 
 
@@ -176,20 +177,25 @@ def qk_norm_rope_cache(qkv, num_heads: int, num_kv_heads: int, cos, sin, cache: 
     if not (isinstance(cache, MXKVCache) and num_kv_heads == cache.num_kv_heads):
         raise RuntimeError("cache must be an MXKVCache of num_kv_heads heads")
     dim = cache.head_dim
-    tokens, dev, stride, table, rest = _rope_arguments(qkv, num_heads, num_kv_heads, dim, cos, sin, positions, q_weight, k_weight)
-    if dev != cache.device:
+    tokens, dev, stride, cp, sp, rows, rot, pos, qw, kw, wt = _rope_arguments(
+        qkv, num_heads, num_kv_heads, dim, cos, sin, positions, q_weight, k_weight)
+    if dev != cache._index:
         raise RuntimeError("qkv must be on the cache's GPU")
     at = _index(slots, tokens, dev, "slots")
     q = qkv.new_empty((tokens, num_heads, dim))
-    _call(dev, "mxfp4_qk_norm_rope_cache", _lib.lib().mxfp4_qk_norm_rope_cache, qkv.data_ptr(), stride, tokens, num_heads,
-          *table, bool(interleaved), *rest, eps, q.data_ptr(), cache._ref, at)
+    fn = _lib.lib().mxfp4_qk_norm_rope_cache
+    args = (qkv.data_ptr(), stride, tokens, num_heads, cp, sp, rows, rot, interleaved, pos, qw, kw, wt, eps, q.data_ptr(),
+            cache._ref, at)
+    code = fn(*args, _raw_stream(dev)) if dev == _device() else _on_device(dev, fn, *args)
+    if code:
+        _lib.check(code, "mxfp4_qk_norm_rope_cache")
     return q
 
 
 def _row_stride(t, cache, tokens, what):
     heads, dim = cache.num_kv_heads, cache.head_dim
-    if not (_is_bf16(t, cache.device) and t.shape == (tokens, heads, dim) and t.stride(2) == 1
-            and (heads == 1 or t.stride(1) == dim)):
+    if not (isinstance(t, _Tensor) and t.dtype is _BF16 and t.get_device() == cache._index and t.shape == (tokens, heads, dim)
+            and t.stride(2) == 1 and (heads == 1 or t.stride(1) == dim)):
         raise RuntimeError(f"{what} must be bfloat16 [tokens, num_kv_heads, head_dim] on the cache's GPU, a token's heads contiguous")
     return t.stride(0) if tokens > 1 else heads * dim
 
@@ -201,11 +207,13 @@ def kv_cache_write(cache: MXKVCache, k, v, slots) -> None:
     ``quantize_mxfp4(..., rule="ocp")`` and :func:`quantize_act_mx8`."""
     if not (isinstance(cache, MXKVCache) and isinstance(k, _Tensor) and k.dim() == 3):
         raise RuntimeError("cache must be an MXKVCache, k [tokens, num_kv_heads, head_dim]")
-    tokens = k.shape[0]
+    tokens, dev = k.shape[0], cache._index
     ks, vs = _row_stride(k, cache, tokens, "k"), _row_stride(v, cache, tokens, "v")
-    at = _index(slots, tokens, cache.device, "slots")
-    _call(cache.device, "mxfp4_kv_cache_write", _lib.lib().mxfp4_kv_cache_write, cache._ref, k.data_ptr(), ks, v.data_ptr(), vs,
-          at, tokens)
+    fn = _lib.lib().mxfp4_kv_cache_write
+    args = (cache._ref, k.data_ptr(), ks, v.data_ptr(), vs, _index(slots, tokens, dev, "slots"), tokens)
+    code = fn(*args, _raw_stream(dev)) if dev == _device() else _on_device(dev, fn, *args)
+    if code:
+        _lib.check(code, "mxfp4_kv_cache_write")
 
 
 def kv_cache_read(cache: MXKVCache, slots):
@@ -213,11 +221,15 @@ def kv_cache_read(cache: MXKVCache, slots):
     head_dim]``; a negative slot reads zeros, the scale byte 255 NaN."""
     if not (isinstance(cache, MXKVCache) and isinstance(slots, _Tensor) and slots.dim() == 1):
         raise RuntimeError("cache must be an MXKVCache, slots a vector")
-    tokens, dev = slots.shape[0], cache.device
+    tokens, dev = slots.shape[0], cache._index
     at = _index(slots, tokens, dev, "slots")
     shape = (tokens, cache.num_kv_heads, cache.head_dim)
     k, v = slots.new_empty(shape, dtype=_BF16), slots.new_empty(shape, dtype=_BF16)
-    _call(dev, "mxfp4_kv_cache_read", _lib.lib().mxfp4_kv_cache_read, cache._ref, at, tokens, k.data_ptr(), v.data_ptr())
+    fn = _lib.lib().mxfp4_kv_cache_read
+    args = (cache._ref, at, tokens, k.data_ptr(), v.data_ptr())
+    code = fn(*args, _raw_stream(dev)) if dev == _device() else _on_device(dev, fn, *args)
+    if code:
+        _lib.check(code, "mxfp4_kv_cache_read")
     return k, v
 
 
@@ -236,30 +248,36 @@ def paged_attention(q, cache: MXKVCache, page_table, lengths, scale: float | Non
     """
     if not isinstance(cache, MXKVCache):
         raise RuntimeError("cache must be an MXKVCache")
-    dev, dim, kv_heads = cache.device, cache.head_dim, cache.num_kv_heads
-    if not (_is_bf16(q, dev) and q.dim() == 3 and q.shape[2] == dim and q.stride(2) == 1):
+    dev, dim = cache._index, cache.head_dim
+    if not (isinstance(q, _Tensor) and q.dtype is _BF16 and q.get_device() == dev and q.dim() == 3):
         raise RuntimeError("q must be bfloat16 [seqs, num_heads, head_dim] on the cache's GPU")
-    seqs, heads, _ = q.shape
-    if heads == 0 or heads % kv_heads or (heads > 1 and q.stride(1) != dim):
+    seqs, heads, width = q.shape
+    row, step, one = q.stride()
+    if width != dim or one != 1 or heads == 0 or heads % cache.num_kv_heads or (step != dim and heads > 1):
         raise RuntimeError("q: num_heads must be a multiple of num_kv_heads, a sequence's heads contiguous")
-    if not (isinstance(page_table, _Tensor) and page_table.dtype is _I32 and page_table.device == dev and page_table.dim() == 2):
+    if not (isinstance(page_table, _Tensor) and page_table.dtype is _I32 and page_table.get_device() == dev and page_table.dim() == 2):
         raise RuntimeError("page_table must be int32 [seqs, max_pages] on the cache's GPU")
     rows, pages = page_table.shape
-    if rows != seqs or pages == 0 or (pages > 1 and page_table.stride(1) != 1):
+    table_row, one = page_table.stride()
+    if rows != seqs or pages == 0 or (one != 1 and pages > 1):
         raise RuntimeError("page_table must be [seqs, max_pages] with contiguous rows")
     lens = _index(lengths, seqs, dev, "lengths")
-    scale = dim ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
+    if scale is None:
+        scale = dim ** -0.5
+    elif not math.isfinite(scale):
         raise RuntimeError("scale must be finite")
     if out is None:
         out = q.new_empty((seqs, heads, dim))
-    elif not (_is_bf16(out, dev) and out.shape == (seqs, heads, dim) and out.is_contiguous()):
+    elif not (isinstance(out, _Tensor) and out.dtype is _BF16 and out.get_device() == dev and out.shape == q.shape and out.is_contiguous()):
         raise RuntimeError("out must be contiguous bfloat16 [seqs, num_heads, head_dim] on the cache's GPU")
     lse = q.new_empty((seqs, heads), dtype=_F32) if return_lse else None
     L = _lib.lib()
     nws = L.mxfp4_paged_attention_workspace_bytes(cache._ref, seqs, heads, pages)
     ws = q.new_empty(nws // 2)
-    _call(dev, "mxfp4_paged_attention", L.mxfp4_paged_attention, q.data_ptr(), q.stride(0) if seqs > 1 else heads * dim, cache._ref,
-          page_table.data_ptr(), page_table.stride(0) if seqs > 1 else pages, pages, lens, seqs, heads, scale, out.data_ptr(),
-          lse.data_ptr() if return_lse else 0, ws.data_ptr(), nws)
+    fn = L.mxfp4_paged_attention
+    args = (q.data_ptr(), row if seqs > 1 else heads * dim, cache._ref, page_table.data_ptr(), table_row if seqs > 1 else pages, pages,
+            lens, seqs, heads, scale, out.data_ptr(), lse.data_ptr() if return_lse else 0, ws.data_ptr(), nws)
+    code = fn(*args, _raw_stream(dev)) if dev == _device() else _on_device(dev, fn, *args)
+    if code:
+        _lib.check(code, "mxfp4_paged_attention")
     return (out, lse) if return_lse else out
