@@ -253,8 +253,9 @@ def test_same_slot_twice_keeps_the_later_token(mx, tokens):
     k, v = bf16(rng, (tokens, 2, 64)), bf16(rng, (tokens, 2, 64))
     slots = rng.integers(0, 64, tokens)
     slots[0] = slots[-1]
-    for _ in range(3):
-        mx.kv_cache_write(cache, k, v, i32(slots))
+    for shift in (0, 1, 2):  # vectors of slots that start at any address
+        pad = i32(np.r_[np.full(shift, 7), slots])
+        mx.kv_cache_write(cache, k, v, pad[shift:])
         last = {int(s): t for t, s in enumerate(slots)}
         at = np.array(sorted(last))
         rk, rv = mx.kv_cache_read(cache, i32(at))
