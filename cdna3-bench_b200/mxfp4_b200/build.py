@@ -3,7 +3,10 @@
     python -m mxfp4_b200.build [--force]
 
 One nvcc invocation over csrc/mxfp4_b200.cu (a single translation unit that includes the
-kernels); the static CUDA runtime keeps the library independent of torch's runtime copy.
+kernels); the static CUDA runtime keeps the library independent of torch's runtime copy.  Beside
+it the host compiler builds ``_attention.so`` from csrc/attention_binding.cpp, the Python binding of
+the attention operators against torch's C++ headers (it holds no kernels and finds the library's
+entries at run time).
 """
 
 from __future__ import annotations
@@ -13,12 +16,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(ROOT, "csrc")
 INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 OUT = os.path.join(PKG_DIR, "libmxfp4_b200.so")
+BINDING = os.path.join(CSRC, "attention_binding.cpp")
+BINDING_OUT = os.path.join(PKG_DIR, "_attention.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -41,14 +47,37 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(OUT):
+def up_to_date(out: str = OUT, of=None) -> bool:
+    if not os.path.exists(out):
         return False
-    t = os.path.getmtime(OUT)
-    return all(os.path.getmtime(s) <= t for s in sources())
+    t = os.path.getmtime(out)
+    return all(os.path.getmtime(s) <= t for s in of or sources())
+
+
+def build_binding(force: bool = False) -> str:
+    """_attention.so; torch's own libraries are already loaded when it is imported."""
+    if not force and up_to_date(BINDING_OUT, (BINDING, os.path.join(INCLUDE, "mxfp4_b200.h"))):
+        return BINDING_OUT
+    import torch
+
+    home = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-isystem", os.path.join(home, "include"), "-isystem", os.path.join(home, "include", "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
+           "-o", BINDING_OUT + ".tmp", BINDING,
+           "-L" + os.path.join(home, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("the host compiler failed building _attention.so")
+    os.replace(BINDING_OUT + ".tmp", BINDING_OUT)
+    return BINDING_OUT
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    build_binding(force)
     if not force and up_to_date():
         return OUT
     cmd = [nvcc(), *NVCC_FLAGS, "-o", OUT + ".tmp", os.path.join(CSRC, "mxfp4_b200.cu")]
