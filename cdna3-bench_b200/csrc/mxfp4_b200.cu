@@ -754,17 +754,18 @@ int rope_args(RowArgs* a, const void* qkv, long long row_stride, int tokens, int
 // Blocks of the attention kernel: as many as are resident together.  kResident is the kernel's
 // launch bound, so this needs no query and holds without a device (148 SMs then).
 struct AttnPlan {
-  int nt, chunks, blocks;
+  int nt, chunks, blocks, unit_keys;
   size_t bytes;
 };
-AttnPlan attn_plan(int dim, int kv_heads, int q_heads, int seqs, int max_pages, int page_size, int sm_count) {
+AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int max_pages, int page_size, int sm_count) {
   AttnPlan p;
   const int group = q_heads / kv_heads;
   p.nt = group > 8 && dim < 256 ? 2 : 1;  // two operand tiles of 8 heads fit the registers below D = 256
   p.chunks = ceil_div(group, 8 * p.nt);
   const long long keys = static_cast<long long>(max_pages) * page_size;
-  const long long units = (keys + kAttnUnitKeys - 1) / kAttnUnitKeys * seqs * kv_heads * p.chunks;
-  p.blocks = static_cast<int>(std::min<long long>(std::max<long long>(units, 1), 1ll * sm_count * attn_resident(dim, p.nt)));
+  p.unit_keys = attn_unit_keys(dim, fmt);
+  const long long units = (keys + p.unit_keys - 1) / p.unit_keys * seqs * kv_heads * p.chunks;
+  p.blocks = static_cast<int>(std::min<long long>(std::max<long long>(units, 1), 1ll * sm_count * attn_resident(dim, fmt, p.nt)));
   p.bytes = static_cast<size_t>(p.blocks) * 2 * 8 * p.nt * (dim + 2) * sizeof(float);
   return p;
 }
@@ -1120,7 +1121,7 @@ size_t mxfp4_paged_attention_workspace_bytes(const mxfp4_kv_cache* cache, int se
   if (cache_view(cache, &c, &fmt) || seqs <= 0 || num_heads <= 0 || num_heads % c.heads || max_pages <= 0) return 0;
   DeviceState* d = nullptr;
   const int sms = current_device(&d) == 0 ? d->sm_count : 148;
-  return attn_plan(c.dim, c.heads, num_heads, seqs, max_pages, cache->page_size, sms).bytes;
+  return attn_plan(c.dim, fmt, c.heads, num_heads, seqs, max_pages, cache->page_size, sms).bytes;
 }
 
 int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cache* cache, const int* page_table,
@@ -1141,14 +1142,14 @@ int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cach
   DeviceState* d = nullptr;
   rc = current_device(&d);
   if (rc) return rc;
-  const AttnPlan p = attn_plan(a.cache.dim, a.cache.heads, num_heads, seqs, max_pages, cache->page_size, d->sm_count);
+  const AttnPlan p = attn_plan(a.cache.dim, fmt, a.cache.heads, num_heads, seqs, max_pages, cache->page_size, d->sm_count);
   if (!workspace || workspace_bytes < p.bytes) return MXFP4_ERR_WORKSPACE;
   a.q = static_cast<const __nv_bfloat16*>(q), a.q_stride = q_stride;
   a.table = page_table, a.table_stride = page_stride, a.max_pages = max_pages;
   a.lengths = lengths, a.seqs = seqs, a.q_heads = num_heads, a.group = num_heads / a.cache.heads, a.chunks = p.chunks;
   a.scale = scale;
   a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
-  a.parts = static_cast<float*>(workspace), a.blocks = p.blocks;
+  a.parts = static_cast<float*>(workspace), a.blocks = p.blocks, a.unit_keys = p.unit_keys;
   auto s = static_cast<cudaStream_t>(stream);
   return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p.nt, d, s) : launch_attention_dim<kFmtE2M1>(a, p.nt, d, s);
 }

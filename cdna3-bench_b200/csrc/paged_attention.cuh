@@ -25,7 +25,7 @@
 //           The transposition between S^T's accumulators and P^T's operand is one
 //           movmatrix per 8 keys.
 //
-// The sequences are cut into units of 4 warps * KT tiles; every block takes an equal, contiguous
+// The sequences are cut into units of kAttnWarps * attn_tiles tiles; every block takes an equal, contiguous
 // share of all units in (sequence, kv head, head chunk) order, whatever the lengths are (they are
 // read on the device).  A head whose units lie in one block is written at once; the parts of the
 // others go to the workspace and attn_join_kernel adds them in the blocks' order.
@@ -41,20 +41,22 @@ namespace mxb {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr int kAttnUnitKeys = 16 * kAttnWarps;  // one tile of 16 keys per warp
 
-// Blocks resident per SM (the kernel's launch bound) and tiles in a warp's ring.
-__host__ __device__ constexpr int attn_resident(int dim, int nt) {
-  return dim == 256 ? 2 : (nt == 2 ? 3 : (dim == 128 ? 4 : 5));
+// Tiles of 16 keys a warp takes in one step; steps in its ring; blocks resident per SM (the kernel's
+// launch bound).
+__host__ __device__ constexpr int attn_tiles(int dim, int fmt) { return dim == 256 && fmt == kFmtE4M3 ? 1 : 2; }
+__host__ __device__ constexpr int attn_ring(int dim, int fmt) { return (dim == 256 && fmt == kFmtE4M3) || dim == 64 ? 3 : 2; }
+__host__ __device__ constexpr int attn_resident(int dim, int fmt, int nt) {
+  return dim == 256 ? 2 : (nt == 2 ? 3 : (dim == 128 ? (fmt == kFmtE4M3 ? 3 : 4) : 4));
 }
-__host__ __device__ constexpr int attn_ring(int dim, int fmt) { return fmt == kFmtE4M3 && dim >= 128 ? 3 : 4; }
+__host__ __device__ constexpr int attn_unit_keys(int dim, int fmt) { return 16 * kAttnWarps * attn_tiles(dim, fmt); }
 __host__ __device__ constexpr int attn_row_bytes(int dim, int fmt) { return fmt == kFmtE4M3 ? dim : dim / 2; }
 // K codes, V codes, K scales, V scales of 16 keys
 __host__ __device__ constexpr int attn_tile_bytes(int dim, int fmt) {
   return 16 * 2 * (attn_row_bytes(dim, fmt) + dim / 32);
 }
 __host__ __device__ constexpr int attn_smem_bytes(int dim, int fmt, int nt) {
-  const int ring = kAttnWarps * attn_ring(dim, fmt) * attn_tile_bytes(dim, fmt);
+  const int ring = kAttnWarps * attn_ring(dim, fmt) * attn_tiles(dim, fmt) * attn_tile_bytes(dim, fmt);
   const int join = kAttnWarps * 8 * nt * (dim + 4 + 2) * 4;  // the warps' parts, after the ring
   return ring > join ? ring : join;
 }
@@ -73,6 +75,7 @@ struct AttnArgs {
   float* lse;              // [seqs][q_heads] or null
   float* parts;            // [blocks][2][8 * NT heads][dim + 2]
   int blocks;              // of the main kernel
+  int unit_keys;
 };
 
 __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -273,9 +276,10 @@ __device__ __forceinline__ void v_pairs(const uint32_t* a, const uint32_t* b, ui
 }
 
 template <int D, int kFmt, int NT>
-__global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int kGroups = D / 32, kHeads = 8 * NT, kRing = attn_ring(D, kFmt);
   constexpr int kRowBytes = attn_row_bytes(D, kFmt), kTile = attn_tile_bytes(D, kFmt);
+  constexpr int KT = attn_tiles(D, kFmt), kUnitKeys = attn_unit_keys(D, kFmt);
   constexpr int kKw = kRowBytes / kGroups / 16;  // words of K codes per lane, key and group: 2 or 1
   constexpr int kVw = kRowBytes / 32;            // words of V codes per lane and key
   constexpr float kCarry = kFmt == kFmtE4M3 ? 56.0f : 62.0f;  // p carries 2^kCarry, v 2^-kCarry
@@ -290,23 +294,23 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kerne
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int key_g = (g >> 1) + 4 * (g & 1);  // pi(g): the key of operand row g (and key_g + 8 of row g + 8)
-  const uint32_t ring = smem_u32(sm) + warp * kRing * kTile;
+  const uint32_t ring = smem_u32(sm) + warp * kRing * KT * kTile;
   const uint32_t base_k = attn_copy_base<D, kFmt, false>(), base_v = attn_copy_base<D, kFmt, true>();
 
   long long total, none;
-  attn_count_units(a, kAttnUnitKeys, 0, total, none, red);
+  attn_count_units(a, kUnitKeys, 0, total, none, red);
   const long long share = attn_share(total, a.blocks);
   long long u = share * blockIdx.x;
   const long long u_end = min(u + share, total);
   if (u >= u_end) return;
   int seq;
   long long begin;
-  attn_find(a, kAttnUnitKeys, u, seq, begin);
+  attn_find(a, kUnitKeys, u, seq, begin);
 
   while (u < u_end) {
     // the segment: units [first, last) of head (seq, head, chunk)
     const int len = attn_length(a, seq);
-    const int units = (len + kAttnUnitKeys - 1) / kAttnUnitKeys;
+    const int units = (len + kUnitKeys - 1) / kUnitKeys;
     if (units == 0) {
       ++seq;
       continue;
@@ -319,13 +323,15 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kerne
     const int nh = min(kHeads, a.group - chunk * kHeads);            // q heads here
     const int* table = a.table + a.table_stride * seq;
     const int tile_shift = a.cache.page_shift - 4;
-    const int tile_last = min(last * kAttnWarps, (len + 15) >> 4);
+    const int tile_last = min(last * kAttnWarps * KT, (len + 15) >> 4);
 
-    // Copies into the ring, one commit group per tile; the page of the tile after is on its way.
-    // `good` has a bit for each of the last copies: whether its page is one of the cache's.
+    // Copies into the ring, one commit group per step; the pages of the step after are on their way.
+    // `good` has KT bits for each of the last copies: whether the tile's page is one of the cache's.
     uint32_t good = 0;
-    int copy_tile = first * kAttnWarps + warp, copy_slot = 0;
-    int page = copy_tile < tile_last ? __ldg(table + (copy_tile >> tile_shift)) : 0;
+    int copy_tile = (first * kAttnWarps + warp) * KT, copy_slot = 0;
+    int page[KT];
+#pragma unroll
+    for (int i = 0; i < KT; ++i) page[i] = copy_tile + i < tile_last ? __ldg(table + ((copy_tile + i) >> tile_shift)) : 0;
     const uint32_t page_rows = static_cast<uint32_t>(a.cache.heads) << a.cache.page_shift;
     const size_t head_rows = static_cast<size_t>(head) << a.cache.page_shift;
     const uint8_t* k_lane = a.cache.k_codes + head_rows * kRowBytes + 16 * lane;
@@ -333,19 +339,23 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kerne
     const uint8_t* s_lane = (lane < kGroups ? a.cache.k_scales + 16 * lane : a.cache.v_scales + 16 * (lane - kGroups)) +
                             head_rows * kGroups;
     auto copy_next = [&]() {
-      good <<= 1;
-      if (copy_tile < tile_last) {
-        if (page >= 0 && page < a.cache.num_pages) {
-          const size_t row = static_cast<size_t>(page) * page_rows + ((copy_tile & ((1 << tile_shift) - 1)) << 4);
-          attn_copy_tile<D, kFmt>(k_lane + row * kRowBytes, v_lane + row * kRowBytes, s_lane + row * kGroups,
-                                  ring + copy_slot * kTile, base_k, base_v);
-          good |= 1;
-        } else {
-          record_error(kErrBadPage);
+      good <<= KT;
+#pragma unroll
+      for (int i = 0; i < KT; ++i)
+        if (copy_tile + i < tile_last) {
+          if (page[i] >= 0 && page[i] < a.cache.num_pages) {
+            const size_t row = static_cast<size_t>(page[i]) * page_rows + (((copy_tile + i) & ((1 << tile_shift) - 1)) << 4);
+            attn_copy_tile<D, kFmt>(k_lane + row * kRowBytes, v_lane + row * kRowBytes, s_lane + row * kGroups,
+                                    ring + (copy_slot * KT + i) * kTile, base_k, base_v);
+            good |= 1u << i;
+          } else {
+            record_error(kErrBadPage);
+          }
         }
-        copy_tile += kAttnWarps;
-        if (copy_tile < tile_last) page = __ldg(table + (copy_tile >> tile_shift));
-      }
+      copy_tile += kAttnWarps * KT;
+#pragma unroll
+      for (int i = 0; i < KT; ++i)
+        if (copy_tile + i < tile_last) page[i] = __ldg(table + ((copy_tile + i) >> tile_shift));
       copy_slot = copy_slot + 1 == kRing ? 0 : copy_slot + 1;
       cp_async_commit();
     };
@@ -399,141 +409,150 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, NT)) attn_kerne
     }
 
     int slot = 0;
-    // One tile; `ragged`: the sequence ends inside it.
-    auto do_tile = [&](int tile, auto ragged) {
-      cp_async_wait<kRing - 2>();
-      __syncwarp();  // every lane's copies have landed, and all lanes have left the slot copied into next
-      copy_next();
-      const uint32_t at = ring + slot * kTile;
-      slot = slot + 1 == kRing ? 0 : slot + 1;
-      if (!((good >> (kRing - 1)) & 1)) return;
-
+    // One step; `ragged`: the sequence ends inside it, or a page of it is missing.
+    auto do_step = [&](int tile, uint32_t have, uint32_t at, auto ragged) {
       // scores
-      float s[NT][4];
+      float s[KT][NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-      uint32_t two[2][kGroups / 2];  // the two keys' scales, a bf16x2 per pair of groups
+      for (int i = 0; i < KT; ++i) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t sa = at + 32 * kRowBytes + (key_g + 8 * h) * kGroups;
-        uint32_t w[(kGroups + 3) / 4];
-        if constexpr (kGroups == 2) {
-          asm volatile("ld.shared.u16 %0, [%1];" : "=r"(w[0]) : "r"(sa));
-          two[h][0] = e8m0x2_bf16x2(w[0]);
-        } else {
-          lds_words<kGroups / 4>(sa, w);
-#pragma unroll
-          for (int b = 0; b < kGroups; b += 4) e8m0x4_bf16x2(w[b / 4], two[h][b / 2], two[h][b / 2 + 1]);
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < kGroups; ++b) {
-        uint32_t f[2][4];  // [key][value pairs 8t + 2j]
+        for (int n = 0; n < NT; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.0f;
+        uint32_t two[2][kGroups / 2];  // the two keys' scales, a bf16x2 per pair of groups
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int key = key_g + 8 * h;
-          const int byte = b * (kRowBytes / kGroups) + 4 * kKw * t;
-          uint32_t w[kKw];
-          lds_words<kKw>(at + key * kRowBytes + (byte ^ (16 * attn_swizzle<D, kFmt, false>(key))), w);
-          if constexpr (kFmt == kFmtE4M3) {
-            e4m3x4_to_f16x2(w[0], f[h][0], f[h][1]);
-            e4m3x4_to_f16x2(w[1], f[h][2], f[h][3]);
+          const uint32_t sa = at + i * kTile + 32 * kRowBytes + (key_g + 8 * h) * kGroups;
+          uint32_t w[(kGroups + 3) / 4];
+          if constexpr (kGroups == 2) {
+            asm volatile("ld.shared.u16 %0, [%1];" : "=r"(w[0]) : "r"(sa));
+            two[h][0] = e8m0x2_bf16x2(w[0]);
           } else {
-            e2m1x8_to_f16x2(w[0], f[h]);
+            lds_words<kGroups / 4>(sa, w);
+#pragma unroll
+            for (int b = 0; b < kGroups; b += 4) e8m0x4_bf16x2(w[b / 4], two[h][b / 2], two[h][b / 2 + 1]);
           }
         }
-        const float s0 = b & 1 ? bf16_hi(two[0][b / 2]) : bf16_lo(two[0][b / 2]);
-        const float s1 = b & 1 ? bf16_hi(two[1][b / 2]) : bf16_lo(two[1][b / 2]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          mma_f16_16816(d, f[0][0], f[1][0], f[0][1], f[1][1], q[n][b][0], q[n][b][1]);
-          mma_f16_16816(d, f[0][2], f[1][2], f[0][3], f[1][3], q[n][b][2], q[n][b][3]);
-          s[n][0] = fmaf(d[0], s0, s[n][0]);
-          s[n][1] = fmaf(d[1], s0, s[n][1]);
-          s[n][2] = fmaf(d[2], s1, s[n][2]);
-          s[n][3] = fmaf(d[3], s1, s[n][3]);
+        for (int b = 0; b < kGroups; ++b) {
+          uint32_t f[2][4];  // [key][value pairs 8t + 2j]
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int key = key_g + 8 * h;
+            const int byte = b * (kRowBytes / kGroups) + 4 * kKw * t;
+            uint32_t w[kKw];
+            lds_words<kKw>(at + i * kTile + key * kRowBytes + (byte ^ (16 * attn_swizzle<D, kFmt, false>(key))), w);
+            if constexpr (kFmt == kFmtE4M3) {
+              e4m3x4_to_f16x2(w[0], f[h][0], f[h][1]);
+              e4m3x4_to_f16x2(w[1], f[h][2], f[h][3]);
+            } else {
+              e2m1x8_to_f16x2(w[0], f[h]);
+            }
+          }
+          const float s0 = b & 1 ? bf16_hi(two[0][b / 2]) : bf16_lo(two[0][b / 2]);
+          const float s1 = b & 1 ? bf16_hi(two[1][b / 2]) : bf16_lo(two[1][b / 2]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma_f16_16816(d, f[0][0], f[1][0], f[0][1], f[1][1], q[n][b][0], q[n][b][1]);
+            mma_f16_16816(d, f[0][2], f[1][2], f[0][3], f[1][3], q[n][b][2], q[n][b][3]);
+            s[i][n][0] = fmaf(d[0], s0, s[i][n][0]);
+            s[i][n][1] = fmaf(d[1], s0, s[i][n][1]);
+            s[i][n][2] = fmaf(d[2], s1, s[i][n][2]);
+            s[i][n][3] = fmaf(d[3], s1, s[i][n][3]);
+          }
         }
-      }
-      // in powers of two, those of no key at -inf
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][j] *= mult[n][j & 1];
-      if constexpr (decltype(ragged)::value) {
+        // in powers of two, those of no key at -inf
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (tile * 16 + key_g + 8 * (j >> 1) >= len) s[n][j] = -kInf;
+          for (int j = 0; j < 4; ++j) {
+            s[i][n][j] *= mult[n][j & 1];
+            if constexpr (decltype(ragged)::value)
+              if (!((have >> i) & 1) || (tile + i) * 16 + key_g + 8 * (j >> 1) >= len) s[i][n][j] = -kInf;
+          }
       }
       // The reference m follows the running maximum only when a score passes it by kRise: p stays
-      // below 2^(kCarry + kRise), and most tiles need no exchange between lanes and no rescaling.
+      // below 2^(kCarry + kRise), and most steps need no exchange between lanes and no rescaling.
+      float top[NT][2];
       bool rise = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) rise |= fmaxf(s[n][j], s[n][j + 2]) > m[n][j] + kRise;
+        for (int j = 0; j < 2; ++j) {
+          top[n][j] = fmaxf(s[0][n][j], s[0][n][j + 2]);
+#pragma unroll
+          for (int i = 1; i < KT; ++i) top[n][j] = fmaxf(top[n][j], fmaxf(s[i][n][j], s[i][n][j + 2]));
+          rise |= top[n][j] > m[n][j] + kRise;
+        }
       if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = fmaxf(m[n][j], fmaxf(s[n][j], s[n][j + 2]));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float base = top == -kInf ? 0.0f : top;  // no score yet
+            float u = fmaxf(m[n][j], top[n][j]);
+            u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 4));
+            u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 8));
+            u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 16));
+            const float base = u == -kInf ? 0.0f : u;  // no score yet
             const float fade = exp2_approx(m[n][j] - base);
-            m[n][j] = top;
+            m[n][j] = u;
             sub[n][j] = base - kCarry;
             lsum[n][j] *= fade;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) acc[i][n][j] *= fade, acc[i][n][j + 2] *= fade;
+            for (int c = 0; c < D / 16; ++c) acc[c][n][j] *= fade, acc[c][n][j + 2] *= fade;
           }
       }
-      uint32_t p[NT][2];
+      uint32_t p[KT][NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float p0 = exp2_approx(s[n][0] - sub[n][0]), p1 = exp2_approx(s[n][1] - sub[n][1]);
-        const float p2 = exp2_approx(s[n][2] - sub[n][0]), p3 = exp2_approx(s[n][3] - sub[n][1]);
-        lsum[n][0] += p0 + p2;
-        lsum[n][1] += p1 + p3;
-        // p is rounded to bf16 for the product (relative 2^-9 each, of either sign); the sum is not
-        p[n][0] = transpose8x8(pack_bf16x2(p0, p1));
-        p[n][1] = transpose8x8(pack_bf16x2(p2, p3));
-      }
+      for (int i = 0; i < KT; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float p0 = exp2_approx(s[i][n][0] - sub[n][0]), p1 = exp2_approx(s[i][n][1] - sub[n][1]);
+          const float p2 = exp2_approx(s[i][n][2] - sub[n][0]), p3 = exp2_approx(s[i][n][3] - sub[n][1]);
+          lsum[n][0] += p0 + p2;
+          lsum[n][1] += p1 + p3;
+          // p is rounded to bf16 for the product (relative 2^-9 each, of either sign); the sum is not
+          p[i][n][0] = transpose8x8(pack_bf16x2(p0, p1));
+          p[i][n][1] = transpose8x8(pack_bf16x2(p2, p3));
+        }
       // output
-      uint32_t w[4][kVw], vs[4];  // keys t, t + 4, t + 8, t + 12
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = t + 4 * j;
-        const uint32_t va = at + 16 * kRowBytes + key * kRowBytes;
+      for (int i = 0; i < KT; ++i) {
+        uint32_t w[4][kVw], vs[4];  // keys t, t + 4, t + 8, t + 12
 #pragma unroll
-        for (int i = 0; i < kVw; i += 4)
-          lds_words<(kVw < 4 ? kVw : 4)>(va + ((4 * kVw * g + 4 * i) ^ (16 * attn_swizzle<D, kFmt, true>(key))), w[j] + i);
-        vs[j] = lds_u8(at + 32 * kRowBytes + 16 * kGroups + key * kGroups + (g * D / 8) / 32);
-        if constexpr (decltype(ragged)::value)
-          if (tile * 16 + key >= len) {  // rows behind the sequence may hold anything
-            vs[j] = 0;
+        for (int j = 0; j < 4; ++j) {
+          const int key = t + 4 * j;
+          const uint32_t row = at + i * kTile + 16 * kRowBytes + key * kRowBytes;
 #pragma unroll
-            for (int i = 0; i < kVw; ++i) w[j][i] = 0;
-          }
+          for (int c = 0; c < kVw; c += 4)
+            lds_words<(kVw < 4 ? kVw : 4)>(row + ((4 * kVw * g + 4 * c) ^ (16 * attn_swizzle<D, kFmt, true>(key))), w[j] + c);
+          vs[j] = lds_u8(at + i * kTile + 32 * kRowBytes + 16 * kGroups + key * kGroups + (g * D / 8) / 32);
+          if constexpr (decltype(ragged)::value)
+            if (!((have >> i) & 1) || (tile + i) * 16 + key >= len) {  // the bytes of no key may be anything
+              vs[j] = 0;
+#pragma unroll
+              for (int c = 0; c < kVw; ++c) w[j][c] = 0;
+            }
+        }
+        uint32_t va[D / 8], vb[D / 8];
+        v_pairs<D, kFmt>(w[0], w[1], v_factor(vs[0], vs[1]), va);
+        v_pairs<D, kFmt>(w[2], w[3], v_factor(vs[2], vs[3]), vb);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            mma_bf16_16816(acc[c][n], va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], p[i][n][0], p[i][n][1]);
       }
-      uint32_t va[D / 8], vb[D / 8];
-      v_pairs<D, kFmt>(w[0], w[1], v_factor(vs[0], vs[1]), va);
-      v_pairs<D, kFmt>(w[2], w[3], v_factor(vs[2], vs[3]), vb);
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          mma_bf16_16816(acc[c][n], va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], p[n][0], p[n][1]);
     };
-    int tile = first * kAttnWarps + warp;
-    const int tile_full = min(tile_last, len >> 4);
 #pragma unroll 1
-    for (; tile < tile_full; tile += kAttnWarps) do_tile(tile, std::false_type{});
-    if (tile < tile_last) do_tile(tile, std::true_type{});
+    for (int tile = (first * kAttnWarps + warp) * KT; tile < tile_last; tile += kAttnWarps * KT) {
+      cp_async_wait<kRing - 2>();
+      __syncwarp();  // every lane's copies have landed, and all lanes have left the slot copied into next
+      copy_next();
+      const uint32_t at = ring + slot * KT * kTile, have = (good >> (KT * (kRing - 1))) & ((1u << KT) - 1);
+      slot = slot + 1 == kRing ? 0 : slot + 1;
+      if (have == (1u << KT) - 1 && (tile + KT) * 16 <= len) do_step(tile, have, at, std::false_type{});
+      else if (have) do_step(tile, have, at, std::true_type{});
+    }
     cp_async_wait<0>();
     __syncthreads();  // the rings become the buffer of the parts
 
@@ -609,8 +628,8 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const __grid_co
   if (h >= a.group - chunk * kHeads) return;
   const size_t at = static_cast<size_t>(seq) * a.q_heads + head * a.group + chunk * kHeads + h;
   long long total, ahead;
-  attn_count_units(a, kAttnUnitKeys, seq, total, ahead, red);
-  const int units = (attn_length(a, seq) + kAttnUnitKeys - 1) / kAttnUnitKeys;
+  attn_count_units(a, a.unit_keys, seq, total, ahead, red);
+  const int units = (attn_length(a, seq) + a.unit_keys - 1) / a.unit_keys;
   const int team = threadIdx.x / kLanes, d = 4 * (threadIdx.x - team * kLanes);
   griddep_wait();
   if (units == 0) {
