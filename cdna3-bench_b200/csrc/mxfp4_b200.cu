@@ -751,10 +751,11 @@ int rope_args(RowArgs* a, const void* qkv, long long row_stride, int tokens, int
   return 0;
 }
 
-// Blocks of the attention kernel: as many as are resident together.  kResident is the kernel's
-// launch bound, so this needs no query and holds without a device (148 SMs then).
+// The attention kernel's pieces: about as many as blocks are resident (the kernel's launch bound, so
+// this needs no query and holds without a device: 148 SMs then), and a head's last piece may
+// be a short one: up to target + heads blocks.  Heads of more than one piece have at most 2 * target.
 struct AttnPlan {
-  int nt, chunks, blocks, unit_keys;
+  int nt, chunks, target, blocks, unit_keys;
   size_t bytes;
 };
 AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int max_pages, int page_size, int sm_count) {
@@ -762,16 +763,18 @@ AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int ma
   const int group = q_heads / kv_heads;
   p.nt = group > 8 && dim < 256 ? 2 : 1;  // two operand tiles of 8 heads fit the registers below D = 256
   p.chunks = ceil_div(group, 8 * p.nt);
-  const long long keys = static_cast<long long>(max_pages) * page_size;
   p.unit_keys = attn_unit_keys(dim, fmt);
-  const long long units = (keys + p.unit_keys - 1) / p.unit_keys * seqs * kv_heads * p.chunks;
-  p.blocks = static_cast<int>(std::min<long long>(std::max<long long>(units, 1), 1ll * sm_count * attn_resident(dim, fmt, p.nt)));
-  p.bytes = static_cast<size_t>(p.blocks) * 2 * 8 * p.nt * (dim + 2) * sizeof(float);
+  const long long keys = static_cast<long long>(max_pages) * page_size, heads = static_cast<long long>(seqs) * kv_heads * p.chunks;
+  const long long units = (keys + p.unit_keys - 1) / p.unit_keys * heads;
+  const long long resident = 1ll * sm_count * attn_resident(dim, fmt, p.nt) * kAttnPieces;
+  p.target = static_cast<int>(std::min(units, resident));
+  p.blocks = static_cast<int>(std::min(units, resident + heads));
+  p.bytes = keys > p.unit_keys ? static_cast<size_t>(p.target) * 2 * 8 * p.nt * (dim + 2) * sizeof(float) : 0;
   return p;
 }
 
 template <int D, int kFmt, int NT>
-int launch_attention(const AttnArgs& a, DeviceState* d, cudaStream_t s) {
+int launch_attention(const AttnArgs& a, int blocks, DeviceState* d, cudaStream_t s) {
   constexpr int smem = attn_smem_bytes(D, kFmt, NT);
   std::atomic<bool>& done = d->attn_attr[((D == 64 ? 0 : D == 128 ? 1 : 2) * 2 + (kFmt - 1)) * 2 + NT - 1];
   if (!done.load(std::memory_order_acquire)) {
@@ -779,18 +782,18 @@ int launch_attention(const AttnArgs& a, DeviceState* d, cudaStream_t s) {
     if (e != cudaSuccess) return ret(e);
     done.store(true, std::memory_order_release);
   }
-  attn_kernel<D, kFmt, NT><<<a.blocks, kAttnThreads, smem, s>>>(a);
+  attn_kernel<D, kFmt, NT><<<blocks, kAttnThreads, smem, s>>>(a);
   const int rc = launch_status();
   if (rc) return rc;
   return launch_pdl_grid(attn_join_kernel<D, NT>, dim3(a.seqs * a.cache.heads * a.chunks, std::min(8 * NT, a.group)), kAttnThreads, 0, s, a);
 }
 
 template <int kFmt>
-int launch_attention_dim(const AttnArgs& a, int nt, DeviceState* d, cudaStream_t s) {
+int launch_attention_dim(const AttnArgs& a, int nt, int blocks, DeviceState* d, cudaStream_t s) {
   switch (a.cache.dim) {
-    case 64: return nt == 1 ? launch_attention<64, kFmt, 1>(a, d, s) : launch_attention<64, kFmt, 2>(a, d, s);
-    case 128: return nt == 1 ? launch_attention<128, kFmt, 1>(a, d, s) : launch_attention<128, kFmt, 2>(a, d, s);
-    default: return launch_attention<256, kFmt, 1>(a, d, s);
+    case 64: return nt == 1 ? launch_attention<64, kFmt, 1>(a, blocks, d, s) : launch_attention<64, kFmt, 2>(a, blocks, d, s);
+    case 128: return nt == 1 ? launch_attention<128, kFmt, 1>(a, blocks, d, s) : launch_attention<128, kFmt, 2>(a, blocks, d, s);
+    default: return launch_attention<256, kFmt, 1>(a, blocks, d, s);
   }
 }
 
@@ -1134,7 +1137,8 @@ int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cach
   if (seqs < 0 || num_heads <= 0 || max_pages <= 0 || page_stride < max_pages) return MXFP4_ERR_INVALID_ARGUMENT;
   if (num_heads % a.cache.heads || static_cast<long long>(max_pages) * cache->page_size >= (1ll << 31))
     return MXFP4_ERR_UNSUPPORTED_SHAPE;
-  if (static_cast<long long>(seqs) * num_heads >= (1ll << 31)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
+  if (static_cast<long long>(seqs) * num_heads >= (1ll << 30)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
+  if (static_cast<long long>(max_pages) * cache->page_size / kAttnMinUnit * seqs >= (1ll << 30)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
   if (q_stride < static_cast<long long>(num_heads) * a.cache.dim) return MXFP4_ERR_INVALID_ARGUMENT;
   if (seqs == 0) return 0;
   if (!q || !page_table || !lengths || !out) return MXFP4_ERR_INVALID_ARGUMENT;
@@ -1143,15 +1147,15 @@ int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cach
   rc = current_device(&d);
   if (rc) return rc;
   const AttnPlan p = attn_plan(a.cache.dim, fmt, a.cache.heads, num_heads, seqs, max_pages, cache->page_size, d->sm_count);
-  if (!workspace || workspace_bytes < p.bytes) return MXFP4_ERR_WORKSPACE;
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return MXFP4_ERR_WORKSPACE;
   a.q = static_cast<const __nv_bfloat16*>(q), a.q_stride = q_stride;
   a.table = page_table, a.table_stride = page_stride, a.max_pages = max_pages;
   a.lengths = lengths, a.seqs = seqs, a.q_heads = num_heads, a.group = num_heads / a.cache.heads, a.chunks = p.chunks;
   a.scale = scale;
   a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
-  a.parts = static_cast<float*>(workspace), a.blocks = p.blocks, a.unit_keys = p.unit_keys;
+  a.parts = static_cast<float*>(workspace), a.target = p.target, a.unit_keys = p.unit_keys;
   auto s = static_cast<cudaStream_t>(stream);
-  return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p.nt, d, s) : launch_attention_dim<kFmtE2M1>(a, p.nt, d, s);
+  return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p.nt, p.blocks, d, s) : launch_attention_dim<kFmtE2M1>(a, p.nt, p.blocks, d, s);
 }
 
 }  // extern "C"

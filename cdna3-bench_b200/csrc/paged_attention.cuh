@@ -25,10 +25,11 @@
 //           The transposition between S^T's accumulators and P^T's operand is one
 //           movmatrix per 8 keys.
 //
-// The sequences are cut into units of kAttnWarps * attn_tiles tiles; every block takes an equal, contiguous
-// share of all units in (sequence, kv head, head chunk) order, whatever the lengths are (they are
-// read on the device).  A head whose units lie in one block is written at once; the parts of the
-// others go to the workspace and attn_join_kernel adds them in the blocks' order.
+// A head's keys are cut into units of kAttnWarps steps, and the heads into pieces of at most `share`
+// units, share so that there are about as many pieces as blocks are resident: one block to a piece,
+// found from the lengths on the device, so that long and short sequences share the GPU evenly and a
+// block's first loads run beside the other blocks' work.  A head of one piece is written at
+// once; the parts of the others go to the workspace and attn_join_kernel adds them in order.
 #pragma once
 
 #include <type_traits>
@@ -41,6 +42,7 @@ namespace mxb {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
+constexpr int kAttnPieces = 1;  // pieces per resident block
 
 // Tiles of 16 keys a warp takes in one step; steps in its ring; blocks resident per SM (the kernel's
 // launch bound).
@@ -51,6 +53,7 @@ __host__ __device__ constexpr int attn_resident(int dim, int fmt, int nt) {
 }
 __host__ __device__ constexpr int attn_unit_keys(int dim, int fmt) { return 16 * kAttnWarps * attn_tiles(dim, fmt); }
 __host__ __device__ constexpr int attn_row_bytes(int dim, int fmt) { return fmt == kFmtE4M3 ? dim : dim / 2; }
+constexpr int kAttnMinUnit = 16 * kAttnWarps;
 // K codes, V codes, K scales, V scales of 16 keys
 __host__ __device__ constexpr int attn_tile_bytes(int dim, int fmt) {
   return 16 * 2 * (attn_row_bytes(dim, fmt) + dim / 32);
@@ -73,8 +76,8 @@ struct AttnArgs {
   float scale;
   __nv_bfloat16* out;      // [seqs][q_heads][dim]
   float* lse;              // [seqs][q_heads] or null
-  float* parts;            // [blocks][2][8 * NT heads][dim + 2]
-  int blocks;              // of the main kernel
+  float* parts;            // [2 * target][8 * NT heads][dim + 2]
+  int target;              // pieces to cut the work into
   int unit_keys;
 };
 
@@ -112,58 +115,77 @@ __device__ __forceinline__ int attn_length(const AttnArgs& a, int b) {
   return len < 0 ? 0 : len;
 }
 
-// Units of all sequences, and of those before sequence `before` (block-wide; red: 2 * warps words).
-__device__ __forceinline__ void attn_count_units(const AttnArgs& a, int unit_keys, int before, long long& total,
-                                                 long long& ahead, long long* red) {
-  long long s = 0, p = 0;
-  for (int b = threadIdx.x; b < a.seqs; b += blockDim.x) {
-    const long long u = (attn_length(a, b) + unit_keys - 1) / unit_keys;
-    s += u;
-    if (b < before) p += u;
-  }
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, m);
-    p += __shfl_xor_sync(0xffffffffu, p, m);
-  }
-  const int w = threadIdx.x >> 5, n = blockDim.x >> 5;
-  if ((threadIdx.x & 31) == 0) red[w] = s, red[n + w] = p;
-  __syncthreads();
-  total = ahead = 0;
-  for (int i = 0; i < n; ++i) total += red[i], ahead += red[n + i];
-  __syncthreads();
-  const long long per = static_cast<long long>(a.cache.heads) * a.chunks;
-  total *= per;
-  ahead *= per;
+__device__ __forceinline__ int attn_units(const AttnArgs& a, int b, int unit_keys) {
+  return (attn_length(a, b) + unit_keys - 1) / unit_keys;
 }
 
-__device__ __forceinline__ long long attn_share(long long total, int blocks) { return (total + blocks - 1) / blocks; }
+// Sum of f(sequence) over sequences 0 .. n - 1 (below 2^31: so is the number of all units).  Every
+// warp on its own.
+template <typename F>
+__device__ __forceinline__ int attn_sum(int n, F f) {
+  int s = 0;
+#pragma unroll 4
+  for (int b = threadIdx.x & 31; b < n; b += 32) s += f(b);
+  return __reduce_add_sync(0xffffffffu, s);
+}
+__device__ __forceinline__ int ceil_ratio(long long a, int b) {
+  if (a < 0x7FFFFFFFll - b) return (static_cast<int>(a) + b - 1) / b;
+  return static_cast<int>(min((a + b - 1) / b, 0x7FFFFFFFll));
+}
 
-// Finds the sequence that unit u of all units lies in, and the unit index at which it begins.
-// One warp; u < total.
-__device__ __forceinline__ void attn_find(const AttnArgs& a, int unit_keys, long long u, int& seq, long long& begin) {
-  const long long per = static_cast<long long>(a.cache.heads) * a.chunks;
-  const int lane = threadIdx.x & 31;
-  long long base = 0;
-  for (int b0 = 0; b0 < a.seqs; b0 += 32) {
-    long long n = b0 + lane < a.seqs ? (attn_length(a, b0 + lane) + unit_keys - 1) / unit_keys * per : 0;
-    long long run = n;
-#pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-      const long long o = __shfl_up_sync(0xffffffffu, run, m);
-      if (lane >= m) run += o;
+// Pieces of each head of a sequence.
+__device__ __forceinline__ int attn_pieces(int units, int share) { return (units + share - 1) / share; }
+
+// Most units of a piece.  All units over the pieces wanted; where the heads are few, the least with
+// which the pieces are no more than wanted, so that they all run at once (rounding up leaves up to one
+// short piece per head, and a second round of blocks for them would double the time).
+__device__ __forceinline__ int attn_share(const AttnArgs& a, int unit_keys) {
+  const long long per = static_cast<long long>(a.cache.heads) * a.chunks, heads = per * a.seqs;
+  const long long total = per * attn_sum(a.seqs, [&](int b) { return attn_units(a, b, unit_keys); });
+  int lo = max(1, ceil_ratio(total, a.target));
+  if (2 * heads <= a.target) {
+    // with total / share + heads <= target there are enough
+    int hi = max(lo, ceil_ratio(total, a.target - static_cast<int>(heads)));
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      if (per * attn_sum(a.seqs, [&](int b) { return attn_pieces(attn_units(a, b, unit_keys), mid); }) <= a.target) hi = mid;
+      else lo = mid + 1;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, base + run > u);
-    if (hit) {
-      const int f = __ffs(hit) - 1;
-      seq = b0 + f;
-      begin = base + __shfl_sync(0xffffffffu, run - n, f);
-      return;
-    }
-    base += __shfl_sync(0xffffffffu, run, 31);
   }
-  seq = a.seqs;
-  begin = base;
+  return lo;
+}
+
+struct AttnPiece {
+  int seq, head_chunk, index, of;  // the index-th of `of` pieces of a head
+  int slot;                        // its place in the workspace, where of > 1
+};
+// The piece-th piece of all; false if there are fewer.  Every warp on its own.
+__device__ __forceinline__ bool attn_find(const AttnArgs& a, int unit_keys, int share, int piece, AttnPiece& found) {
+  const int per = a.cache.heads * a.chunks, lane = threadIdx.x & 31;
+  int pieces = 0, slots = 0;  // of the sequences before
+  for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+    const int n = b0 + lane < a.seqs ? attn_pieces(attn_units(a, b0 + lane, unit_keys), share) : 0;
+    const int all = __reduce_add_sync(0xffffffffu, n) * per, held = __reduce_add_sync(0xffffffffu, n > 1 ? n : 0) * per;
+    if (pieces + all > piece) {
+      int run = n, kept = n > 1 ? n : 0;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, run, m), y = __shfl_up_sync(0xffffffffu, kept, m);
+        if (lane >= m) run += x, kept += y;
+      }
+      const int f = __ffs(__ballot_sync(0xffffffffu, pieces + run * per > piece)) - 1;
+      found.seq = b0 + f;
+      found.of = __shfl_sync(0xffffffffu, n, f);
+      const int r = piece - pieces - (__shfl_sync(0xffffffffu, run, f) - found.of) * per;
+      found.head_chunk = r / found.of;
+      found.index = r - found.head_chunk * found.of;
+      found.slot = slots + (__shfl_sync(0xffffffffu, kept, f) - found.of) * per + r;
+      return true;
+    }
+    pieces += all;
+    slots += held;
+  }
+  return false;
 }
 
 // Placement of the 16-byte units of key row r (0..15) of a tile in shared memory: unit u of the row
@@ -289,7 +311,6 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
   extern __shared__ __align__(128) float sm[];                // the warps' rings; then [warps][kHeads][kStride]
   float* sm_m = sm + kAttnWarps * kHeads * kStride;           // and m, l [warps][kHeads]
   float* sm_l = sm_m + kAttnWarps * kHeads;
-  __shared__ long long red[2 * kAttnWarps];
 
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -297,28 +318,13 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
   const uint32_t ring = smem_u32(sm) + warp * kRing * KT * kTile;
   const uint32_t base_k = attn_copy_base<D, kFmt, false>(), base_v = attn_copy_base<D, kFmt, true>();
 
-  long long total, none;
-  attn_count_units(a, kUnitKeys, 0, total, none, red);
-  const long long share = attn_share(total, a.blocks);
-  long long u = share * blockIdx.x;
-  const long long u_end = min(u + share, total);
-  if (u >= u_end) return;
-  int seq;
-  long long begin;
-  attn_find(a, kUnitKeys, u, seq, begin);
-
-  while (u < u_end) {
-    // the segment: units [first, last) of head (seq, head, chunk)
-    const int len = attn_length(a, seq);
-    const int units = (len + kUnitKeys - 1) / kUnitKeys;
-    if (units == 0) {
-      ++seq;
-      continue;
-    }
-    const int hc = static_cast<int>((u - begin) / units);
-    const int first = static_cast<int>((u - begin) - static_cast<long long>(hc) * units);
-    const int last = static_cast<int>(min(static_cast<long long>(units), first + (u_end - u)));
-    const int head = hc / a.chunks, chunk = hc - head * a.chunks;
+  AttnPiece me;
+  if (!attn_find(a, kUnitKeys, attn_share(a, kUnitKeys), blockIdx.x, me)) return;
+  {
+    const int seq = me.seq, len = attn_length(a, seq), units = attn_units(a, seq, kUnitKeys);
+    const int first = static_cast<int>(static_cast<long long>(units) * me.index / me.of);  // units first .. last - 1
+    const int last = static_cast<int>(static_cast<long long>(units) * (me.index + 1) / me.of);
+    const int head = me.head_chunk / a.chunks, chunk = me.head_chunk - head * a.chunks;
     const int h0 = head * a.group + chunk * kHeads;                  // first q head
     const int nh = min(kHeads, a.group - chunk * kHeads);            // q heads here
     const int* table = a.table + a.table_stride * seq;
@@ -573,8 +579,8 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
           *reinterpret_cast<float2*>(dst + 2 * c) = make_float2(acc[c][n][j], acc[c][n][j + 2]);
       }
     __syncthreads();
-    const bool whole = first == 0 && last == units;
-    float* part = a.parts + (2 * static_cast<size_t>(blockIdx.x) + (first == 0 ? 1 : 0)) * kHeads * (D + 2);
+    const bool whole = me.of == 1;
+    float* part = a.parts + static_cast<size_t>(me.slot) * kHeads * (D + 2);
     for (int i = threadIdx.x; i < nh * (D / 4); i += kAttnThreads) {
       const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
       float top = -kInf;
@@ -603,23 +609,16 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
         if (d == 0) part[kHeads * D + 2 * h] = top, part[kHeads * D + 2 * h + 1] = l;
       }
     }
-    __syncthreads();
-    u += last - first;
-    if (last == units && hc + 1 == a.cache.heads * a.chunks) {
-      begin += static_cast<long long>(units) * a.cache.heads * a.chunks;
-      ++seq;
-    }
   }
 }
 
-// Joins the parts of the heads that lie in several blocks' shares, in a fixed order, and writes the
-// rows of empty sequences.  One block per (sequence, kv head, chunk) and query head; the parts are
+// Joins the parts of the heads of several pieces, in a fixed order, and writes the rows of empty
+// sequences.  One block per (sequence, kv head, chunk) and query head; the parts are
 // dealt to its lanes, D / 4 of them to a part.
 template <int D, int NT>
 __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int kHeads = 8 * NT, kLanes = D / 4, kTeams = kAttnThreads / kLanes;
   constexpr float kInf = __builtin_huge_valf();
-  __shared__ long long red[2 * kAttnWarps];
   __shared__ float4 sums[kTeams][kLanes];
   __shared__ float ls[kTeams];
   const int per = a.cache.heads * a.chunks;
@@ -627,30 +626,31 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const __grid_co
   const int head = hc / a.chunks, chunk = hc - head * a.chunks, h = blockIdx.y;
   if (h >= a.group - chunk * kHeads) return;
   const size_t at = static_cast<size_t>(seq) * a.q_heads + head * a.group + chunk * kHeads + h;
-  long long total, ahead;
-  attn_count_units(a, a.unit_keys, seq, total, ahead, red);
-  const int units = (attn_length(a, seq) + a.unit_keys - 1) / a.unit_keys;
+  const int share = attn_share(a, a.unit_keys);
+  const int pieces = attn_pieces(attn_units(a, seq, a.unit_keys), share);
+  const int slot = pieces < 2 ? 0
+                              : (attn_sum(seq, [&](int b) {
+                                  const int n = attn_pieces(attn_units(a, b, a.unit_keys), share);
+                                  return n > 1 ? n : 0;
+                                })) * per + hc * pieces;
   const int team = threadIdx.x / kLanes, d = 4 * (threadIdx.x - team * kLanes);
   griddep_wait();
-  if (units == 0) {
+  if (pieces == 0) {
     if (team == 0) *reinterpret_cast<uint2*>(a.out + at * D + d) = make_uint2(0, 0);
     if (a.lse && threadIdx.x == 0) a.lse[at] = -kInf;
     return;
   }
-  const long long share = attn_share(total, a.blocks), u0 = ahead + static_cast<long long>(hc) * units;
-  const int c0 = static_cast<int>(u0 / share), c1 = static_cast<int>((u0 + units - 1) / share);
-  if (c0 == c1) return;
-  // the head begins in block c0 (its slot 1) and covers the start of the others (their slot 0)
-  auto part_of = [&](int c) { return a.parts + (2 * static_cast<size_t>(c) + (c == c0 ? 1 : 0)) * kHeads * (D + 2); };
+  if (pieces == 1) return;
+  auto part_of = [&](int c) { return a.parts + static_cast<size_t>(slot + c) * kHeads * (D + 2); };
   float top = -kInf;
-  for (int c = c0 + static_cast<int>(threadIdx.x & 31); c <= c1; c += 32) top = fmaxf(top, part_of(c)[kHeads * D + 2 * h]);
+  for (int c = threadIdx.x & 31; c < pieces; c += 32) top = fmaxf(top, part_of(c)[kHeads * D + 2 * h]);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
   const float base = top == -kInf ? 0.0f : top;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float l = 0.0f;
 #pragma unroll 4
-  for (int c = c0 + team; c <= c1; c += kTeams) {
+  for (int c = team; c < pieces; c += kTeams) {
     const float* part = part_of(c);
     const float2 ml = *reinterpret_cast<const float2*>(part + kHeads * D + 2 * h);
     const float4 x4 = *reinterpret_cast<const float4*>(part + h * D + d);

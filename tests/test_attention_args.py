@@ -77,7 +77,7 @@ def attend(L, q=p, stride=1024, table=p, tstride=4, pages=4, lengths=p, seqs=2, 
 @pytest.mark.parametrize("change,code", [
     ({"q": None}, 1000), ({"table": None}, 1000), ({"lengths": None}, 1000), ({"out": None}, 1000), ({"heads": 0}, 1000), ({"heads": 3}, 1001),
     ({"seqs": -1}, 1000), ({"pages": 0}, 1000), ({"tstride": 3}, 1000), ({"stride": 504}, 1000), ({"stride": 1028}, 1002), ({"q": P(4100)}, 1002),
-    ({"out": P(4100)}, 1002), ({"ws": P(4100)}, 1002), ({"pages": 1 << 26, "tstride": 1 << 26}, 1001), ({"seqs": 1 << 30}, 1001),
+    ({"out": P(4100)}, 1002), ({"ws": P(4100)}, 1002), ({"pages": 1 << 26, "tstride": 1 << 26}, 1001), ({"seqs": 1 << 30}, 1001), ({"seqs": 1 << 28}, 1001), ({"seqs": 1 << 20, "pages": 1 << 17, "tstride": 1 << 17}, 1001),
     ({"seqs": 0}, 0),
 ])
 def test_attention_refuses(L, change, code):
@@ -85,10 +85,11 @@ def test_attention_refuses(L, change, code):
 
 
 def test_workspace_grows_to_the_resident_blocks(L):
+    """Nothing for heads that are never cut, and never more than the resident blocks' parts."""
     lib = L.lib()
     sizes = [lib.mxfp4_paged_attention_workspace_bytes(ctypes.byref(cache_of(L, heads=8, pages=1 << 20)), b, 64, n)
              for b, n in ((1, 1), (1, 64), (16, 64), (64, 4096))]
-    assert all(s > 0 and s % 16 == 0 for s in sizes) and sizes == sorted(sizes) and sizes[-1] < 64 << 20
+    assert sizes[0] == 0 and all(s % 16 == 0 for s in sizes) and 0 < sizes[1] <= sizes[2] <= sizes[3] < 64 << 20
 
 
 def test_python_entry_points_refuse_what_is_not_on_a_gpu():
