@@ -754,9 +754,12 @@ int rope_args(RowArgs* a, const void* qkv, long long row_stride, int tokens, int
 // The attention kernel's pieces: about as many as blocks are resident (the kernel's launch bound, so
 // this needs no query and holds without a device: 148 SMs then), and a head's last piece may
 // be a short one: up to target + heads blocks.  Heads of more than one piece have at most 2 * target.
+//
+// `cluster` blocks to a head instead, where the page table bounds a head at kAttnClusterSteps units to each
+// of them: as many (a power of two up to 8) as the longest sequence has units and the SMs have room for.
 struct AttnPlan {
-  int nt, chunks, target, blocks, unit_keys;
-  size_t bytes;
+  int nt, chunks, target, blocks, unit_keys, cluster;
+  size_t parts_at, bytes;  // the workspace: a word pair per head, then the parts
 };
 AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int max_pages, int page_size, int sm_count) {
   AttnPlan p;
@@ -769,7 +772,13 @@ AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int ma
   const long long resident = 1ll * sm_count * attn_resident(dim, fmt, p.nt) * kAttnPieces;
   p.target = static_cast<int>(std::min(units, resident));
   p.blocks = static_cast<int>(std::min(units, resident + heads));
-  p.bytes = keys > p.unit_keys ? static_cast<size_t>(p.target) * 2 * 8 * p.nt * (dim + 2) * sizeof(float) : 0;
+  const long long most = (keys + p.unit_keys - 1) / p.unit_keys;  // units of a head
+  int c = 1;
+  while (c < 8 && c < most && 2 * c * heads <= resident) c *= 2;
+  p.cluster = most <= kAttnClusterSteps * c && heads * c < (1ll << 30) ? c : 0;
+  if (p.cluster) p.blocks = static_cast<int>(heads * c);
+  p.parts_at = (static_cast<size_t>(heads) * sizeof(int2) + 15) / 16 * 16;
+  p.bytes = p.cluster ? 0 : p.parts_at + static_cast<size_t>(p.target) * 2 * 8 * p.nt * (dim + 2) * sizeof(float);
   return p;
 }
 
@@ -782,9 +791,22 @@ int launch_attention(const AttnArgs& a, int blocks, DeviceState* d, cudaStream_t
     if (e != cudaSuccess) return ret(e);
     done.store(true, std::memory_order_release);
   }
+  if (a.cluster > 1) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(kAttnThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {static_cast<unsigned>(a.cluster), 1, 1};
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return ret(cudaLaunchKernelEx(&cfg, attn_kernel<D, kFmt, NT>, a));
+  }
   attn_kernel<D, kFmt, NT><<<blocks, kAttnThreads, smem, s>>>(a);
   const int rc = launch_status();
-  if (rc) return rc;
+  if (rc || a.cluster) return rc;
   return launch_pdl_grid(attn_join_kernel<D, NT>, dim3(a.seqs * a.cache.heads * a.chunks, std::min(8 * NT, a.group)), kAttnThreads, 0, s, a);
 }
 
@@ -1153,7 +1175,8 @@ int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cach
   a.lengths = lengths, a.seqs = seqs, a.q_heads = num_heads, a.group = num_heads / a.cache.heads, a.chunks = p.chunks;
   a.scale = scale;
   a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
-  a.parts = static_cast<float*>(workspace), a.target = p.target, a.unit_keys = p.unit_keys;
+  a.heads = static_cast<int2*>(workspace);
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + (p.bytes ? p.parts_at : 0)), a.target = p.target, a.unit_keys = p.unit_keys, a.cluster = p.cluster;
   auto s = static_cast<cudaStream_t>(stream);
   return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p.nt, p.blocks, d, s) : launch_attention_dim<kFmtE2M1>(a, p.nt, p.blocks, d, s);
 }

@@ -30,6 +30,9 @@
 // found from the lengths on the device, so that long and short sequences share the GPU evenly and a
 // block's first loads run beside the other blocks' work.  A head of one piece is written at
 // once; the parts of the others go to the workspace and attn_join_kernel adds them in order.
+// Where even the longest sequence that the page table can hold is a few units, a cluster of 1 to 8
+// blocks takes a head instead and joins its parts through distributed shared memory: one launch, no
+// workspace, and each block looks at the length of its own sequence only.
 #pragma once
 
 #include <type_traits>
@@ -42,7 +45,8 @@ namespace mxb {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr int kAttnPieces = 1;  // pieces per resident block
+constexpr int kAttnPieces = 1;        // pieces per resident block
+constexpr int kAttnClusterSteps = 16; // units to a block of a cluster, at most
 
 // Tiles of 16 keys a warp takes in one step; steps in its ring; blocks resident per SM (the kernel's
 // launch bound).
@@ -60,7 +64,7 @@ __host__ __device__ constexpr int attn_tile_bytes(int dim, int fmt) {
 }
 __host__ __device__ constexpr int attn_smem_bytes(int dim, int fmt, int nt) {
   const int ring = kAttnWarps * attn_ring(dim, fmt) * attn_tiles(dim, fmt) * attn_tile_bytes(dim, fmt);
-  const int join = kAttnWarps * 8 * nt * (dim + 4 + 2) * 4;  // the warps' parts, after the ring
+  const int join = 8 * nt * (kAttnWarps * (dim + 4 + 2) + 2) * 4;  // the warps' parts, after the ring
   return ring > join ? ring : join;
 }
 
@@ -76,9 +80,11 @@ struct AttnArgs {
   float scale;
   __nv_bfloat16* out;      // [seqs][q_heads][dim]
   float* lse;              // [seqs][q_heads] or null
+  int2* heads;             // [seqs][kv heads][chunks]: pieces of each head that has any, and its first part
   float* parts;            // [2 * target][8 * NT heads][dim + 2]
   int target;              // pieces to cut the work into
   int unit_keys;
+  int cluster;             // blocks to a head, joining among themselves; 0: pieces
 };
 
 __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -311,6 +317,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
   extern __shared__ __align__(128) float sm[];                // the warps' rings; then [warps][kHeads][kStride]
   float* sm_m = sm + kAttnWarps * kHeads * kStride;           // and m, l [warps][kHeads]
   float* sm_l = sm_m + kAttnWarps * kHeads;
+  float* sm_joined = sm_l + kAttnWarps * kHeads;              // of the block: m, l [kHeads]
 
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -319,7 +326,14 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
   const uint32_t base_k = attn_copy_base<D, kFmt, false>(), base_v = attn_copy_base<D, kFmt, true>();
 
   AttnPiece me;
-  if (!attn_find(a, kUnitKeys, attn_share(a, kUnitKeys), blockIdx.x, me)) return;
+  if (a.cluster) {
+    const int per = a.cache.heads * a.chunks, all = blockIdx.x / a.cluster;
+    me.of = a.cluster, me.index = blockIdx.x - all * a.cluster;
+    me.seq = all / per, me.head_chunk = all - me.seq * per;
+    me.slot = 0;
+  } else if (!attn_find(a, kUnitKeys, attn_share(a, kUnitKeys), blockIdx.x, me)) {
+    return;
+  }
   {
     const int seq = me.seq, len = attn_length(a, seq), units = attn_units(a, seq, kUnitKeys);
     const int first = static_cast<int>(static_cast<long long>(units) * me.index / me.of);  // units first .. last - 1
@@ -580,7 +594,9 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
       }
     __syncthreads();
     const bool whole = me.of == 1;
-    float* part = a.parts + static_cast<size_t>(me.slot) * kHeads * (D + 2);
+    if (!a.cluster && me.index == 0 && threadIdx.x == 0)
+      a.heads[static_cast<size_t>(seq) * a.cache.heads * a.chunks + me.head_chunk] = make_int2(me.of, me.slot);
+    float* part = a.cluster ? nullptr : a.parts + static_cast<size_t>(me.slot) * kHeads * (D + 2);
     for (int i = threadIdx.x; i < nh * (D / 4); i += kAttnThreads) {
       const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
       float top = -kInf;
@@ -604,10 +620,37 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
         o2.x = pack_bf16x2(o.x * r, o.y * r), o2.y = pack_bf16x2(o.z * r, o.w * r);
         *reinterpret_cast<uint2*>(a.out + at * D + d) = o2;
         if (a.lse && d == 0) a.lse[at] = l == 0.0f ? -kInf : (top + log2f(l)) * 0.6931471805599453f;
+      } else if (a.cluster) {
+        // over the first warp's part, which no other thread reads here
+        *reinterpret_cast<float4*>(sm + h * kStride + d) = o;
+        if (d == 0) sm_joined[h] = top, sm_joined[kHeads + h] = l;
       } else {
         *reinterpret_cast<float4*>(part + h * D + d) = o;
         if (d == 0) part[kHeads * D + 2 * h] = top, part[kHeads * D + 2 * h + 1] = l;
       }
+    }
+    if (a.cluster > 1) {  // every block of the cluster gets here: none returns before
+      cluster_sync_all();
+      for (int i = me.index * kAttnThreads + threadIdx.x; i < nh * (D / 4); i += a.cluster * kAttnThreads) {
+        const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
+        float top = -kInf;
+        for (int c = 0; c < a.cluster; ++c) top = fmaxf(top, ld_dsmem_f32(sm_joined + h, c));
+        const float base = top == -kInf ? 0.0f : top;
+        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
+        for (int c = 0; c < a.cluster; ++c) {
+          const float f = exp2_approx(ld_dsmem_f32(sm_joined + h, c) - base);
+          l = fmaf(ld_dsmem_f32(sm_joined + kHeads + h, c), f, l);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = fmaf(ld_dsmem_f32(sm + h * kStride + d + j, c), f, o[j]);
+        }
+        const float r = l == 0.0f ? 0.0f : 1.0f / l;
+        const size_t at = static_cast<size_t>(seq) * a.q_heads + h0 + h;
+        uint2 o2;
+        o2.x = pack_bf16x2(o[0] * r, o[1] * r), o2.y = pack_bf16x2(o[2] * r, o[3] * r);
+        *reinterpret_cast<uint2*>(a.out + at * D + d) = o2;
+        if (a.lse && d == 0) a.lse[at] = l == 0.0f ? -kInf : (top + log2f(l)) * 0.6931471805599453f;
+      }
+      cluster_sync_all();  // the others may still read this block's part
     }
   }
 }
@@ -626,20 +669,16 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const __grid_co
   const int head = hc / a.chunks, chunk = hc - head * a.chunks, h = blockIdx.y;
   if (h >= a.group - chunk * kHeads) return;
   const size_t at = static_cast<size_t>(seq) * a.q_heads + head * a.group + chunk * kHeads + h;
-  const int share = attn_share(a, a.unit_keys);
-  const int pieces = attn_pieces(attn_units(a, seq, a.unit_keys), share);
-  const int slot = pieces < 2 ? 0
-                              : (attn_sum(seq, [&](int b) {
-                                  const int n = attn_pieces(attn_units(a, b, a.unit_keys), share);
-                                  return n > 1 ? n : 0;
-                                })) * per + hc * pieces;
   const int team = threadIdx.x / kLanes, d = 4 * (threadIdx.x - team * kLanes);
+  const bool empty = attn_length(a, seq) == 0;
   griddep_wait();
-  if (pieces == 0) {
+  if (empty) {
     if (team == 0) *reinterpret_cast<uint2*>(a.out + at * D + d) = make_uint2(0, 0);
     if (a.lse && threadIdx.x == 0) a.lse[at] = -kInf;
     return;
   }
+  const int2 mine = a.heads[blockIdx.x];
+  const int pieces = mine.x, slot = mine.y;
   if (pieces == 1) return;
   auto part_of = [&](int c) { return a.parts + static_cast<size_t>(slot + c) * kHeads * (D + 2); };
   float top = -kInf;

@@ -84,12 +84,13 @@ def test_attention_refuses(L, change, code):
     assert attend(L, **change) == code
 
 
-def test_workspace_grows_to_the_resident_blocks(L):
-    """Nothing for heads that are never cut, and never more than the resident blocks' parts."""
+def test_workspace_is_none_for_short_tables_and_bounded_for_long_ones(L):
+    """Nothing where a cluster takes a head; else the resident blocks' parts and a word pair per head."""
     lib = L.lib()
-    sizes = [lib.mxfp4_paged_attention_workspace_bytes(ctypes.byref(cache_of(L, heads=8, pages=1 << 20)), b, 64, n)
-             for b, n in ((1, 1), (1, 64), (16, 64), (64, 4096))]
-    assert sizes[0] == 0 and all(s % 16 == 0 for s in sizes) and 0 < sizes[1] <= sizes[2] <= sizes[3] < 64 << 20
+    c = ctypes.byref(cache_of(L, heads=8, pages=1 << 20))
+    sizes = [lib.mxfp4_paged_attention_workspace_bytes(c, b, 64, n) for b, n in ((1, 1), (16, 16), (1, 4096), (64, 4096), (4096, 4096))]
+    assert sizes[0] == sizes[1] == 0 and all(s % 16 == 0 for s in sizes)
+    assert 0 < sizes[2] <= sizes[3] <= sizes[4] < 64 << 20
 
 
 def test_python_entry_points_refuse_what_is_not_on_a_gpu():
