@@ -3,6 +3,7 @@
     python -m mxfp4_b200.bench [--shapes M,N,K ...] [--out results/sweep.csv]
                                [--warmup 50] [--iters 100]
     python -m mxfp4_b200.bench --quantize [K,N ...]      # GPU quantiser + prepack throughput
+    python -m mxfp4_b200.bench --attention [SEQS,HEADS,KV_HEADS,DIM,LENGTH ...]   # the attention operators
 
 Mirrors python/mxfp4_cdna3/bench.py:31-119 (_bench_one, run_sweep): seed-0 inputs
 (A ~ N(0,1) bf16, W ~ N(0,1) quantised along K), 8 rotating weight copies, one CUDA event
@@ -23,6 +24,7 @@ from pathlib import Path
 import numpy as np
 import torch
 
+from . import attention as at
 from . import cost_model as cm
 from . import kernels as kk
 
@@ -132,6 +134,65 @@ def bench_quantize(shapes, n_iter: int = 20, rule: str = "ocp") -> list[dict]:
     return out
 
 
+def bench_attention(specs, n_iter: int = 30) -> list[dict]:
+    """Norm, rotation and cache write of a prompt of LENGTH tokens, the read-back of its rows, and one token's
+    attention for SEQS sequences of LENGTH keys, in both cache formats: a CUDA graph of `n_iter` calls over two
+    copies of the inputs, microseconds and bytes each input read and each output written once."""
+    dev = torch.device("cuda:0")
+    hbm = cm.load_peaks().hbm_gbs
+    out = []
+    for seqs, heads, kv_heads, dim, length in specs:
+        page = 64
+        pages = -(-length // page)
+        gen = torch.Generator(device=dev).manual_seed(0)
+        angle = torch.arange(length, device=dev)[:, None] * 10000.0 ** (-torch.arange(0, dim, 2, device=dev) / dim)
+        cos, sin = angle.cos().float(), angle.sin().float()
+        slots = torch.arange(length, dtype=torch.int32, device=dev)
+        w = torch.ones(dim, dtype=torch.bfloat16, device=dev)
+        qkv = [torch.randn(length, (heads + 2 * kv_heads) * dim, generator=gen, device=dev).bfloat16() for _ in range(2)]
+        q = torch.randn(seqs, heads, dim, generator=gen, device=dev).bfloat16()
+        lens = torch.full((seqs,), length, dtype=torch.int32, device=dev)
+        for fmt in at.KV_FORMATS:
+            row = 2 * kv_heads * (dim // (1 if fmt == "mxfp8" else 2) + dim // 32)
+            caches = [at.new_kv_cache(seqs * pages, kv_heads, dim, page, fmt, dev) for _ in range(2)]
+            table = torch.randperm(seqs * pages, device=dev).to(torch.int32).view(seqs, pages)
+            for c in caches:  # values to read
+                for t in (c.k_codes, c.v_codes):
+                    t.random_(0, 100, generator=gen)
+                for t in (c.k_scales, c.v_scales):
+                    t.random_(117, 121, generator=gen)
+            calls = {
+                "norm_rope_cache": (lambda i: at.qk_norm_rope_cache(qkv[i], heads, kv_heads, cos, sin, caches[i], slots, q_weight=w,
+                                                                    k_weight=w),
+                                    length * (heads * dim * 4 + 2 * kv_heads * dim * 2 + row + dim * 4)),
+                "read": (lambda i: at.kv_cache_read(caches[i], slots), length * (row + 4 * kv_heads * dim)),
+                "attention": (lambda i: at.paged_attention(q, caches[i], table, lens), seqs * (length * row + 4 * heads * dim)),
+            }
+            for name, (fn, nbytes) in calls.items():
+                for i in range(2):
+                    fn(i)
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    for i in range(n_iter):
+                        fn(i & 1)
+                graph.replay()
+                torch.cuda.synchronize()
+                ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+                ev[0].record()
+                graph.replay()
+                ev[1].record()
+                torch.cuda.synchronize()
+                us = ev[0].elapsed_time(ev[1]) * 1e3 / n_iter
+                rec = {"op": name, "format": fmt, "seqs": seqs, "heads": heads, "kv_heads": kv_heads, "dim": dim, "length": length,
+                       "us": us, "gbs": nbytes / us / 1e3, "hbm_peak_gbs": hbm}
+                log.info("%s %s seqs=%d heads=%d/%d dim=%d length=%d: %.1f us %.0f GB/s (HBM copy peak %.0f)", name, fmt, seqs, heads,
+                         kv_heads, dim, length, us, rec["gbs"], hbm)
+                out.append(rec)
+                del graph
+    return out
+
+
 def summarize(rows) -> dict:
     """(strategy, M, N, K) -> p50 ns, from run_sweep rows."""
     acc: dict = {}
@@ -148,9 +209,14 @@ def main(argv=None) -> None:
     ap.add_argument("--iters", type=int, default=100)
     ap.add_argument("--quantize", nargs="*", default=None, metavar="K,N",
                     help="time the GPU quantiser and prepack on K x N fp32 weights instead of the GEMM sweep")
+    ap.add_argument("--attention", nargs="*", default=None, metavar="SEQS,HEADS,KV_HEADS,DIM,LENGTH",
+                    help="time the attention operators instead of the GEMM sweep")
     ap.add_argument("--log-level", default="INFO")
     args = ap.parse_args(argv)
     logging.basicConfig(level=args.log_level, format="%(asctime)s %(levelname)s %(name)s: %(message)s")
+    if args.attention is not None:
+        bench_attention([tuple(int(x) for x in s.split(",")) for s in (args.attention or ["1,64,8,128,4096", "32,64,8,128,4096"])])
+        return
     if args.quantize is not None:
         bench_quantize([tuple(int(x) for x in s.split(",")) for s in (args.quantize or ["3072,3072", "8192,57344"])])
         return

@@ -41,3 +41,29 @@ def ref_gemm(A: np.ndarray, B_packed: np.ndarray, B_scales: np.ndarray) -> np.nd
     """fp32 A[M, K] @ dequant(B)[K, N] on the CPU."""
     A32 = np.asarray(A, dtype=np.float32)
     return A32 @ dequantize_ref_layout(B_packed, B_scales)
+
+
+# ---- the attention operators' checkers (no counterpart in the reference), in fp64
+_E4M3 = np.array([(-1.0) ** (c >> 7) * ((c & 7) * 2.0**-9 if not c >> 3 & 15 else (1 + (c & 7) / 8) * 2.0 ** ((c >> 3 & 15) - 7))
+                  for c in range(256)])
+_E4M3[0x7F] = _E4M3[0xFF] = np.nan
+
+
+def cache_values(codes: np.ndarray, scales: np.ndarray, format: str) -> np.ndarray:
+    """What rows of an MX key-value cache stand for: codes [..., D] ("mxfp8") or [..., D / 2] ("mxfp4"),
+    scales [..., D / 32]."""
+    c = np.asarray(codes, dtype=np.uint8)
+    v = _E4M3[c] if format == "mxfp8" else _BYTE_PAIR[c].astype(np.float64).reshape(*c.shape[:-1], 2 * c.shape[-1])
+    s = np.asarray(scales, dtype=np.int64)
+    two = np.where(s == 255, np.nan, np.ldexp(1.0, s - 127))
+    return (v.reshape(*v.shape[:-1], v.shape[-1] // 32, 32) * two[..., None]).reshape(v.shape)
+
+
+def attention(q: np.ndarray, k: np.ndarray, v: np.ndarray, scale: float) -> np.ndarray:
+    """One sequence's new token: q [heads, D], k and v [n, kv_heads, D] -> [heads, D]; zeros for n = 0."""
+    n, kv_heads, dim = k.shape
+    if n == 0:
+        return np.zeros(q.shape)
+    z = np.einsum("hgd,nhd->hgn", np.asarray(q, dtype=np.float64).reshape(kv_heads, -1, dim), k) * scale
+    p = np.exp(z - z.max(-1, keepdims=True))
+    return np.einsum("hgn,nhd->hgd", p / p.sum(-1, keepdims=True), v).reshape(q.shape)

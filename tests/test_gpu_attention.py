@@ -348,6 +348,28 @@ def test_attention_over_edge_lengths(mx, fmt, dim, heads, kv, page):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,heads,kv,seqs", [(64, 4, 2, 21), (64, 24, 2, 40), (128, 3, 3, 21), (128, 12, 1, 150), (256, 10, 1, 21), (256, 2, 2, 400)])
+def test_attention_with_a_wide_page_table(mx, fmt, dim, heads, kv, seqs):
+    """A table that could hold far longer sequences: the pieces come from the lengths on the device, with few
+    heads and with more than there are blocks; entries past a sequence's pages are never read."""
+    rng = np.random.default_rng(dim + seqs)
+    lengths = (EDGES * 20)[:seqs]
+    lengths[seqs // 2] = 5000
+    page = 32
+    cache = random_cache(mx, rng, sum(-(-n // page) for n in lengths) + 1, kv, dim, page, fmt)
+    table = random_table(rng, cache, lengths)
+    wide = np.full((seqs, 9000), 2**30)  # 288000 keys
+    wide[:, :table.shape[1]] = table
+    q = bf16(rng, (seqs, heads, dim))
+    out, lse = mx.paged_attention(q, cache, i32(wide), i32(lengths), return_lse=True)
+    check_attention(out, lse, q, cache, table, lengths, dim ** -0.5)
+    again, lse2 = mx.paged_attention(q, cache, i32(wide), i32(lengths), return_lse=True)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    none, lse = mx.paged_attention(q, cache, i32(wide), i32([0] * seqs), return_lse=True)
+    assert (none == 0).all() and (lse == -float("inf")).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("seqs,longest,dim,heads,kv", [(1, 40000, 128, 16, 2), (3, 9000, 64, 8, 1), (300, 200, 128, 4, 4),
                                                        (2, 6000, 256, 4, 1), (40, 3000, 128, 24, 2)])
 def test_attention_split_and_joined(mx, fmt, seqs, longest, dim, heads, kv):

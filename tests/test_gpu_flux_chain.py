@@ -59,3 +59,40 @@ def test_flux_chain_matches_cpu_chain(mx):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(chain.out, first)
+
+
+def test_flux_chain_with_norm_and_rotation(mx):
+    """The chain with the block's query and key norms and its rotation, at a small size: sampled rows
+    against the CPU chain, the keys, and a replayed graph."""
+    from mxfp4_b200.flux import FluxChain, QKTurn, reference_rows, turn_rows
+
+    M, d, heads = 300, 256, 4
+    g = torch.Generator(device="cuda").manual_seed(3)
+    weights, deq = [], []
+    for N, K in ((3 * d, d), (d, d), (4 * d, d), (d, 4 * d)):
+        W = torch.randn((K, N), generator=g, device="cuda") * 0.05
+        Bp, Bs = mx.quantize_mxfp4(W, axis=0, rule="ocp")
+        weights.append(mx.prepack_b200(Bp, Bs))
+        deq.append(o.dequantize_mxfp4(Bp.cpu().numpy(), Bs.cpu().numpy(), axis=0))
+    x0 = torch.randn((M, d), generator=g, device="cuda").to(torch.bfloat16)
+    qw, kw = ((1 + torch.randn(d // heads, generator=g, device="cuda") / 4).bfloat16() for _ in range(2))
+    angle = torch.rand((M, d // heads // 2), generator=g, device="cuda") * 100
+    turn = QKTurn(heads, qw, kw, angle.cos(), angle.sin())
+    chain = FluxChain(weights, x0, turn)
+    first = chain.forward().clone()
+    torch.cuda.synchronize()
+    x = x0.float().cpu().numpy()
+    cos, sin = turn.cos.cpu().numpy(), turn.sin.cpu().numpy()
+    want = reference_rows(x, deq, turn=lambda q: turn_rows(q, heads, qw.float().cpu().numpy(), cos, sin))
+    assert rel_err(first.float().cpu().numpy(), want) <= 1e-2
+    keys = turn_rows(chain.qkv[:, d:2 * d].float().cpu().numpy(), heads, kw.float().cpu().numpy(), cos, sin)
+    assert rel_err(chain.k.view(M, d).float().cpu().numpy(), keys) <= 2.0**-8
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain.forward()
+    chain.out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(chain.out, first)
+    with pytest.raises(ValueError):
+        FluxChain(weights, x0, QKTurn(3, qw, kw, turn.cos, turn.sin))

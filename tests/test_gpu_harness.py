@@ -68,3 +68,20 @@ def test_quantize_bench_runs():
 
     rows = bench.bench_quantize([(256, 384)], n_iter=2)
     assert rows[0]["quantize_gbs"] > 0 and rows[0]["prepack_gbs"] > 0
+
+
+def test_validate_attention():
+    from mxfp4_b200 import validate
+
+    assert validate.validate_attention(3, 8, 2, 64, 150)
+    with pytest.raises(SystemExit) as e:
+        validate.main(["--attention", "2,16,1,128,70", "1,4,4,256,20", "--log-level", "WARNING"])
+    assert e.value.code == 0
+
+
+def test_attention_bench_runs():
+    from mxfp4_b200 import bench
+
+    rows = bench.bench_attention([(2, 8, 2, 64, 100)], n_iter=2)
+    assert {(r["op"], r["format"]) for r in rows} == {(o, f) for o in ("norm_rope_cache", "read", "attention") for f in ("mxfp8", "mxfp4")}
+    assert all(r["us"] > 0 and r["gbs"] > 0 for r in rows)
