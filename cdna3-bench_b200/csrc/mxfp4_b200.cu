@@ -758,7 +758,7 @@ int rope_args(RowArgs* a, const void* qkv, long long row_stride, int tokens, int
 // `cluster` blocks to a head instead, where the page table bounds a head at kAttnClusterSteps units to each
 // of them: as many (a power of two up to 8) as the longest sequence has units and the SMs have room for.
 struct AttnPlan {
-  int nt, chunks, target, blocks, unit_keys, cluster;
+  int nt, chunks, target, fit, blocks, unit_keys, cluster;
   size_t parts_at, bytes;  // the workspace: a word pair per head, then the parts
 };
 AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int max_pages, int page_size, int sm_count) {
@@ -769,9 +769,12 @@ AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int ma
   p.unit_keys = attn_unit_keys(dim, fmt);
   const long long keys = static_cast<long long>(max_pages) * page_size, heads = static_cast<long long>(seqs) * kv_heads * p.chunks;
   const long long units = (keys + p.unit_keys - 1) / p.unit_keys * heads;
-  const long long resident = 1ll * sm_count * attn_resident(dim, fmt, p.nt) * kAttnPieces;
-  p.target = static_cast<int>(std::min(units, resident));
-  p.blocks = static_cast<int>(std::min(units, resident + heads));
+  const long long resident = 1ll * sm_count * attn_resident(dim, fmt, p.nt);
+  p.fit = 2 * heads <= resident;
+  const long long target = std::min(units, p.fit ? resident : resident * kAttnPieces);
+  p.fit = p.fit && heads < target;
+  p.target = static_cast<int>(target);
+  p.blocks = static_cast<int>(std::min(units, target + heads));
   const long long most = (keys + p.unit_keys - 1) / p.unit_keys;  // units of a head
   int c = 1;
   while (c < 8 && c < most && 2 * c * heads <= resident) c *= 2;
@@ -1176,7 +1179,7 @@ int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cach
   a.scale = scale;
   a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
   a.heads = static_cast<int2*>(workspace);
-  a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + (p.bytes ? p.parts_at : 0)), a.target = p.target, a.unit_keys = p.unit_keys, a.cluster = p.cluster;
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + (p.bytes ? p.parts_at : 0)), a.target = p.target, a.fit = p.fit, a.unit_keys = p.unit_keys, a.cluster = p.cluster;
   auto s = static_cast<cudaStream_t>(stream);
   return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p.nt, p.blocks, d, s) : launch_attention_dim<kFmtE2M1>(a, p.nt, p.blocks, d, s);
 }

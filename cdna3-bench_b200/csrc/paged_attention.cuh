@@ -45,7 +45,7 @@ namespace mxb {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr int kAttnPieces = 1;        // pieces per resident block
+constexpr int kAttnPieces = 2;        // pieces per resident block, where the heads are many
 constexpr int kAttnClusterSteps = 16; // units to a block of a cluster, at most
 
 // Tiles of 16 keys a warp takes in one step; steps in its ring; blocks resident per SM (the kernel's
@@ -83,6 +83,7 @@ struct AttnArgs {
   int2* heads;             // [seqs][kv heads][chunks]: pieces of each head that has any, and its first part
   float* parts;            // [2 * target][8 * NT heads][dim + 2]
   int target;              // pieces to cut the work into
+  int fit;                 // heads are few: no more pieces than that
   int unit_keys;
   int cluster;             // blocks to a head, joining among themselves; 0: pieces
 };
@@ -149,7 +150,7 @@ __device__ __forceinline__ int attn_share(const AttnArgs& a, int unit_keys) {
   const long long per = static_cast<long long>(a.cache.heads) * a.chunks, heads = per * a.seqs;
   const long long total = per * attn_sum(a.seqs, [&](int b) { return attn_units(a, b, unit_keys); });
   int lo = max(1, ceil_ratio(total, a.target));
-  if (2 * heads <= a.target) {
+  if (a.fit) {
     // with total / share + heads <= target there are enough
     int hi = max(lo, ceil_ratio(total, a.target - static_cast<int>(heads)));
     while (lo < hi) {
