@@ -1,6 +1,6 @@
 // Python binding of the attention operators (mxfp4_b200/attention.py): argument checks, output and
 // workspace allocation and the C call in one step, for calls whose work on the GPU is a few
-// microseconds (measured per call, checks in Python and ctypes against this: 18 -> 8 us for
+// microseconds (measured per call, checks in Python and ctypes against this: 17 to 21 -> 9 us for
 // qk_norm_rope).  The C entries' addresses come from the library that _lib.py loaded, so that
 // both bindings call the same one.
 #include <Python.h>

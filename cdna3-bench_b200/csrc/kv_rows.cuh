@@ -440,6 +440,14 @@ __device__ __forceinline__ void cp_async_wait() {
 // 24th bit would pick the neighbouring code, and with it the stored byte would depend on how
 // the norm's sum was ordered.  store_keys settles almost all of them in 32 bits.
 //
+// Measured: 4608 tokens of 24 + 24 heads of 128, interleaved: 23.8 us, 4.8 TB/s, 73 % of the HBM copy
+// rate; a set of 4 rows is 153 instructions and a warp's start 414, so it is bound by issue and by the
+// short lives of its warps as much as by bytes.  4096 tokens of 64 + 8 + 8 heads with the cache
+// write: 44 us, 3.5 TB/s, 54 %: the keys' intervals and codes are 370 instructions per two rows.
+// 64-thread blocks against 128: 24.7 and 27.8 us on the first; 8 values to a lane with the partner
+// brought by shuffles: 26.4 us there and 62 us against 54 on the second; a persistent ring over the
+// tokens: no faster (33 and 71 us), its bookkeeping costs what it hides.
+//
 // Two tokens of one launch that name the same slot: the later one is stored (every block looks
 // through the slots behind its own; the caller keeps a launch to 4096 tokens).
 template <int LPR, int kFmt, bool kInter>
@@ -630,6 +638,7 @@ __device__ __forceinline__ uint4 decode8(const uint2& w, float scale) {
 constexpr int kReadThreads = 128;
 constexpr int kReadRows = 4;  // rows per block, their loads in flight together
 
+// Bound by HBM: 20000 rows of 8 x 128 E4M3, k and v, 21.3 us, 5.8 TB/s, 89 % of the HBM copy rate.
 // k and v of the cache rows that `slots` names, [rows][heads][dim] bf16; a negative slot reads zeros.
 template <int kFmt>
 __global__ void __launch_bounds__(kReadThreads)

@@ -7,32 +7,42 @@
 // to a block), so the kernel is bound by the cache's bytes: 2 * D * (8 or 4) / 8 + D / 16 per key.
 // One pass: running maximum and sum of the softmax in fp32, sums of o in fp32.
 //
-// A warp works on tiles of 16 keys and holds everything in registers; the codes come by plain
-// loads straight into the lanes that need them as MMA operands, so there is no shared memory and
-// no wait in the loop.  With lane = 4 g + t:
-//   scores  S^T[key][head] = K Q^T, K as the 16-row operand (m16n8k16, f16).  Lane (g, t) holds,
-//           of keys g and g + 8, the 8 values 32 b + 8 t .. + 7 of each 32-value group b.  The
+// A warp takes steps of attn_tiles tiles of 16 keys through a ring of asynchronous copies of its own
+// (16-byte copies that each lane sends for and waits for itself, then one __syncwarp: no barrier, no
+// mbarrier, nothing that could hang).  With lane = 4 g + t:
+//   scores  S^T[key][head] = K Q^T, K as the 16-row operand (m16n8k16, f16): row g is key
+//           pi(g) = g / 2 + 4 (g % 2), row g + 8 key pi(g) + 8.  Lane (g, t) holds their values 32 b + 8 t
+//           .. + 7 of each 32-value group b (any order of the values serves, if q has the same).  The
 //           codes convert exactly to f16; q is scaled per head by a power of two so that f16
 //           holds every bf16 bit of it, and each group's fp32 partial is multiplied by the key's
 //           scale.
-//   output  O^T[d][head] = V^T P^T, V as the 16-row operand (m16n8k16, bf16).  Lane (g, t) holds,
-//           of keys 2t, 2t+1, 2t+8, 2t+9, the D / 8 values from g D / 8 on: all in one 32-value
-//           group, so one scale byte per key.  The codes become bf16 by moving their fields into
-//           place, which is the value times 2^-120 (E4M3) or 2^-126 (E2M1), and one exact multiply by
-//           scale * 2^64, which leaves v * 2^-kCarry (kCarry = 56 or 62); p carries 2^kCarry.
-//           bf16 has the range for any scale below 2^64 whatever the other keys' scales are;
-//           larger ones count as 2^63.
-//           The transposition between S^T's accumulators and P^T's operand is one
-//           movmatrix per 8 keys.
+//   output  O^T[d][head] = V^T P^T, V as the 16-row operand (m16n8k16, bf16).  With pi, lane (g, t) needs
+//           keys t, t + 4, t + 8, t + 12, which lie in different banks, and holds the D / 8 values from
+//           g D / 8 on: all in one 32-value group, so one scale byte per key.  The codes become bf16 by
+//           moving their fields into place, which is the value times 2^-120 (E4M3) or 2^-126
+//           (E2M1), and one exact multiply by scale * 2^64, which leaves v * 2^-kCarry (kCarry = 56 or
+//           62); p carries 2^kCarry.  bf16 has the range for any scale below 2^64 whatever the other
+//           keys' scales are; larger ones count as 2^63.  (f16 here, with the hardware's conversion
+//           and a scale relative to a running one, measured 5 to 8 % faster and would lose weights
+//           below 2^-36 and values 2^-20 below the largest: not taken.)
+//           The transposition between S^T's accumulators and P^T's operand is one movmatrix per 8 keys.
+// What bounds it, measured: E4M3 D = 128, 8 heads to a kv head, 2 x 131072 keys: 92 % of the HBM copy
+// rate in steady state (91.5 us for 554 MB); 387 instructions per tile, of them 190 for V.  E2M1 is
+// bound by issue: 410 instructions per tile for half the bytes, 60 % of the issue slots, 55 % of the
+// copy rate.  D = 256: 97 % (E4M3) and 68 % (E2M1).  Two tiles to a step against one: 91 -> 84 us on 2 x
+// ~115k keys; three resident blocks of 167 registers against four of 127: 91 -> 87 us there.  Loads
+// straight into registers (no ring): 111 us there, 12 warps cannot both hold the bytes and compute.
 //
 // A head's keys are cut into units of kAttnWarps steps, and the heads into pieces of at most `share`
 // units, share so that there are about as many pieces as blocks are resident: one block to a piece,
 // found from the lengths on the device, so that long and short sequences share the GPU evenly and a
-// block's first loads run beside the other blocks' work.  A head of one piece is written at
+// block's first loads run beside the other blocks' work (64 ragged sequences, E2M1: 42 us; 46 with one
+// equal share of all units to a block, which then went through several heads one after another).  A head of one piece is written at
 // once; the parts of the others go to the workspace and attn_join_kernel adds them in order.
 // Where even the longest sequence that the page table can hold is a few units, a cluster of 1 to 8
 // blocks takes a head instead and joins its parts through distributed shared memory: one launch, no
-// workspace, and each block looks at the length of its own sequence only.
+// workspace, and each block looks at the length of its own sequence only (one sequence of 700 keys: 7.1 us
+// against 7.8; 200 of up to 500: 31 us against 67, which also paid for the joining kernel's blocks).
 #pragma once
 
 #include <type_traits>
@@ -45,8 +55,12 @@ namespace mxb {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-constexpr int kAttnPieces = 2;        // pieces per resident block, where the heads are many
-constexpr int kAttnClusterSteps = 16; // units to a block of a cluster, at most
+// Pieces per resident block, where the heads are many: 1, 2, 3, 4 measured 66, 62, 60, 64 us on 32 x 4096 keys
+// (E4M3, 8 kv heads), 44, 42, 43, 45 us on 64 ragged sequences (E2M1).
+constexpr int kAttnPieces = 2;
+// Units to a block of a cluster, at most: 4, 8, 16, 32 measured 64, 48, 48, 48 us on 256 sequences of up to
+// 1000 keys, 26, 26, 26, 41 us on 16 of up to 8192.
+constexpr int kAttnClusterSteps = 16;
 
 // Tiles of 16 keys a warp takes in one step; steps in its ring; blocks resident per SM (the kernel's
 // launch bound).

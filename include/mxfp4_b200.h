@@ -81,8 +81,9 @@ int mxfp4_abi_version(void);
 /* Device properties (replaces the reference's device_info, csrc/mxfp4_ext.cpp:156-168). */
 int mxfp4_device_info_get(int device, mxfp4_device_info* out);
 
-/* Reads the device error word that bounded waits inside the kernels set when they give up
- * (0 = none); clears it when `clear` is non-zero.  Synchronises the device. */
+/* Reads the device error word that bounded waits inside the kernels set when they give up, and the
+ * attention operators' kernels when they meet an index out of range (0 = none; the first code
+ * stays); clears it when `clear` is non-zero.  Synchronises the device. */
 int mxfp4_device_error(int clear, unsigned int* code_out);
 
 const char* mxfp4_error_string(int code);
@@ -272,8 +273,8 @@ int mxfp4_qk_norm_rope(const void* qkv, long long row_stride, int tokens, int nu
 
 /* The same pass with the keys (normed, rotated, then coded without a rounding in between) and the
  * values written into `cache` (its num_kv_heads and head_dim) at slots[token]; a negative slot
- * stores nothing.  Of two tokens with the same slot the later one is stored.  The key path runs
- * in 64 bits, so the stored bytes do not depend on how a sum was ordered. */
+ * stores nothing.  Of two tokens with the same slot the later one is stored.  The stored codes are
+ * those of the key computed in 64 bits, so they do not depend on how a sum was ordered. */
 int mxfp4_qk_norm_rope_cache(const void* qkv, long long row_stride, int tokens, int num_heads, const float* cos,
                              const float* sin, int table_rows, int rot, int interleaved, const int* positions,
                              const void* q_weight, const void* k_weight, int weight_dtype, double eps, void* q_out,
@@ -297,7 +298,9 @@ int mxfp4_kv_cache_read(const mxfp4_kv_cache* cache, const int* slots, int token
  * sequence's last page are not read.
  * q bf16 [seqs] rows of num_heads * head_dim, q_stride elements apart (a multiple of 8); out bf16
  * [seqs][num_heads][head_dim]; page_table rows page_stride ints apart.  Results do not depend on
- * timing: the same call gives the same bits. */
+ * timing: the same call gives the same bits.
+ * Unsupported shape (1001): max_pages * page_size of 2^31 and more, seqs * num_heads of 2^30 and
+ * more, seqs * max_pages * page_size of 2^36 and more. */
 size_t mxfp4_paged_attention_workspace_bytes(const mxfp4_kv_cache* cache, int seqs, int num_heads, int max_pages);
 int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cache* cache, const int* page_table,
                           long long page_stride, int max_pages, const int* lengths, int seqs, int num_heads,
