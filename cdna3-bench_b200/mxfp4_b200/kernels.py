@@ -448,7 +448,8 @@ def device_info(dev_id=0) -> dict:
 
 
 def device_error(clear: bool = True) -> int:
-    """Device error word set by a kernel's bounded wait giving up (0 = none)."""
+    """Device error word set by a kernel's bounded wait giving up or by an attention operator's index out of
+    range (0 = none)."""
     code = ctypes.c_uint(0)
     _lib.check(_lib.lib().mxfp4_device_error(int(clear), ctypes.byref(code)), "mxfp4_device_error")
     return code.value

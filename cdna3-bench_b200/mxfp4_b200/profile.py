@@ -2,6 +2,8 @@
 
     # run one entry point `--iters` times (wrap the command in ncu)
     python -m mxfp4_b200.profile one --path tc --M 4608 --N 9216 --K 3072
+    # the same for an attention operator
+    python -m mxfp4_b200.profile attention --op attention --format mxfp8 --seqs 2 --length 131072
     # summarise a launch list (ncu --metrics gpu__time_duration.sum --clock-control none --csv --log-file L.csv)
     python -m mxfp4_b200.profile launches L.csv
     # summarise a capture (ncu -i R.ncu-rep --page raw --csv > R.csv)
@@ -146,6 +148,19 @@ def run_one(path: str, M: int, N: int, K: int, iters: int, seed: int) -> None:
     print(f"{path} M={M} N={N} K={K} iters={iters}")
 
 
+def run_attention(op: str, fmt: str, spec, iters: int) -> None:
+    """`iters` calls of one attention operator on seeded inputs (bench.attention_calls)."""
+    import torch
+
+    from . import bench
+
+    call, nbytes = bench.attention_calls(*spec, fmt)[op]
+    for i in range(iters):
+        call(i & 1)
+    torch.cuda.synchronize()
+    print(f"{op} {fmt} seqs,heads,kv_heads,dim,length={','.join(map(str, spec))} iters={iters} bytes={nbytes}")
+
+
 def main(argv=None) -> None:
     ap = argparse.ArgumentParser()
     sub = ap.add_subparsers(dest="cmd", required=True)
@@ -157,6 +172,11 @@ def main(argv=None) -> None:
     one.add_argument("--K", type=int, required=True)
     one.add_argument("--iters", type=int, default=10)
     one.add_argument("--seed", type=int, default=0)
+    an = sub.add_parser("attention")
+    an.add_argument("--op", default="attention", choices=["attention", "norm_rope_cache", "read"])
+    an.add_argument("--format", default="mxfp8", choices=["mxfp8", "mxfp4"])
+    for name, default in (("seqs", 2), ("heads", 64), ("kv-heads", 8), ("dim", 128), ("length", 4096), ("iters", 3)):
+        an.add_argument(f"--{name}", type=int, default=default)
     la = sub.add_parser("launches")
     la.add_argument("csv")
     rw = sub.add_parser("raw")
@@ -164,6 +184,8 @@ def main(argv=None) -> None:
     args = ap.parse_args(argv)
     if args.cmd == "one":
         run_one(args.path, args.M, args.N, args.K, args.iters, args.seed)
+    elif args.cmd == "attention":
+        run_attention(args.op, args.format, (args.seqs, args.heads, args.kv_heads, args.dim, args.length), args.iters)
     elif args.cmd == "launches":
         with open(args.csv) as f:
             print(launch_table(parse_launches(f.read())))
