@@ -239,33 +239,44 @@ __device__ __forceinline__ void turn_row16(const RowArgs& a, uint4 (&x)[2], cons
   uint64_t v2[8], y2[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v2[i] = pack_f32x2(v[2 * i], v[2 * i + 1]);
+  if (norm) {
+    auto mean_square = [&](float eps) {
+      uint64_t s2 = mul_f32x2(v2[0], v2[0]);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) s2 = fma_f32x2(v2[i], v2[i], s2);
+      float ss, s1;
+      unpack_f32x2(s2, ss, s1);
+      ss += s1;
+#pragma unroll
+      for (int m = LPR / 4; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+      return fmaf(ss, static_cast<float>(a.inv_dim), eps);
+    };
+    float ms = mean_square(static_cast<float>(a.eps));
+    if (!__all_sync(0xffffffffu, ms < 0x1p120f && ms > 0x1p-90f)) {
+      // squares that leave the range of fp32, or nearly: those rows again, 2^-70 or 2^70 as large
+      const float two = ms > 0x1p-90f ? (ms < 0x1p120f ? 1.0f : 0x1p-70f) : 0x1p70f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v2[i] = mul_f32x2(v2[i], pack_f32x2(two, two));
+      ms = mean_square(static_cast<float>(a.eps * two * two));
+    }
+    const float r = rsqrtf(ms);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v2[i] = mul_f32x2(v2[i], pack_f32x2(r, r));
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) y2[i] = mul_f32x2(v2[i], pack_f32x2(q.cw[2 * i], q.cw[2 * i + 1]));
   if (rotated) {  // past the rotated part an infinity times s = 0 would be a NaN
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if constexpr (kInter) {
-        float lo, hi;
+        float lo, hi, vlo, vhi;
         unpack_f32x2(y2[i], lo, hi);
-        y2[i] = pack_f32x2(fmaf(v[2 * i + 1], q.sw[2 * i], lo), fmaf(v[2 * i], q.sw[2 * i + 1], hi));
+        unpack_f32x2(v2[i], vlo, vhi);
+        y2[i] = pack_f32x2(fmaf(vhi, q.sw[2 * i], lo), fmaf(vlo, q.sw[2 * i + 1], hi));
       } else {
         y2[i] = fma_f32x2(v2[i ^ 4], pack_f32x2(q.sw[2 * i], q.sw[2 * i + 1]), y2[i]);
       }
     }
-  }
-  if (norm) {
-    uint64_t s2 = mul_f32x2(v2[0], v2[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s2 = fma_f32x2(v2[i], v2[i], s2);
-    float ss, s1;
-    unpack_f32x2(s2, ss, s1);
-    ss += s1;
-#pragma unroll
-    for (int m = LPR / 4; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-    const float r = rsqrtf(fmaf(ss, static_cast<float>(a.inv_dim), static_cast<float>(a.eps)));
-    const uint64_t r2 = pack_f32x2(r, r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y2[i] = mul_f32x2(y2[i], r2);
   }
   uint32_t o[8];
 #pragma unroll
@@ -390,25 +401,34 @@ __device__ __noinline__ void store_keys_exact(const RowArgs* ap, int t, int p, i
 // Where the group's exponent and all codes are the same at both
 // ends of that interval they are the 64-bit ones.  Returns false otherwise (about one call in
 // a hundred: 256 values, 2^-14 each), with nothing stored.  The whole warp.
+//
+// The bound counts roundings of normal numbers.  With r in [2^-30, 2^30] (so |x| < 2^34, and the squares
+// that fp32 loses are nothing to their sum) and T_i >= 2^-60, what a subnormal product, sum or c w can
+// be off by (2^-150 * 2^34 r) is nothing to 2^-19 r T_i >= 2^-109 either.  Other rows, one with a zero
+// among them, are left to the 64 bits; rows of zeros alone have no error.
 template <int LPR, int kFmt, bool kInter>
 __device__ __forceinline__ bool store_keys(const RowArgs& a, const uint4& x, const float (&cw)[8], const float (&sw)[8], bool here,
                                            size_t row, int at) {
   float v[8], z[8], lo[8], hi[8];
   unpack_bf16x8(x, v);
   const float r = a.k_weight ? inverse_rms<LPR>(a, v) : 1.0f;
+  const bool zeros = !__any_sync(0xffffffffu, (x.x | x.y | x.z | x.w) & 0x7FFF7FFFu);
   partner_values<LPR, kInter>(a, x, v, z);
   // values that no rounding touches (past the rotated part, without a norm) are their own interval
-  const float off = a.k_weight || at < a.rot ? r * 1.9073486328125e-6f : 0.0f;
-  float top_lo = 0.0f, top_hi = 0.0f;
-  bool ok = true;
+  const bool rounded = a.k_weight || at < a.rot;
+  const float off = rounded ? r * 0x1p-19f : 0.0f;
+  float top_lo = 0.0f, top_hi = 0.0f, least = 1.0f;
+  bool ok = r >= 0x1p-30f && r <= 0x1p30f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float u = z[i] * sw[i], y = fmaf(v[i], cw[i], u) * r, e = fmaf(fabsf(v[i]), fabsf(cw[i]), fabsf(u)) * off;
+    const float u = z[i] * sw[i], y = fmaf(v[i], cw[i], u) * r, sum = fmaf(fabsf(v[i]), fabsf(cw[i]), fabsf(u)), e = sum * off;
+    least = fminf(least, sum);
     lo[i] = y - e, hi[i] = y + e;
     top_lo = fmaxf(top_lo, fabsf(y) - e);
     top_hi = fmaxf(top_hi, fabsf(y) + e);
     ok &= fabsf(y) + e < 3.0e38f;  // infinities and NaN are left to the exact path
   }
+  ok &= least >= 0x1p-60f || zeros || !rounded;
   const uint32_t b0 = group_max(__float_as_uint(top_lo)), b1 = group_max(__float_as_uint(top_hi));
   const int byte = scale_byte<kFmt>(b1);
   const float inv = exp2_neg(byte - 127);

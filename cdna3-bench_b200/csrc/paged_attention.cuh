@@ -137,7 +137,7 @@ __device__ __forceinline__ int attn_length(const AttnArgs& a, int b) {
 }
 
 __device__ __forceinline__ int attn_units(const AttnArgs& a, int b, int unit_keys) {
-  return (attn_length(a, b) + unit_keys - 1) / unit_keys;
+  return static_cast<int>((static_cast<unsigned>(attn_length(a, b)) + unit_keys - 1) / unit_keys);
 }
 
 // Sum of f(sequence) over sequences 0 .. n - 1 (below 2^31: so is the number of all units).  Every
@@ -155,7 +155,9 @@ __device__ __forceinline__ int ceil_ratio(long long a, int b) {
 }
 
 // Pieces of each head of a sequence.
-__device__ __forceinline__ int attn_pieces(int units, int share) { return (units + share - 1) / share; }
+__device__ __forceinline__ int attn_pieces(int units, int share) {
+  return static_cast<int>((static_cast<unsigned>(units) + share - 1) / share);
+}
 
 // Most units of a piece.  All units over the pieces wanted; where the heads are few, the least with
 // which the pieces are no more than wanted, so that they all run at once (rounding up leaves up to one
@@ -545,7 +547,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
           const float p2 = exp2_approx(s[i][n][2] - sub[n][0]), p3 = exp2_approx(s[i][n][3] - sub[n][1]);
           lsum[n][0] += p0 + p2;
           lsum[n][1] += p1 + p3;
-          // p is rounded to bf16 for the product (relative 2^-9 each, of either sign); the sum is not
+          // p is rounded to bf16 for the product (relative 2^-8 each at most, of either sign); the sum is not
           p[i][n][0] = transpose8x8(pack_bf16x2(p0, p1));
           p[i][n][1] = transpose8x8(pack_bf16x2(p2, p3));
         }

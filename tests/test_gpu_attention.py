@@ -245,6 +245,55 @@ def test_norm_rope_cache_is_byte_exact(mx, fmt, heads, kv, dim, rot, inter, norm
         np.testing.assert_array_equal(codes.cpu().numpy(), want_c)
 
 
+def range_rows(rng, heads, dim):
+    """One token per power of two, squares of whose values fp32 can and cannot hold; heads of one and of
+    mixed size, and zeros among the values."""
+    powers = np.r_[np.arange(-120, 121, 8), -31, -30, -29, 29, 30, 31, 33, 34, 35]
+    x = rng.standard_normal((len(powers), heads, dim))
+    x = np.where(np.abs(x) < 2.0**-6, 2.0**-6, x) * np.exp2(powers.astype(float))[:, None, None]
+    x[:, 1] = rng.standard_normal((len(powers), dim))
+    x[:, 2, ::5] = 0
+    x[0] = 0
+    return torch.from_numpy(x.astype(np.float32)).bfloat16().cuda()
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-6])
+@pytest.mark.parametrize("weight", [1.0, 2.0**100, 2.0**-100])
+@pytest.mark.parametrize("inter", [False, True])
+def test_norm_rope_over_the_whole_range(mx, eps, weight, inter):
+    rng = np.random.default_rng(5)
+    x = range_rows(rng, 5, 64)
+    if eps == 0:
+        x = x[1:]  # zeros have no norm then
+    cos, sin = tables(len(x), 32)
+    w = ((1 + torch.rand(64, device="cuda")) * weight).bfloat16()
+    q, k = mx.qk_norm_rope(x.flatten(1), 3, 1, cos, sin, q_weight=w, k_weight=w, eps=eps, interleaved=inter)
+    for got, rows in ((q, x[:, :3]), (k, x[:, 3:4])):
+        want, mag = ref.norm_rope(f64(rows), f64(cos), f64(sin), f64(w), eps, inter)
+        keep = (np.abs(want) > 2.0**-120) | (mag == 0)  # values that bf16 can hold to its 8 bits
+        close_rows(got[torch.from_numpy(keep).cuda()], want[keep], mag[keep])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("eps,weight", [(1e-6, 1.0), (1e-30, 1.0), (1e-6, 2.0**-100), (1e-30, 2.0**100), (None, 1.0)])
+@pytest.mark.parametrize("inter", [False, True])
+def test_norm_rope_cache_is_byte_exact_over_the_whole_range(mx, fmt, eps, weight, inter):
+    rng = np.random.default_rng(6)
+    x = range_rows(rng, 7, 64)  # 1 query head, 3 of each
+    n = len(x)
+    x[:, 1:4] = x[:, :3].clone()
+    cos, sin = tables(n, 32)
+    w = None if eps is None else ((1 + torch.rand(64, device="cuda")) * weight).bfloat16()
+    cache = mx.new_kv_cache(-(-n // 16), 3, 64, 16, fmt)
+    mx.qk_norm_rope_cache(x.flatten(1), 1, 3, cos, sin, cache, i32(np.arange(n)), q_weight=w, k_weight=w,
+                          eps=eps or 0.0, interleaved=inter)
+    want, _ = ref.norm_rope(f64(x[:, 1:4]), f64(cos), f64(sin), None if w is None else f64(w), eps or 0.0, inter)
+    codes, scales = ref.code_groups(want, fmt)
+    got, got_s = (t.cpu().numpy().transpose(0, 2, 1, 3).reshape(-1, 3, t.shape[-1])[:n] for t in (cache.k_codes, cache.k_scales))
+    wrong = np.unique(np.nonzero((got_s != scales).any(-1) | (got != codes).any(-1))[0])
+    assert not len(wrong), wrong
+
+
 @pytest.mark.parametrize("tokens", [2, 200, 4097, 9000])
 def test_same_slot_twice_keeps_the_later_token(mx, tokens):
     """Within one launch and across the launches a long call is cut into."""
