@@ -238,7 +238,7 @@ ENTRY(paged_attention, 8)
   const int pages = static_cast<int>(as_int(table->size(1), "max_pages"));
   const int* lengths = index_vector(args[4], seqs, c.dev, "lengths");
   const double scale = args[5] == Py_None ? 1.0 / std::sqrt(static_cast<double>(dim)) : real(args[5]);
-  if (!std::isfinite(scale)) refuse("scale must be finite");
+  if (!std::isfinite(static_cast<float>(scale))) refuse("scale must be finite in fp32");
   const c10::DeviceGuard guard(c.dev);
   at::Tensor out, lse;
   if (args[7] == Py_None) {

@@ -676,6 +676,7 @@ int cache_view(const mxfp4_kv_cache* c, KvCacheView* v, int* fmt) {
   if (c->format != MXFP4_KV_MXFP8 && c->format != MXFP4_KV_MXFP4) return MXFP4_ERR_INVALID_ARGUMENT;
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return MXFP4_ERR_UNSUPPORTED_SHAPE;
   if (!valid_page_size(c->page_size)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
+  if (static_cast<long long>(c->num_kv_heads) * c->head_dim >= (1ll << 30)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
   if (static_cast<long long>(c->num_pages) * c->page_size >= (1ll << 31)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
   if (!aligned16(c->k_codes) || !aligned16(c->v_codes) || !aligned16(c->k_scales) || !aligned16(c->v_scales))
     return MXFP4_ERR_MISALIGNED;
@@ -731,6 +732,7 @@ int rope_args(RowArgs* a, const void* qkv, long long row_stride, int tokens, int
   if ((q_weight == nullptr) != (k_weight == nullptr) || !(eps >= 0.0)) return MXFP4_ERR_INVALID_ARGUMENT;
   if (weight_dtype != MXFP4_DTYPE_F32 && weight_dtype != MXFP4_DTYPE_BF16) return MXFP4_ERR_INVALID_ARGUMENT;
   if (dim % 32 || dim > 256 || rot % 16 || rot > dim) return MXFP4_ERR_UNSUPPORTED_SHAPE;
+  if ((static_cast<long long>(q_heads) + 2ll * kv_heads) * dim >= (1ll << 30)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
   if (rot > 0 && (!cos || !sin || table_rows <= 0)) return MXFP4_ERR_INVALID_ARGUMENT;
   if (rot > 0 && !positions && table_rows < tokens) return MXFP4_ERR_INVALID_ARGUMENT;
   if (row_stride < (static_cast<long long>(q_heads) + 2ll * kv_heads) * dim) return MXFP4_ERR_INVALID_ARGUMENT;
@@ -1160,6 +1162,7 @@ int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cach
   int rc = cache_view(cache, &a.cache, &fmt);
   if (rc) return rc;
   if (seqs < 0 || num_heads <= 0 || max_pages <= 0 || page_stride < max_pages) return MXFP4_ERR_INVALID_ARGUMENT;
+  if (static_cast<long long>(num_heads) * cache->head_dim >= (1ll << 30)) return MXFP4_ERR_UNSUPPORTED_SHAPE;
   if (num_heads % a.cache.heads || static_cast<long long>(max_pages) * cache->page_size >= (1ll << 31))
     return MXFP4_ERR_UNSUPPORTED_SHAPE;
   if (static_cast<long long>(seqs) * num_heads >= (1ll << 30)) return MXFP4_ERR_UNSUPPORTED_SHAPE;

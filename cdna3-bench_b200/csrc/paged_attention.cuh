@@ -151,7 +151,7 @@ __device__ __forceinline__ int attn_sum(int n, F f) {
 }
 __device__ __forceinline__ int ceil_ratio(long long a, int b) {
   if (a < 0x7FFFFFFFll - b) return (static_cast<int>(a) + b - 1) / b;
-  return static_cast<int>(min((a + b - 1) / b, 0x7FFFFFFFll));
+  return static_cast<int>(min((a + b - 1) / b, 0x3FFFFFFFll));  // no head has more units
 }
 
 // Pieces of each head of a sequence.

@@ -50,8 +50,9 @@ class MXKVCache:
     ``k_codes`` / ``v_codes``: uint8 ``[num_pages, num_kv_heads, page_size, head_dim]`` E4M3 codes
     (``format="mxfp8"``) or ``[..., head_dim // 2]`` pairs of E2M1 codes (``"mxfp4"``, even element in
     the low nibble); ``k_scales`` / ``v_scales``: uint8 ``[..., head_dim // 32]`` E8M0 bytes.  The
-    tensors are contiguous and stay the caller's: the object only refers to them.  head_dim 64, 128
-    or 256; page_size 16, 32, 64, 128 or 256.  :func:`new_kv_cache` allocates one.
+    tensors are contiguous and stay the caller's: the object only refers to them, always to the same
+    ones (its attributes are read-only).  head_dim 64, 128 or 256; page_size 16, 32, 64, 128 or 256.
+    :func:`new_kv_cache` allocates one.
     """
 
     __slots__ = ("k_codes", "v_codes", "k_scales", "v_scales", "format", "num_pages", "num_kv_heads", "page_size",
@@ -70,13 +71,14 @@ class MXKVCache:
         _check(pages > 0 and heads > 0 and pages * size < 2**31, "num_pages * page_size must be in 1 .. 2**31 - 1")
         for t in (k_scales, v_scales):
             _check(tuple(t.shape) == (pages, heads, size, dim // 32), "scales shape")
-        self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
-        self.format, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = format, pages, heads, size, dim
-        self.device = k_codes.device
-        self._index = k_codes.get_device()
-        self._struct = _lib.KVCache(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
-                                    pages, heads, size, dim, KV_FORMATS[format])
-        self._address = ctypes.addressof(self._struct)
+        struct = _lib.KVCache(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                              pages, heads, size, dim, KV_FORMATS[format])
+        for name, value in zip(self.__slots__, (k_codes, v_codes, k_scales, v_scales, format, pages, heads, size, dim,
+                                                k_codes.device, k_codes.get_device(), struct, ctypes.addressof(struct))):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise RuntimeError("an MXKVCache refers to the same tensors for good: make another one")
 
     def nbytes(self) -> int:
         return 2 * (self.k_codes.numel() + self.k_scales.numel())
@@ -153,7 +155,8 @@ def paged_attention(q, cache: MXKVCache, page_table, lengths, scale: float | Non
     page a sequence needs are not read.  A length of zero gives a row of zeros.  ``scale`` defaults to
     ``head_dim ** -0.5``.  Returns bf16 ``[seqs, num_heads, head_dim]`` (``out`` if given), with
     ``return_lse`` also fp32 ``[seqs, num_heads]``: the natural log of the sum of exp(scale * q . k), -inf
-    for an empty sequence.  The same call gives the same bits.
+    for an empty sequence.  ``out`` may be ``q`` itself, and must not overlap it otherwise.  The same call
+    gives the same bits.
     """
     if not isinstance(cache, MXKVCache):
         raise RuntimeError("cache must be an MXKVCache")

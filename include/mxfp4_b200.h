@@ -299,8 +299,9 @@ int mxfp4_kv_cache_read(const mxfp4_kv_cache* cache, const int* slots, int token
  * q bf16 [seqs] rows of num_heads * head_dim, q_stride elements apart (a multiple of 8); out bf16
  * [seqs][num_heads][head_dim]; page_table rows page_stride ints apart.  Results do not depend on
  * timing: the same call gives the same bits.
+ * out may be q itself (q_stride == num_heads * head_dim); it must not overlap q otherwise.
  * Unsupported shape (1001): max_pages * page_size of 2^31 and more, seqs * num_heads of 2^30 and
- * more, seqs * max_pages * page_size of 2^36 and more. */
+ * more, seqs * max_pages * page_size of 2^36 and more; here and above, rows of 2^30 values and more. */
 size_t mxfp4_paged_attention_workspace_bytes(const mxfp4_kv_cache* cache, int seqs, int num_heads, int max_pages);
 int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cache* cache, const int* page_table,
                           long long page_stride, int max_pages, const int* lengths, int seqs, int num_heads,

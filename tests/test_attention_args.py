@@ -34,7 +34,8 @@ def rope(L, qkv=p, stride=1024, tokens=4, heads=4, kv=2, dim=128, cos=p, sin=p, 
     ({"cos": None}, 1000), ({"rows": 0}, 1000), ({"rows": 3}, 1000), ({"qw": p}, 1000), ({"wt": 5}, 1000), ({"eps": -1.0}, 1000),
     ({"eps": float("nan")}, 1000), ({"stride": 1016}, 1000), ({"dim": 100, "rot": 0}, 1001), ({"dim": 288, "stride": 4096}, 1001),
     ({"rot": 24}, 1001), ({"rot": 144}, 1001), ({"rot": -16}, 1000), ({"stride": 1025}, 1002), ({"qkv": P(4098)}, 1002),
-    ({"cos": P(4100)}, 1002), ({"k": P(4104)}, 1002),
+    ({"cos": P(4100)}, 1002), ({"k": P(4104)}, 1002), ({"heads": 1 << 23, "stride": 1 << 31}, 1001),
+    ({"kv": 1 << 30, "stride": 1 << 40}, 1001),
 ])
 def test_norm_rope_refuses(L, change, code):
     assert rope(L, **change) == code
@@ -42,7 +43,7 @@ def test_norm_rope_refuses(L, change, code):
 
 @pytest.mark.parametrize("change,code", [
     ({"pages": 0}, 1000), ({"heads": 0}, 1000), ({"fmt": 2}, 1000), ({"dim": 96}, 1001), ({"dim": 512}, 1001), ({"page": 48}, 1001),
-    ({"page": 8}, 1001), ({"page": 512}, 1001), ({"pages": 1 << 25}, 1001), ({"ptr": 0}, 1000), ({"ptr": 4104}, 1002),
+    ({"page": 8}, 1001), ({"page": 512}, 1001), ({"pages": 1 << 25}, 1001), ({"heads": 1 << 23}, 1001), ({"ptr": 0}, 1000), ({"ptr": 4104}, 1002),
 ])
 def test_every_cache_entry_refuses_a_bad_cache(L, change, code):
     lib, c = L.lib(), ctypes.byref(cache_of(L, **change))
@@ -78,7 +79,7 @@ def attend(L, q=p, stride=1024, table=p, tstride=4, pages=4, lengths=p, seqs=2, 
     ({"q": None}, 1000), ({"table": None}, 1000), ({"lengths": None}, 1000), ({"out": None}, 1000), ({"heads": 0}, 1000), ({"heads": 3}, 1001),
     ({"seqs": -1}, 1000), ({"pages": 0}, 1000), ({"tstride": 3}, 1000), ({"stride": 504}, 1000), ({"stride": 1028}, 1002), ({"q": P(4100)}, 1002),
     ({"out": P(4100)}, 1002), ({"ws": P(4100)}, 1002), ({"pages": 1 << 26, "tstride": 1 << 26}, 1001), ({"seqs": 1 << 30}, 1001), ({"seqs": 1 << 28}, 1001), ({"seqs": 1 << 20, "pages": 1 << 17, "tstride": 1 << 17}, 1001),
-    ({"seqs": 0}, 0),
+    ({"seqs": 0}, 0), ({"heads": 1 << 23, "stride": 1 << 30}, 1001),
 ])
 def test_attention_refuses(L, change, code):
     assert attend(L, **change) == code
@@ -158,6 +159,8 @@ def test_python_entry_points_refuse_other_forms():
         lambda: mx.paged_attention(gpu(3, 4, 64), c, gpu(2, 3, dtype=torch.int32).t(), idx),
         lambda: mx.paged_attention(gpu(3, 4, 64), c, gpu(3, 2, dtype=torch.int32), idx.long()),
         lambda: mx.paged_attention(gpu(3, 4, 64), c, gpu(3, 2, dtype=torch.int32), idx, scale=float("inf")),
+        lambda: mx.paged_attention(gpu(3, 4, 64), c, gpu(3, 2, dtype=torch.int32), idx, scale=1e39),
+        lambda: setattr(c, "k_codes", c.v_codes),
         lambda: mx.paged_attention(gpu(3, 4, 64), c, gpu(3, 2, dtype=torch.int32), idx, out=gpu(3, 4, 32)),
         lambda: mx.paged_attention(gpu(3, 4, 64).float(), c, gpu(3, 2, dtype=torch.int32), idx),
     ]

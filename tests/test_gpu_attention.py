@@ -525,6 +525,19 @@ def test_attention_of_large_and_tiny_queries(mx):
         check_attention(out, lse, q[rows], cache, table[rows], [90] * len(rows), scale)
 
 
+@pytest.mark.parametrize("seqs,longest,heads", [(5, 900, 16), (2, 30000, 16), (70, 3000, 48)])
+def test_attention_into_its_own_query(mx, seqs, longest, heads):
+    """out may be q itself: one block, clusters and joined pieces."""
+    rng = np.random.default_rng(seqs)
+    lengths = rng.integers(0, longest, seqs)
+    cache = random_cache(mx, rng, 64, 2, 128, 64, "mxfp8")
+    table = i32(rng.integers(0, 64, (seqs, -(-longest // 64))))
+    q = bf16(rng, (seqs, heads, 128))
+    want = mx.paged_attention(q, cache, table, i32(lengths))
+    assert mx.paged_attention(q, cache, table, i32(lengths), out=q) is not None
+    assert torch.equal(q, want)
+
+
 def test_bad_pages_and_lengths(mx):
     """A page outside the cache loses its keys, a length past the table's row is cut; both set the error word."""
     rng = np.random.default_rng(6)
