@@ -100,7 +100,7 @@ def qk_norm_rope(qkv, num_heads: int, num_kv_heads: int, cos=None, sin=None, pos
     """RMS norm of every query and key head and its rotation, in one pass over ``qkv``.
 
     ``qkv`` bf16 ``[tokens, (num_heads + 2 * num_kv_heads) * head_dim]``: query, key and value heads
-    side by side, rows of any stride that is a multiple of 8; head_dim is a multiple of 32 up to
+    side by side, rows apart by a multiple of 8; head_dim is a multiple of 32 up to
     256.  With ``q_weight`` / ``k_weight`` (``[head_dim]``, bf16 or fp32, both or neither) a head x becomes
     ``x * weight / sqrt(mean(x * x) + eps)``.  ``cos`` / ``sin`` fp32 ``[rows, rot / 2]`` turn the first
     ``rot`` values (a multiple of 16): row ``positions[token]`` (int32), or the token's own index;
@@ -150,7 +150,7 @@ def paged_attention(q, cache: MXKVCache, page_table, lengths, scale: float | Non
 
     ``q`` bf16 ``[seqs, num_heads, head_dim]`` (each sequence's heads contiguous), num_heads a multiple of
     the cache's num_kv_heads: query head h reads kv head ``h // (num_heads // num_kv_heads)``.
-    ``page_table`` int32 ``[seqs, max_pages]`` (rows of any stride): key j of sequence s is row ``j %
+    ``page_table`` int32 ``[seqs, max_pages]`` (rows apart by max_pages or more): key j of sequence s is row ``j %
     page_size`` of page ``page_table[s, j // page_size]``, j < ``lengths[s]`` (int32); entries past the last
     page a sequence needs are not read.  A length of zero gives a row of zeros.  ``scale`` defaults to
     ``head_dim ** -0.5``.  Returns bf16 ``[seqs, num_heads, head_dim]`` (``out`` if given), with
