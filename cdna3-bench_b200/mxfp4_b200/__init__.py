@@ -67,7 +67,8 @@ def __getattr__(name):
     if name in _ATTENTION_OPS:
         from . import attention
 
-        return getattr(attention, name)
+        globals()[name] = getattr(attention, name)  # found at once from now on: a lookup here takes a microsecond
+        return globals()[name]
     if name in _OPS:
         from . import kernels
 
