@@ -1183,6 +1183,7 @@ int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cach
   a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
   a.heads = static_cast<int2*>(workspace);
   a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + (p.bytes ? p.parts_at : 0)), a.target = p.target, a.fit = p.fit, a.unit_keys = p.unit_keys, a.cluster = p.cluster;
+  a.stride = p.unit_keys / 16 * std::max(1, p.cluster);
   auto s = static_cast<cudaStream_t>(stream);
   return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p.nt, p.blocks, d, s) : launch_attention_dim<kFmtE2M1>(a, p.nt, p.blocks, d, s);
 }

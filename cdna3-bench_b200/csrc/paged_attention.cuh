@@ -100,6 +100,7 @@ struct AttnArgs {
   int fit;                 // heads are few: no more pieces than that
   int unit_keys;
   int cluster;             // blocks to a head, joining among themselves; 0: pieces
+  int stride;              // tiles from one step of a warp to its next: of one unit, times the cluster's blocks
 };
 
 __device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -123,6 +124,14 @@ __device__ __forceinline__ float exp2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+
+__device__ __forceinline__ float4 ld_dsmem_f32x4(const float* local, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+  return v;
 }
 
 // Length of a sequence in keys, within what its page table can hold.
@@ -352,23 +361,39 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
     return;
   }
   {
-    const int seq = me.seq, len = attn_length(a, seq), units = attn_units(a, seq, kUnitKeys);
-    const int first = static_cast<int>(static_cast<long long>(units) * me.index / me.of);  // units first .. last - 1
-    const int last = static_cast<int>(static_cast<long long>(units) * (me.index + 1) / me.of);
+    const int seq = me.seq;
+    const int* table = a.table + a.table_stride * seq;
+    const int tile_shift = a.cache.page_shift - 4;
+    // The blocks of a cluster take units in turn, so that the first is known, and its pages are on their
+    // way, before the length is.
+    int first = me.index, page[KT];
+    if (a.cluster) {
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+        const int at = ((first * kAttnWarps + warp) * KT + i) >> tile_shift;
+        page[i] = at < a.max_pages ? __ldg(table + at) : 0;
+      }
+    }
+    const int len = attn_length(a, seq);
+    int tile_last = (len + 15) >> 4;
+    if (!a.cluster) {  // units first .. of a piece
+      const int units = attn_units(a, seq, kUnitKeys);
+      first = static_cast<int>(static_cast<long long>(units) * me.index / me.of);
+      tile_last = min(static_cast<int>(static_cast<long long>(units) * (me.index + 1) / me.of) * kAttnWarps * KT, tile_last);
+#pragma unroll
+      for (int i = 0; i < KT; ++i) {
+        const int at = (first * kAttnWarps + warp) * KT + i;
+        page[i] = at < tile_last ? __ldg(table + (at >> tile_shift)) : 0;
+      }
+    }
     const int head = me.head_chunk / a.chunks, chunk = me.head_chunk - head * a.chunks;
     const int h0 = head * a.group + chunk * kHeads;                  // first q head
     const int nh = min(kHeads, a.group - chunk * kHeads);            // q heads here
-    const int* table = a.table + a.table_stride * seq;
-    const int tile_shift = a.cache.page_shift - 4;
-    const int tile_last = min(last * kAttnWarps * KT, (len + 15) >> 4);
 
     // Copies into the ring, one commit group per step; the pages of the step after are on their way.
     // `good` has KT bits for each of the last copies: whether the tile's page is one of the cache's.
     uint32_t good = 0;
     int copy_tile = (first * kAttnWarps + warp) * KT, copy_slot = 0;
-    int page[KT];
-#pragma unroll
-    for (int i = 0; i < KT; ++i) page[i] = copy_tile + i < tile_last ? __ldg(table + ((copy_tile + i) >> tile_shift)) : 0;
     const uint32_t page_rows = static_cast<uint32_t>(a.cache.heads) << a.cache.page_shift;
     const size_t head_rows = static_cast<size_t>(head) << a.cache.page_shift;
     const uint8_t* k_lane = a.cache.k_codes + head_rows * kRowBytes + 16 * lane;
@@ -389,7 +414,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
             record_error(kErrBadPage);
           }
         }
-      copy_tile += kAttnWarps * KT;
+      copy_tile += a.stride;
 #pragma unroll
       for (int i = 0; i < KT; ++i)
         if (copy_tile + i < tile_last) page[i] = __ldg(table + ((copy_tile + i) >> tile_shift));
@@ -581,7 +606,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
       }
     };
 #pragma unroll 1
-    for (int tile = (first * kAttnWarps + warp) * KT; tile < tile_last; tile += kAttnWarps * KT) {
+    for (int tile = (first * kAttnWarps + warp) * KT; tile < tile_last; tile += a.stride) {
       cp_async_wait<kRing - 2>();
       __syncwarp();  // every lane's copies have landed, and all lanes have left the slot copied into next
       copy_next();
@@ -650,15 +675,27 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
       cluster_sync_all();
       for (int i = me.index * kAttnThreads + threadIdx.x; i < nh * (D / 4); i += a.cluster * kAttnThreads) {
         const int h = i / (D / 4), d = 4 * (i - h * (D / 4));
-        float top = -kInf;
-        for (int c = 0; c < a.cluster; ++c) top = fmaxf(top, ld_dsmem_f32(sm_joined + h, c));
+        float top = -kInf, m_of[8], l_of[8];  // all loads before the first use: each is a trip to another SM
+        float4 o_of[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          m_of[c] = -kInf, l_of[c] = 0.0f, o_of[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (c < a.cluster) {
+            m_of[c] = ld_dsmem_f32(sm_joined + h, c);
+            l_of[c] = ld_dsmem_f32(sm_joined + kHeads + h, c);
+            o_of[c] = ld_dsmem_f32x4(sm + h * kStride + d, c);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) top = fmaxf(top, m_of[c]);
         const float base = top == -kInf ? 0.0f : top;
         float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
-        for (int c = 0; c < a.cluster; ++c) {
-          const float f = exp2_approx(ld_dsmem_f32(sm_joined + h, c) - base);
-          l = fmaf(ld_dsmem_f32(sm_joined + kHeads + h, c), f, l);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) o[j] = fmaf(ld_dsmem_f32(sm + h * kStride + d + j, c), f, o[j]);
+        for (int c = 0; c < 8; ++c) {
+          const float f = exp2_approx(m_of[c] - base);
+          l = fmaf(l_of[c], f, l);
+          o[0] = fmaf(o_of[c].x, f, o[0]), o[1] = fmaf(o_of[c].y, f, o[1]);
+          o[2] = fmaf(o_of[c].z, f, o[2]), o[3] = fmaf(o_of[c].w, f, o[3]);
         }
         const float r = l == 0.0f ? 0.0f : 1.0f / l;
         const size_t at = static_cast<size_t>(seq) * a.q_heads + h0 + h;
