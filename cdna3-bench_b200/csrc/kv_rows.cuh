@@ -468,12 +468,16 @@ __device__ __forceinline__ void cp_async_wait() {
 // brought by shuffles: 26.4 us there and 62 us against 54 on the second; a persistent ring over the
 // tokens: no faster (33 and 71 us), its bookkeeping costs what it hides.
 //
+// A programmatic dependent launch, as is the read below: 2.0 -> 1.8 us for the small calls in a graph.
+//
 // Two tokens of one launch that name the same slot: the later one is stored (every block looks
 // through the slots behind its own; the caller keeps a launch to 4096 tokens).
 template <int LPR, int kFmt, bool kInter>
 __global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(const __grid_constant__ RowArgs a, int first) {
   constexpr int kRows = 32 / LPR;  // rows to be coded a warp works on at a time
   __shared__ __align__(16) uint8_t stage_s[kRowThreads / 32][2 * kRowStage * 1024];
+  griddep_wait();  // before anything is read: only the launch itself runs beside the kernel before
+  griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, at = 8 * (lane & (LPR - 1)), sub = lane / LPR;
   const bool live = at < a.dim;
   const int t = first + blockIdx.x, part = blockIdx.y * (kRowThreads / 32) + warp, parts = gridDim.y * (kRowThreads / 32);
@@ -664,6 +668,8 @@ template <int kFmt>
 __global__ void __launch_bounds__(kReadThreads)
     kv_read_kernel(const __grid_constant__ KvCacheView cache, const int* __restrict__ slots, int rows,
                    __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v) {
+  griddep_wait();
+  griddep_launch_dependents();
   const int per_head = cache.dim / 8, units = cache.heads * per_head;
   const int r0 = blockIdx.x * kReadRows;
   int slot[kReadRows];

@@ -699,8 +699,7 @@ int launch_head_rows(const RowArgs& a, cudaStream_t s, const DeviceState* d) {
     const int n = std::min(most, a.tokens - first);
     // few tokens: their rows are spread over blocks until the SMs have eight each
     const int y = std::max(1, std::min(ceil_div(sets, kRowThreads / 32), 8 * d->sm_count / n));
-    head_rows_kernel<LPR, kFmt, kInter><<<dim3(n, y), kRowThreads, 0, s>>>(a, first);
-    const int rc = launch_status();
+    const int rc = launch_pdl_grid(head_rows_kernel<LPR, kFmt, kInter>, dim3(n, y), kRowThreads, 0, s, a, first);
     if (rc) return rc;
     if (a.tokens - first <= most) break;  // first + most may pass the int range
   }
@@ -809,6 +808,8 @@ int launch_attention(const AttnArgs& a, int blocks, DeviceState* d, cudaStream_t
     cfg.numAttrs = 1;
     return ret(cudaLaunchKernelEx(&cfg, attn_kernel<D, kFmt, NT>, a));
   }
+  // An ordinary launch: started beside the kernel before, its blocks would fill up the first SMs to be
+  // free (8 sequences of 1000 keys one after another: 9.1 us against 7.9).
   attn_kernel<D, kFmt, NT><<<blocks, kAttnThreads, smem, s>>>(a);
   const int rc = launch_status();
   if (rc || a.cluster) return rc;
@@ -1140,9 +1141,8 @@ int mxfp4_kv_cache_read(const mxfp4_kv_cache* cache, const int* slots, int token
   auto s = static_cast<cudaStream_t>(stream);
   const int blocks = ceil_div(tokens, kReadRows);
   auto *ko = static_cast<__nv_bfloat16*>(k), *vo = static_cast<__nv_bfloat16*>(v);
-  if (fmt == kFmtE4M3) kv_read_kernel<kFmtE4M3><<<blocks, kReadThreads, 0, s>>>(c, slots, tokens, ko, vo);
-  else kv_read_kernel<kFmtE2M1><<<blocks, kReadThreads, 0, s>>>(c, slots, tokens, ko, vo);
-  return launch_status();
+  return launch_pdl_grid(fmt == kFmtE4M3 ? kv_read_kernel<kFmtE4M3> : kv_read_kernel<kFmtE2M1>, dim3(blocks), kReadThreads, 0, s, c,
+                         slots, tokens, ko, vo);
 }
 
 size_t mxfp4_paged_attention_workspace_bytes(const mxfp4_kv_cache* cache, int seqs, int num_heads, int max_pages) {

@@ -628,6 +628,54 @@ def test_graphs_replay_with_new_contents_and_streams(mx):
         assert torch.equal(eager, state[0][3]) and torch.equal(elses, state[0][4])
 
 
+def test_each_call_sees_what_ran_before_it(mx):
+    """The row kernels may be launched while the kernel before them still runs: a copy, a memset, another
+    stream's event and each other's writes come first all the same, eager and in a graph."""
+    tokens, kv, dim = 3000, 8, 128
+    rng = np.random.default_rng(3)
+    k, v = bf16(rng, (tokens, kv, dim)), bf16(rng, (tokens, kv, dim))
+    cache = mx.new_kv_cache(-(-tokens // 64), kv, dim, 64)
+    slots, held, staged = i32(rng.permutation(cache.num_pages * 64)[:tokens]), torch.zeros_like(k), torch.zeros_like(v)
+    zeros, other = torch.zeros_like(slots) - 1, torch.cuda.Stream()
+
+    def steps():
+        out = []
+        for i in range(4):
+            here = torch.cuda.current_stream()
+            held.copy_(k * (i + 1))  # a kernel and a copy
+            other.wait_stream(here)
+            with torch.cuda.stream(other):
+                staged.copy_(v * (i + 1))
+            here.wait_stream(other)
+            mx.kv_cache_write(cache, held, staged, slots)
+            held.zero_()
+            mx.kv_cache_write(cache, held, held, zeros)  # writes nothing
+            out.append(mx.kv_cache_read(cache, slots))
+            cache.k_codes.zero_()  # a memset
+            out.append(mx.kv_cache_read(cache, slots))
+            mx.kv_cache_write(cache, held, staged, slots)
+            out.append(mx.kv_cache_read(cache, slots))
+        return out
+
+    def check(out):
+        for i in range(4):
+            mx.kv_cache_write(cache, k * (i + 1), v * (i + 1), slots)
+            rk, rv = mx.kv_cache_read(cache, slots)
+            (ak, av), (bk, bv), (ck, cv) = out[3 * i:3 * i + 3]
+            assert torch.equal(ak, rk) and all(torch.equal(x, rv) for x in (av, bv, cv))
+            assert (bk == 0).all() and (ck == 0).all()
+
+    check(steps())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = steps()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_decoding_through_the_gemms(mx, fmt):
     """A layer's attention as it is used: a prompt, then single tokens, each through the QKV GEMM, the norm
