@@ -760,6 +760,7 @@ int rope_args(RowArgs* a, const void* qkv, long long row_stride, int tokens, int
 // of them: as many (a power of two up to 8) as the longest sequence has units and the SMs have room for.
 struct AttnPlan {
   int nt, chunks, target, fit, blocks, unit_keys, cluster;
+  bool beside;  // its blocks may be placed while the kernel before still runs
   size_t parts_at, bytes;  // the workspace: a word pair per head, then the parts
 };
 AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int max_pages, int page_size, int sm_count) {
@@ -781,13 +782,18 @@ AttnPlan attn_plan(int dim, int fmt, int kv_heads, int q_heads, int seqs, int ma
   while (c < 8 && c < most && 2 * c * heads <= resident) c *= 2;
   p.cluster = most <= kAttnClusterSteps * c && heads * c < (1ll << 30) ? c : 0;
   if (p.cluster) p.blocks = static_cast<int>(heads * c);
+  // A programmatic launch saves 2 us between queued calls (16 x 4000 keys in pieces of a head: 31.6 -> 29.5, 64 x 500:
+  // 20.5 -> 17.8).  But its blocks go to the SMs that are free first: where they do not fill the
+  // GPU and have much to do each, some SMs get three and others none (16 x 4000 keys, 256 blocks behind a small
+  // kernel: 34.9 -> 42.3).
+  p.beside = !p.cluster || most <= 2 * c || 4ll * p.blocks >= 3 * resident;
   p.parts_at = (static_cast<size_t>(heads) * sizeof(int2) + 15) / 16 * 16;
   p.bytes = p.cluster ? 0 : p.parts_at + static_cast<size_t>(p.target) * 2 * 8 * p.nt * (dim + 2) * sizeof(float);
   return p;
 }
 
 template <int D, int kFmt, int NT>
-int launch_attention(const AttnArgs& a, int blocks, DeviceState* d, cudaStream_t s) {
+int launch_attention(const AttnArgs& a, const AttnPlan& p, DeviceState* d, cudaStream_t s) {
   constexpr int smem = attn_smem_bytes(D, kFmt, NT);
   std::atomic<bool>& done = d->attn_attr[((D == 64 ? 0 : D == 128 ? 1 : 2) * 2 + (kFmt - 1)) * 2 + NT - 1];
   if (!done.load(std::memory_order_acquire)) {
@@ -795,33 +801,32 @@ int launch_attention(const AttnArgs& a, int blocks, DeviceState* d, cudaStream_t
     if (e != cudaSuccess) return ret(e);
     done.store(true, std::memory_order_release);
   }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.blocks);
+  cfg.blockDim = dim3(kAttnThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
   if (a.cluster > 1) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(kAttnThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {static_cast<unsigned>(a.cluster), 1, 1};
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return ret(cudaLaunchKernelEx(&cfg, attn_kernel<D, kFmt, NT>, a));
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs++].val.clusterDim = {static_cast<unsigned>(a.cluster), 1, 1};
   }
-  // An ordinary launch: started beside the kernel before, its blocks would fill up the first SMs to be
-  // free (8 sequences of 1000 keys one after another: 9.1 us against 7.9).
-  attn_kernel<D, kFmt, NT><<<blocks, kAttnThreads, smem, s>>>(a);
-  const int rc = launch_status();
+  if (p.beside && pdl_enabled()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  cfg.attrs = attr;
+  const int rc = ret(cudaLaunchKernelEx(&cfg, attn_kernel<D, kFmt, NT>, a));
   if (rc || a.cluster) return rc;
   return launch_pdl_grid(attn_join_kernel<D, NT>, dim3(a.seqs * a.cache.heads * a.chunks, std::min(8 * NT, a.group)), kAttnThreads, 0, s, a);
 }
 
 template <int kFmt>
-int launch_attention_dim(const AttnArgs& a, int nt, int blocks, DeviceState* d, cudaStream_t s) {
+int launch_attention_dim(const AttnArgs& a, const AttnPlan& p, DeviceState* d, cudaStream_t s) {
   switch (a.cache.dim) {
-    case 64: return nt == 1 ? launch_attention<64, kFmt, 1>(a, blocks, d, s) : launch_attention<64, kFmt, 2>(a, blocks, d, s);
-    case 128: return nt == 1 ? launch_attention<128, kFmt, 1>(a, blocks, d, s) : launch_attention<128, kFmt, 2>(a, blocks, d, s);
-    default: return launch_attention<256, kFmt, 1>(a, blocks, d, s);
+    case 64: return p.nt == 1 ? launch_attention<64, kFmt, 1>(a, p, d, s) : launch_attention<64, kFmt, 2>(a, p, d, s);
+    case 128: return p.nt == 1 ? launch_attention<128, kFmt, 1>(a, p, d, s) : launch_attention<128, kFmt, 2>(a, p, d, s);
+    default: return launch_attention<256, kFmt, 1>(a, p, d, s);
   }
 }
 
@@ -1185,7 +1190,7 @@ int mxfp4_paged_attention(const void* q, long long q_stride, const mxfp4_kv_cach
   a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + (p.bytes ? p.parts_at : 0)), a.target = p.target, a.fit = p.fit, a.unit_keys = p.unit_keys, a.cluster = p.cluster;
   a.stride = p.unit_keys / 16 * std::max(1, p.cluster);
   auto s = static_cast<cudaStream_t>(stream);
-  return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p.nt, p.blocks, d, s) : launch_attention_dim<kFmtE2M1>(a, p.nt, p.blocks, d, s);
+  return fmt == kFmtE4M3 ? launch_attention_dim<kFmtE4M3>(a, p, d, s) : launch_attention_dim<kFmtE2M1>(a, p, d, s);
 }
 
 }  // extern "C"

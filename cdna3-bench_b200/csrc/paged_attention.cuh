@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
   float* sm_l = sm_m + kAttnWarps * kHeads;
   float* sm_joined = sm_l + kAttnWarps * kHeads;              // of the block: m, l [kHeads]
 
-  griddep_launch_dependents();
+  griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int key_g = (g >> 1) + 4 * (g & 1);  // pi(g): the key of operand row g (and key_g + 8 of row g + 8)
   const uint32_t ring = smem_u32(sm) + warp * kRing * KT * kTile;
@@ -616,6 +616,8 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
       else if (have) do_step(tile, have, at, std::true_type{});
     }
     cp_async_wait<0>();
+    // Not earlier: the blocks of a call after this one would fill up the SMs that are busy already.
+    griddep_launch_dependents();
     __syncthreads();  // the rings become the buffer of the parts
 
     // join the warps
@@ -724,8 +726,9 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const __grid_co
   if (h >= a.group - chunk * kHeads) return;
   const size_t at = static_cast<size_t>(seq) * a.q_heads + head * a.group + chunk * kHeads + h;
   const int team = threadIdx.x / kLanes, d = 4 * (threadIdx.x - team * kLanes);
-  const bool empty = attn_length(a, seq) == 0;
+  const bool empty = attn_length(a, seq) == 0;  // before the wait: attn_kernel's blocks have waited themselves
   griddep_wait();
+  griddep_launch_dependents();
   if (empty) {
     if (team == 0) *reinterpret_cast<uint2*>(a.out + at * D + d) = make_uint2(0, 0);
     if (a.lse && threadIdx.x == 0) a.lse[at] = -kInf;

@@ -676,6 +676,43 @@ def test_each_call_sees_what_ran_before_it(mx):
         check(out)
 
 
+@pytest.mark.parametrize("seqs,longest,heads,kv", [(1, 700, 16, 2), (16, 4000, 16, 8), (3, 40000, 16, 2), (300, 500, 4, 4), (70, 3000, 20, 2)])
+def test_attention_sees_what_ran_before_it(mx, seqs, longest, heads, kv):
+    """However it is launched (one block or a cluster to a head, pieces and their joining), the query, lengths
+    and pages of a call are those written just before it, eager and in a graph."""
+    rng = np.random.default_rng(seqs)
+    cache = random_cache(mx, rng, 80, kv, 128, 64, "mxfp8")
+    width = -(-longest // 64)
+    calls = [(bf16(rng, (seqs, heads, 128)), i32(rng.integers(0, longest, seqs)), i32(rng.integers(0, 80, (seqs, width)))) for _ in range(3)]
+    want = [mx.paged_attention(q, cache, table, lengths, return_lse=True) for q, lengths, table in calls]
+    q, lengths, table = (torch.zeros_like(t) for t in calls[0])
+
+    def steps():
+        out = []
+        for i in range(6):
+            for to, of in zip((q, lengths, table), calls[i % 3]):
+                to.copy_(of)
+            out.append(mx.paged_attention(q, cache, table, lengths, return_lse=True))
+            out.append(mx.paged_attention(q, cache, table, lengths, return_lse=True))
+            for t in (q, lengths, table):
+                t.zero_()
+        return out
+
+    def check(out):
+        for i, (o, lse) in enumerate(out):
+            assert torch.equal(o, want[i // 2 % 3][0]) and torch.equal(lse, want[i // 2 % 3][1]), i
+
+    check(steps())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = steps()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_decoding_through_the_gemms(mx, fmt):
     """A layer's attention as it is used: a prompt, then single tokens, each through the QKV GEMM, the norm
