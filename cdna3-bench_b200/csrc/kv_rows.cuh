@@ -490,49 +490,60 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(cons
   const bool live16 = piece.b < a.dim, rotated = l16 < (a.rot >> 4);
   const uint32_t stage1 = smem_u32(stage_s[warp]) + 16 * lane, stage2 = stage1 + 1024 * kRowStage;
   const int step = parts * 2 * kRows;  // heads from set to set
-  auto stage_rows = [&](uint32_t st, const __nv_bfloat16* src, int h, int heads) {
-#pragma unroll
-    for (int i = 0; i < kRowStage; ++i, h += step)
-      if (live16 && h < heads) {
-        cp_async16(st + 1024 * i, src + h * a.dim + piece.a);
-        cp_async16(st + 1024 * i + 512, src + h * a.dim + piece.b);
-      }
+  const int q0 = part * 2 * kRows, k0 = back * 2 * kRows;  // first heads of the first sets
+  auto send_row = [&](uint32_t st, const __nv_bfloat16* src, int h, int heads) {
+    if (live16 && h < heads) {
+      cp_async16(st, src + h * a.dim + piece.a);
+      cp_async16(st + 512, src + h * a.dim + piece.b);
+    }
   };
-  auto turn_rows = [&](uint32_t st, __nv_bfloat16* dst, int h, int heads, const LaneTurn16& turn, bool norm, bool good) {
+  // Heads h, h + step, ... of one kind that stay bf16; the first kRowStage sets are on their way, each
+  // set's place is filled with the one kRowStage sets on.
+  auto turn_rows = [&](uint32_t base, const __nv_bfloat16* src, __nv_bfloat16* dst, int h, int heads, const LaneTurn16& turn,
+                       bool norm, bool good) {
+    uint32_t st = base;
 #pragma unroll 1
-    for (int i = 0; i < kRowStage && h - sub16 < heads; ++i, h += step) {
+    for (; h - sub16 < heads; h += step) {
       const bool here = live16 && h < heads;
       uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-      if (here && good) x[0] = lds128(st + 1024 * i), x[1] = lds128(st + 1024 * i + 512);
+      cp_async_wait<kRowStage - 1>();
+      if (here && good) x[0] = lds128(st), x[1] = lds128(st + 512);
       if (good) turn_row16<LPR, kInter>(a, x, turn, norm, rotated);
       if (here) {
         *reinterpret_cast<uint4*>(dst + h * a.dim + piece.a) = x[0];
         *reinterpret_cast<uint4*>(dst + h * a.dim + piece.b) = x[1];
       }
+      send_row(st, src, h + kRowStage * step, heads);
+      cp_async_commit();
+      st = st == base + 1024 * (kRowStage - 1) ? base : st + 1024;
     }
   };
   const __nv_bfloat16* q_src = a.q + a.q_stride * t;
   const __nv_bfloat16* k_src = a.k + a.k_stride * t;
   const __nv_bfloat16* v_src = a.v + a.v_stride * t;
-  const int q0 = part * 2 * kRows, k0 = back * 2 * kRows;  // first heads of the first sets
   // for a cache: sets of kRows rows, k's and then v's
   const int kv_sets = ceil_div(a.kv_heads, kRows);
   auto coded = [&](int g, bool& value) {
     value = g >= kv_sets;
     return (value ? g - kv_sets : g) * kRows + sub;
   };
-  auto stage_coded = [&](int g) {
-#pragma unroll
-    for (int i = 0; i < kRowStage; ++i, g += parts) {
-      bool value;
-      const int h = coded(g, value);
-      if (live && g < 2 * kv_sets && h < a.kv_heads) cp_async16(stage2 + 1024 * i, (value ? v_src : k_src) + h * a.dim + at);
-    }
+  auto send_coded = [&](uint32_t st, int g) {
+    bool value;
+    const int h = coded(g, value);
+    if (live && g < 2 * kv_sets && h < a.kv_heads) cp_async16(st, (value ? v_src : k_src) + h * a.dim + at);
   };
-  stage_rows(stage1, q_src, q0 + sub16, a.q_heads);
-  if constexpr (kFmt == kFmtNone) stage_rows(stage2, k_src, k0 + sub16, a.kv_heads);
-  else stage_coded(back);
+  // k and v in one group, then each set of q in its own
+#pragma unroll
+  for (int i = 0; i < kRowStage; ++i) {
+    if constexpr (kFmt == kFmtNone) send_row(stage2 + 1024 * i, k_src, k0 + sub16 + i * step, a.kv_heads);
+    else send_coded(stage2 + 1024 * i, back + i * parts);
+  }
   cp_async_commit();
+#pragma unroll
+  for (int i = 0; i < kRowStage; ++i) {
+    send_row(stage1 + 1024 * i, q_src, q0 + sub16 + i * step, a.q_heads);
+    cp_async_commit();
+  }
 
   const int p = a.rot && a.positions ? __ldg(a.positions + t) : t;
   const bool good = !a.rot || (p >= 0 && p < a.table_rows);
@@ -567,55 +578,37 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(cons
   if (q0 < a.q_heads) {
     LaneTurn16 turn;
     if (good) load_turn16<kInter>(a, p, a.q_weight, l16, turn);
-    cp_async_wait<0>();
-    __nv_bfloat16* dst = a.q_out + static_cast<size_t>(t) * a.q_heads * a.dim;
-    for (int h = q0; h < a.q_heads; h += kRowStage * step) {
-      if (h != q0) {
-        stage_rows(stage1, q_src, h + sub16, a.q_heads);
-        cp_async_commit();
-        cp_async_wait<0>();
-      }
-      turn_rows(stage1, dst, h + sub16, a.q_heads, turn, a.q_weight != nullptr, good);
-    }
+    turn_rows(stage1, q_src, a.q_out + static_cast<size_t>(t) * a.q_heads * a.dim, q0 + sub16, a.q_heads, turn, a.q_weight != nullptr,
+              good);
   }
   cp_async_wait<0>();
   if constexpr (kFmt == kFmtNone) {
     if (k0 >= a.kv_heads) return;
     LaneTurn16 turn;
     if (good) load_turn16<kInter>(a, p, a.k_weight, l16, turn);
-    __nv_bfloat16* dst = a.k_out + static_cast<size_t>(t) * a.kv_heads * a.dim;
-    for (int h = k0; h < a.kv_heads; h += kRowStage * step) {
-      if (h != k0) {
-        stage_rows(stage2, k_src, h + sub16, a.kv_heads);
-        cp_async_commit();
-        cp_async_wait<0>();
-      }
-      turn_rows(stage2, dst, h + sub16, a.kv_heads, turn, a.k_weight != nullptr, good);
-    }
+    turn_rows(stage2, k_src, a.k_out + static_cast<size_t>(t) * a.kv_heads * a.dim, k0 + sub16, a.kv_heads, turn,
+              a.k_weight != nullptr, good);
   } else {
     if (slot < 0) return;
     const bool turned = a.rot || a.k_weight;
-    for (int g0 = back; g0 < 2 * kv_sets; g0 += kRowStage * parts) {
-      if (g0 != back) {
-        stage_coded(g0);
-        cp_async_commit();
-        cp_async_wait<0>();
-      }
-      float cw[8], sw[8];
-      if (turned && g0 < kv_sets) {
-        LaneTurn q;
-        load_turn<LPR, kInter>(a, p, a.k_weight, q);
+    float cw[8], sw[8];
+    if (turned && back < kv_sets) {
+      LaneTurn q;
+      load_turn<LPR, kInter>(a, p, a.k_weight, q);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) cw[j] = q.c[j] * q.w[j], sw[j] = q.s[j] * q.wp[j];
-      }
-      uint32_t open = 0;  // sets whose codes 32 bits did not settle
+      for (int j = 0; j < 8; ++j) cw[j] = q.c[j] * q.w[j], sw[j] = q.s[j] * q.wp[j];
+    }
+    uint32_t st = stage2;
+    for (int g0 = back; g0 < 2 * kv_sets; g0 += 32 * parts) {
+      uint32_t open = 0;  // of 32 sets: those whose codes 32 bits did not settle
 #pragma unroll 1
-      for (int i = 0, g = g0; i < kRowStage && g < 2 * kv_sets; ++i, g += parts) {
+      for (int i = 0, g = g0; i < 32 && g < 2 * kv_sets; ++i, g += parts) {
         bool value;
         const int h = coded(g, value);
         const bool here = live && h < a.kv_heads;
         uint4 x = make_uint4(0, 0, 0, 0);
-        if (here) x = lds128(stage2 + 1024 * i);
+        cp_async_wait<kRowStage - 1>();
+        if (here) x = lds128(st);
         const size_t row = here ? a.cache.row(slot, h) : 0;
         if (!value && turned) {
           if (!store_keys<LPR, kFmt, kInter>(a, x, cw, sw, here, row, at)) open |= 1u << i;
@@ -624,14 +617,18 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(cons
           unpack_bf16x8(x, f);
           code_and_store<kFmt>(a.cache, !value, f, here, row, at);
         }
+        send_coded(st, g + kRowStage * parts);
+        cp_async_commit();
+        st = st == stage2 + 1024 * (kRowStage - 1) ? stage2 : st + 1024;
       }
-      while (open) {  // nothing is kept over the call
+      while (open) {  // after the loop, so that none of its values are kept over the calls
         const int i = __ffs(open) - 1;
         open &= open - 1;
         store_keys_exact<LPR, kFmt, kInter>(&a, t, p, slot, (g0 + i * parts) * kRows);
       }
     }
   }
+  cp_async_wait<0>();
 }
 
 // E8M0 byte as fp32: 2^(b-127), 255 is NaN.
