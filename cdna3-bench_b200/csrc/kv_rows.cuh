@@ -562,13 +562,13 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(cons
       if ((reinterpret_cast<uintptr_t>(a.slots) & 15u) == 0) {
         const int4* s4 = reinterpret_cast<const int4*>(a.slots);
 #pragma unroll 4
-        for (int u = (t + 1) / 4 + threadIdx.x; 4 * u + 3 < end; u += kRowThreads) {
+        for (int u = t / 4 + 1 + threadIdx.x; u < end / 4; u += kRowThreads) {
           const int4 s = __ldg(s4 + u);
-          later |= (s.x == slot && 4 * u > t) || (s.y == slot && 4 * u + 1 > t) || (s.z == slot && 4 * u + 2 > t) ||
-                   (s.w == slot && 4 * u + 3 > t);
+          later |= s.x == slot || s.y == slot || s.z == slot || s.w == slot;
         }
-        const int u = end / 4 * 4 + threadIdx.x;  // what a whole int4 would pass the end with
-        if (u < end && u > t) later |= __ldg(a.slots + u) == slot;
+        // up to the first and from the last whole int4
+        const int u = threadIdx.x < 4 ? t + 1 + threadIdx.x : end / 4 * 4 + threadIdx.x - 4;
+        if (threadIdx.x < 8 && u > t && u < end) later |= __ldg(a.slots + u) == slot;
       } else {
         for (int u = t + 1 + threadIdx.x; u < end; u += kRowThreads) later |= __ldg(a.slots + u) == slot;
       }
