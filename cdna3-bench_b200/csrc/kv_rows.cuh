@@ -1,9 +1,9 @@
 // Head rows between the QKV GEMM and the attention: per-head RMS norm, rotation, and the MX
 // key-value cache those rows are coded into and read back from.
 //
-// A row is one head of one token, D bf16 values (D % 32 == 0, D <= 256).  For the rows to be coded a
-// lane holds 8 neighbouring values (one 16-byte load), so a row takes LPR = 4, 8, 16 or 32 lanes and
-// a warp works on 32 / LPR rows of one kind at a time; for those that stay bf16 it holds 16.
+// A row is one head of one token, D bf16 values (D % 32 == 0, D <= 256).  For a key that is turned and
+// coded a lane holds 8 neighbouring values (one 16-byte load), so a row takes LPR = 4, 8, 16 or 32 lanes
+// and a warp works on 32 / LPR rows at a time; for rows that stay bf16 or are coded as they are it holds 16.
 //
 //   norm      y_i = x_i * w_i / sqrt(mean(x^2) + eps)
 //   rotation  of the first R values with c = cos[p][i], s = sin[p][i], i < R/2:
@@ -352,6 +352,27 @@ __device__ __forceinline__ void code_and_store(const KvCacheView& c, bool key, c
   if (here) store_codes<kFmt>(c, key, row, at, o, byte);
 }
 
+// Codes 16 neighbouring values per lane, x as they are in memory, and stores them.  The whole warp.
+template <int kFmt>
+__device__ __forceinline__ void code_and_store16(const KvCacheView& c, bool key, const uint4 (&x)[2], bool here, size_t row, int at) {
+  float f[2][8];
+  unpack_bf16x8(x[0], f[0]);
+  unpack_bf16x8(x[1], f[1]);
+  uint32_t amax = max(magnitude_bits(f[0]), magnitude_bits(f[1]));
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  const int byte = scale_byte<kFmt>(amax);
+  uint2 lo = make_uint2(0, 0), hi = lo;
+  if (byte != 255) {
+    const float inv = exp2_neg(byte - 127);
+    lo = code8<kFmt>(f[0], inv), hi = code8<kFmt>(f[1], inv);
+  }
+  if (!here) return;
+  uint8_t* codes = key ? c.k_codes : c.v_codes;
+  if constexpr (kFmt == kFmtE4M3) *reinterpret_cast<uint4*>(codes + row * c.dim + at) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  else *reinterpret_cast<uint2*>(codes + row * (c.dim / 2) + at / 2) = make_uint2(lo.x, hi.x);
+  if ((at & 31) == 0) (key ? c.k_scales : c.v_scales)[row * (c.dim / 32) + at / 32] = static_cast<uint8_t>(byte);
+}
+
 constexpr int kRowThreads = 64;
 constexpr int kRowBlocks = 10;  // resident per SM
 
@@ -474,7 +495,7 @@ __device__ __forceinline__ void cp_async_wait() {
 // through the slots behind its own; the caller keeps a launch to 4096 tokens).
 template <int LPR, int kFmt, bool kInter>
 __global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(const __grid_constant__ RowArgs a, int first) {
-  constexpr int kRows = 32 / LPR;  // rows to be coded a warp works on at a time
+  constexpr int kRows = 32 / LPR;  // turned keys a warp works on at a time; 2 * kRows of other rows
   __shared__ __align__(16) uint8_t stage_s[kRowThreads / 32][2 * kRowStage * 1024];
   griddep_wait();  // before anything is read: only the launch itself runs beside the kernel before
   griddep_launch_dependents();
@@ -521,16 +542,27 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(cons
   const __nv_bfloat16* q_src = a.q + a.q_stride * t;
   const __nv_bfloat16* k_src = a.k + a.k_stride * t;
   const __nv_bfloat16* v_src = a.v + a.v_stride * t;
-  // for a cache: sets of kRows rows, k's and then v's
-  const int kv_sets = ceil_div(a.kv_heads, kRows);
-  auto coded = [&](int g, bool& value) {
-    value = g >= kv_sets;
-    return (value ? g - kv_sets : g) * kRows + sub;
+  // For a cache: key_sets sets of kRows keys to be turned, a lane's bytes to its own place; then sets of
+  // 2 * kRows rows that are coded as they are (v, and k before it if nothing turns it), in memory's order.
+  const bool turned = a.rot || a.k_weight;
+  const int key_sets = turned ? ceil_div(a.kv_heads, kRows) : 0, plain_sets = ceil_div(a.kv_heads, 2 * kRows);
+  const int coded_sets = key_sets + (turned ? 1 : 2) * plain_sets;
+  auto plain = [&](int g, bool& key) {  // first head of a plain set
+    const int i = g - key_sets;
+    key = !turned && i < plain_sets;
+    return (key || turned ? i : i - plain_sets) * 2 * kRows;
   };
   auto send_coded = [&](uint32_t st, int g) {
-    bool value;
-    const int h = coded(g, value);
-    if (live && g < 2 * kv_sets && h < a.kv_heads) cp_async16(st, (value ? v_src : k_src) + h * a.dim + at);
+    if (g < key_sets) {
+      const int h = g * kRows + sub;
+      if (live && h < a.kv_heads) cp_async16(st, k_src + h * a.dim + at);
+    } else if (g < coded_sets) {
+      bool key;
+      const int h = plain(g, key);
+      const __nv_bfloat16* src = (key ? k_src : v_src) + h * a.dim + 8 * lane;
+      if (h + sub < a.kv_heads) cp_async16(st, src);
+      if (h + kRows + sub < a.kv_heads) cp_async16(st + 512, src + 256);
+    }
   };
   // k and v in one group, then each set of q in its own
 #pragma unroll
@@ -590,33 +622,35 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(cons
               a.k_weight != nullptr, good);
   } else {
     if (slot < 0) return;
-    const bool turned = a.rot || a.k_weight;
     float cw[8], sw[8];
-    if (turned && back < kv_sets) {
+    if (back < key_sets) {
       LaneTurn q;
       load_turn<LPR, kInter>(a, p, a.k_weight, q);
 #pragma unroll
       for (int j = 0; j < 8; ++j) cw[j] = q.c[j] * q.w[j], sw[j] = q.s[j] * q.wp[j];
     }
     uint32_t st = stage2;
-    for (int g0 = back; g0 < 2 * kv_sets; g0 += 32 * parts) {
+    for (int g0 = back; g0 < coded_sets; g0 += 32 * parts) {
       uint32_t open = 0;  // of 32 sets: those whose codes 32 bits did not settle
 #pragma unroll 1
-      for (int i = 0, g = g0; i < 32 && g < 2 * kv_sets; ++i, g += parts) {
-        bool value;
-        const int h = coded(g, value);
-        const bool here = live && h < a.kv_heads;
-        uint4 x = make_uint4(0, 0, 0, 0);
+      for (int i = 0, g = g0; i < 32 && g < coded_sets; ++i, g += parts) {
         cp_async_wait<kRowStage - 1>();
-        if (here) x = lds128(st);
-        const size_t row = here ? a.cache.row(slot, h) : 0;
-        if (!value && turned) {
-          if (!store_keys<LPR, kFmt, kInter>(a, x, cw, sw, here, row, at)) open |= 1u << i;
+        __syncwarp();  // a plain set's bytes are copied by other lanes
+        if (g < key_sets) {
+          const int h = g * kRows + sub;
+          const bool here = live && h < a.kv_heads;
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (here) x = lds128(st);
+          if (!store_keys<LPR, kFmt, kInter>(a, x, cw, sw, here, here ? a.cache.row(slot, h) : 0, at)) open |= 1u << i;
         } else {
-          float f[8];
-          unpack_bf16x8(x, f);
-          code_and_store<kFmt>(a.cache, !value, f, here, row, at);
+          bool key;
+          const int h = plain(g, key) + sub16;
+          const bool here = h < a.kv_heads;
+          uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+          if (here) x[0] = lds128(st + 16 * lane), x[1] = lds128(st + 16 * lane + 16);
+          code_and_store16<kFmt>(a.cache, key, x, here, here ? a.cache.row(slot, h) : 0, 16 * l16);
         }
+        __syncwarp();
         send_coded(st, g + kRowStage * parts);
         cp_async_commit();
         st = st == stage2 + 1024 * (kRowStage - 1) ? stage2 : st + 1024;

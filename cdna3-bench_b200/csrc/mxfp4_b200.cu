@@ -693,7 +693,8 @@ constexpr int kStoreTokens = 4096;
 template <int LPR, int kFmt, bool kInter>
 int launch_head_rows(const RowArgs& a, cudaStream_t s, const DeviceState* d) {
   constexpr int rows = 32 / LPR;
-  const int sets = ceil_div(a.q_heads, 2 * rows) + (kFmt == kFmtNone ? ceil_div(a.kv_heads, 2 * rows) : 2 * ceil_div(a.kv_heads, rows));
+  const int plain = ceil_div(a.kv_heads, 2 * rows), keys = a.rot || a.k_weight ? ceil_div(a.kv_heads, rows) : plain;
+  const int sets = ceil_div(a.q_heads, 2 * rows) + plain + (kFmt == kFmtNone ? 0 : keys);
   const int most = kFmt == kFmtNone ? a.tokens : kStoreTokens;
   for (int first = 0; first < a.tokens; first += most) {
     const int n = std::min(most, a.tokens - first);
@@ -711,7 +712,8 @@ int launch_head_rows_dim(const RowArgs& a, cudaStream_t s) {
   DeviceState* d = nullptr;
   const int rc = current_device(&d);
   if (rc) return rc;
-  if (a.dim <= 32) return launch_head_rows<4, kFmt, kInter>(a, s, d);
+  if constexpr (kFmt == kFmtNone)  // a cache's rows are longer
+    if (a.dim <= 32) return launch_head_rows<4, kFmt, kInter>(a, s, d);
   if (a.dim <= 64) return launch_head_rows<8, kFmt, kInter>(a, s, d);
   if (a.dim <= 128) return launch_head_rows<16, kFmt, kInter>(a, s, d);
   return launch_head_rows<32, kFmt, kInter>(a, s, d);
