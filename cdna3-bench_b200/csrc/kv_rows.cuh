@@ -473,23 +473,27 @@ __device__ __forceinline__ void cp_async_wait() {
 
 // One token per blockIdx.x, a share of its head rows per warp of blockIdx.y's blocks.
 //
-// Bound by HBM: each row is read once and written once.  A warp first sends for its rows (up to
-// kRowStage sets of each kind) with asynchronous copies to shared memory, each lane's bytes to a
-// place of its own, so that bytes in flight cost no registers.  q is computed in 32 bits and rounded
+// Bound by HBM: each row is read once and written once.  A warp sends for kRowStage sets of rows of
+// each kind at once with asynchronous copies to shared memory, so that bytes in flight cost no
+// registers, and refills a set's place as soon as it is read.  q is computed in 32 bits and rounded
 // to bf16 once, with cos, sin and the weight multiplied together once per warp.  A key on its
 // way into the cache has the codes of the 64-bit value: next to a rounding border an error in the
 // 24th bit would pick the neighbouring code, and with it the stored byte would depend on how
 // the norm's sum was ordered.  store_keys settles almost all of them in 32 bits.
 //
-// Measured: 4608 tokens of 24 + 24 heads of 128, interleaved: 23.8 us, 4.8 TB/s, 73 % of the HBM copy
+// Measured: 4608 tokens of 24 + 24 heads of 128, interleaved: 23.0 us, 5.0 TB/s, 77 % of the HBM copy
 // rate; a set of 4 rows is 153 instructions and a warp's start 414, so it is bound by issue and by the
 // short lives of its warps as much as by bytes.  4096 tokens of 64 + 8 + 8 heads with the cache
-// write: 44 us, 3.5 TB/s, 54 %: the keys' intervals and codes are 370 instructions per two rows.
-// 64-thread blocks against 128: 24.7 and 27.8 us on the first; 8 values to a lane with the partner
-// brought by shuffles: 26.4 us there and 62 us against 54 on the second; a persistent ring over the
-// tokens: no faster (33 and 71 us), its bookkeeping costs what it hides.
+// write: 38.2 us, 4.1 TB/s, 63 %; 2780 instructions per warp, 61 % of the issue slots.  There the rows of q
+// are 18 us of it, the keys' intervals 3, the look through later slots 2, the exact path 0.2.
+// Tried: all places refilled only when all are read 44 us (and 24.0 on the first), one ring for all
+// kinds 40.6 (26.0); kRowStage 2, 3, 4: 40.2, 38.8, 40.9; kRowBlocks 8, 9, 10, 12: 41.6, 38.8, 38.9, 40.5;
+// 128 threads to a block 45; 8 values to a lane for all kinds with the partner brought by shuffles 52; a
+// persistent ring over the tokens no faster (its bookkeeping costs what it hides); cos, sin and weights
+// sent for before the look through the slots 38.3, and 5 % slower on small calls.
 //
-// A programmatic dependent launch, as is the read below: 2.0 -> 1.8 us for the small calls in a graph.
+// A programmatic dependent launch, as is the read below: 2 us between queued calls (26.6 -> 24.6 us on the
+// first), 2.0 -> 1.8 us for the smallest calls in a graph.
 //
 // Two tokens of one launch that name the same slot: the later one is stored (every block looks
 // through the slots behind its own; the caller keeps a launch to 4096 tokens).
@@ -693,7 +697,7 @@ __device__ __forceinline__ uint4 decode8(const uint2& w, float scale) {
 constexpr int kReadThreads = 128;
 constexpr int kReadRows = 4;  // rows per block, their loads in flight together
 
-// Bound by HBM: 20000 rows of 8 x 128 E4M3, k and v, 21.3 us, 5.8 TB/s, 89 % of the HBM copy rate.
+// Bound by HBM: 20000 rows of 8 x 128 E4M3, k and v, 20.8 us, 6.0 TB/s, 91 % of the HBM copy rate.
 // k and v of the cache rows that `slots` names, [rows][heads][dim] bf16; a negative slot reads zeros.
 template <int kFmt>
 __global__ void __launch_bounds__(kReadThreads)

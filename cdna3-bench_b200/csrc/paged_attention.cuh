@@ -26,10 +26,13 @@
 //           and a scale relative to a running one, measured 5 to 8 % faster and would lose weights
 //           below 2^-36 and values 2^-20 below the largest: not taken.)
 //           The transposition between S^T's accumulators and P^T's operand is one movmatrix per 8 keys.
-// What bounds it, measured: E4M3 D = 128, 8 heads to a kv head, 2 x 131072 keys: 92 % of the HBM copy
-// rate in steady state (91.5 us for 554 MB); 387 instructions per tile, of them 190 for V.  E2M1 is
-// bound by issue: 410 instructions per tile for half the bytes, 60 % of the issue slots, 55 % of the
-// copy rate.  D = 256: 97 % (E4M3) and 68 % (E2M1).  Two tiles to a step against one: 91 -> 84 us on 2 x
+// What bounds it, measured: E4M3 D = 128, 8 heads to a kv head, 2 x 131072 keys: 94 % of the HBM copy
+// rate in steady state (89.9 us for 554 MB); 387 instructions per tile, of them 190 for V.  E2M1 is
+// bound by issue: 400 instructions per tile for half the bytes, 67 % of the issue slots, 56 % of the
+// copy rate (78.0 us); with 1, 2, 3, 4 tiles to a step 83, 78, 76, 75 us there but 80, 76, 82, 90 on 256 x 1000
+// keys; five blocks of 96 registers 89; the left shifts of its decode as multiplications by a number the
+// compiler does not know 77, and as much slower elsewhere.  D = 64: 74 % (E4M3), D = 256: 89 % (E4M3)
+// and 62 % (E2M1, 4 heads to a kv head).  Two tiles to a step against one: 91 -> 84 us on 2 x
 // ~115k keys; three resident blocks of 167 registers against four of 127: 91 -> 87 us there.  Loads
 // straight into registers (no ring): 111 us there, 12 warps cannot both hold the bytes and compute.
 //
@@ -37,12 +40,15 @@
 // units, share so that there are about as many pieces as blocks are resident: one block to a piece,
 // found from the lengths on the device, so that long and short sequences share the GPU evenly and a
 // block's first loads run beside the other blocks' work (64 ragged sequences, E2M1: 42 us; 46 with one
-// equal share of all units to a block, which then went through several heads one after another).  A head of one piece is written at
-// once; the parts of the others go to the workspace and attn_join_kernel adds them in order.
+// equal share of all units to a block, which then went through several heads one after another).  A
+// head of one piece is written at once; the parts of the others go to the workspace and
+// attn_join_kernel adds them in order.
 // Where even the longest sequence that the page table can hold is a few units, a cluster of 1 to 8
 // blocks takes a head instead and joins its parts through distributed shared memory: one launch, no
-// workspace, and each block looks at the length of its own sequence only (one sequence of 700 keys: 7.1 us
-// against 7.8; 200 of up to 500: 31 us against 67, which also paid for the joining kernel's blocks).
+// workspace, and each block looks at the length of its own sequence only (200 of up to 500 keys: 31 us
+// against 67, which also paid for the joining kernel's blocks).  Its blocks take units in turn, so that the
+// first pages are known before the length is, and all remote parts are loaded before the first is
+// used: one sequence of 700 keys 5.3 us, 7.1 without the two.
 #pragma once
 
 #include <type_traits>
