@@ -489,8 +489,9 @@ __device__ __forceinline__ void cp_async_wait() {
 // Tried: all places refilled only when all are read 44 us (and 24.0 on the first), one ring for all
 // kinds 40.6 (26.0); kRowStage 2, 3, 4: 40.2, 38.8, 40.9; kRowBlocks 8, 9, 10: 41.6, 38.8, 38.9 (12, with
 // 80 registers: 43.7 us against 40.1 on 16 + 8 heads of 256); 128 threads to a block 45; 8 values to a lane for
-// all kinds with the partner brought by shuffles: a sixth slower; a persistent ring over the tokens no faster (its bookkeeping costs what it hides); cos, sin and weights
-// sent for before the look through the slots 38.3, and 5 % slower on small calls.
+// all kinds with the partner brought by shuffles: a sixth slower; a persistent ring over the tokens no
+// faster (its bookkeeping costs what it hides); cos, sin and weights sent for before the look through
+// the slots 38.3, and 5 % slower on small calls.
 //
 // A programmatic dependent launch, as is the read below: 2 us between queued calls (26.6 -> 24.6 us on the
 // first), 2.0 -> 1.8 us for the smallest calls in a graph.
