@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
   constexpr int KT = attn_tiles(D, kFmt), kUnitKeys = attn_unit_keys(D, kFmt);
   constexpr int kKw = kRowBytes / kGroups / 16;  // words of K codes per lane, key and group: 2 or 1
   constexpr int kVw = kRowBytes / 32;            // words of V codes per lane and key
-  constexpr float kCarry = kFmt == kFmtE4M3 ? 56.0f : 62.0f;  // p carries 2^kCarry, v 2^-kCarry
+  constexpr float kRaise = kFmt == kFmtE4M3 ? 0x1p56f : 0x1p62f;  // 2^kCarry: what p carries, and v its inverse
   constexpr float kRise = 8.0f;                               // see below
   constexpr int kStride = D + 4;                              // floats per head of a warp's part in shared memory
   constexpr float kInf = __builtin_huge_valf();
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
     }
 
     float acc[D / 16][NT][4];
-    float m[NT][2], sub[NT][2], lsum[NT][2];  // reference maximum, what p's exponent subtracts, sum of p
+    float m[NT][2], sub[NT][2], lsum[NT][2];  // reference maximum, the same or 0 before any score, sum of p
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
       m[n][0] = m[n][1] = -kInf;
-      sub[n][0] = sub[n][1] = -kCarry;
+      sub[n][0] = sub[n][1] = 0.0f;
       lsum[n][0] = lsum[n][1] = 0.0f;
     }
 
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
             const float base = u == -kInf ? 0.0f : u;  // no score yet
             const float fade = exp2_approx(m[n][j] - base);
             m[n][j] = u;
-            sub[n][j] = base - kCarry;
+            sub[n][j] = base;
             lsum[n][j] *= fade;
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) acc[c][n][j] *= fade, acc[c][n][j + 2] *= fade;
@@ -574,8 +574,9 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
       for (int i = 0; i < KT; ++i)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const float p0 = exp2_approx(s[i][n][0] - sub[n][0]), p1 = exp2_approx(s[i][n][1] - sub[n][1]);
-          const float p2 = exp2_approx(s[i][n][2] - sub[n][0]), p3 = exp2_approx(s[i][n][3] - sub[n][1]);
+          // times 2^kCarry, not the exponent plus kCarry: that sum would be rounded to 2^-19
+          const float p0 = exp2_approx(s[i][n][0] - sub[n][0]) * kRaise, p1 = exp2_approx(s[i][n][1] - sub[n][1]) * kRaise;
+          const float p2 = exp2_approx(s[i][n][2] - sub[n][0]) * kRaise, p3 = exp2_approx(s[i][n][3] - sub[n][1]) * kRaise;
           lsum[n][0] += p0 + p2;
           lsum[n][1] += p1 + p3;
           // p is rounded to bf16 for the product (relative 2^-8 each at most, of either sign); the sum is not
@@ -662,7 +663,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
         l = fmaf(sm_l[w * kHeads + h], f, l);
         o.x = fmaf(x4.x, f, o.x), o.y = fmaf(x4.y, f, o.y), o.z = fmaf(x4.z, f, o.z), o.w = fmaf(x4.w, f, o.w);
       }
-      l *= exp2f(-kCarry);
+      l *= 1.0f / kRaise;
       if (whole) {
         const float r = l == 0.0f ? 0.0f : 1.0f / l;  // no key in reach (bad pages): zeros
         const size_t at = static_cast<size_t>(seq) * a.q_heads + h0 + h;

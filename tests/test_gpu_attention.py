@@ -11,9 +11,8 @@ Tolerances, derived:
   more for the scales); a weight is then off by 2 d + 2^-20 relative (2 d: numerator and sum) and is
   rounded to bf16 once, 2^-8; the output is rounded to bf16 once:
   |err| <= 2^-8 |o| + (2^-8 + 2 d + 2^-20) A, and |lse err| <= d + 2^-20 + 2^-22 |lse|.
-  What lies below the formats' range is lost: a weight under 2^-126 (the smallest normal fp32; the
-  kernel's own limit is 2^-182) may count as nothing, n 2^-126 max |v| in all, and the smallest bf16
-  is 2^-133.
+  What lies below the formats' range is lost: a weight under 2^-126 (the smallest normal fp32) may
+  count as nothing, n 2^-126 max |v| in all, and the smallest bf16 is 2^-133.
 """
 
 import numpy as np
@@ -536,6 +535,19 @@ def test_attention_into_its_own_query(mx, seqs, longest, heads):
     want = mx.paged_attention(q, cache, table, i32(lengths))
     assert mx.paged_attention(q, cache, table, i32(lengths), out=q) is not None
     assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,heads,kv,longest", [(64, 40, 2, 40), (128, 64, 8, 700), (256, 16, 4, 30), (128, 8, 8, 12000)])
+def test_weights_of_nearly_equal_scores(mx, fmt, dim, heads, kv, longest):
+    """Scores near zero: nothing but the exponential's and the sums' own errors is left of the bounds."""
+    rng = np.random.default_rng(longest)
+    lengths = [longest, 10, 3, longest // 2]
+    cache = random_cache(mx, rng, 250, kv, dim, 64, fmt)
+    table = rng.integers(0, 250, (4, -(-longest // 64)))
+    q = bf16(rng, (4, heads, dim), 0.01)
+    got, lse = mx.paged_attention(q, cache, i32(table), i32(lengths), scale=0.01, return_lse=True)
+    check_attention(got, lse, q, cache, table, lengths, 0.01)
 
 
 def test_bad_pages_and_lengths(mx):
