@@ -43,7 +43,7 @@ def ref_gemm(A: np.ndarray, B_packed: np.ndarray, B_scales: np.ndarray) -> np.nd
     return A32 @ dequantize_ref_layout(B_packed, B_scales)
 
 
-# ---- the attention operators' checkers (no counterpart in the reference), in fp64
+# ---- plain forms of the attention operators (no counterpart in the reference), in fp64
 _E4M3 = np.array([(-1.0) ** (c >> 7) * ((c & 7) * 2.0**-9 if not c >> 3 & 15 else (1 + (c & 7) / 8) * 2.0 ** ((c >> 3 & 15) - 7))
                   for c in range(256)])
 _E4M3[0x7F] = _E4M3[0xFF] = np.nan
