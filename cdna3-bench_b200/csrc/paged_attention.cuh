@@ -25,7 +25,8 @@
 //           keys' scales are; larger ones count as 2^63.  (f16 here, with the hardware's conversion
 //           and a scale relative to a running one, measured 5 to 8 % faster and would lose weights
 //           below 2^-36 and values 2^-20 below the largest: not taken.)
-//           The transposition between S^T's accumulators and P^T's operand is one movmatrix per 8 keys.
+//           P^T is two bf16 operands whose sum holds 16 bits of each weight, so the output is rounded once.
+//           The transposition between S^T's accumulators and P^T's operands is one movmatrix each per 8 keys.
 // What bounds it, measured: E4M3 D = 128, 8 heads to a kv head, 2 x 131072 keys: 94 % of the HBM copy
 // rate in steady state (89.9 us for 554 MB); 387 instructions per tile, of them 190 for V.  E2M1 is
 // bound by issue: 400 instructions per tile for half the bytes, 67 % of the issue slots, 56 % of the
@@ -571,7 +572,9 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
             for (int c = 0; c < D / 16; ++c) acc[c][n][j] *= fade, acc[c][n][j + 2] *= fade;
           }
       }
-      uint32_t p[KT][NT][2];
+      // p as the sum of two bf16 values, the rounded weight and what that rounding left: relative 2^-16 at
+      // most (each rounds by 2^-8), where the rounded weight alone is off by as much as the output's own rounding.
+      uint32_t p[KT][NT][2], rest[KT][NT][2];
 #pragma unroll
       for (int i = 0; i < KT; ++i)
 #pragma unroll
@@ -581,9 +584,11 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
           const float p2 = exp2_approx(s[i][n][2] - sub[n][0]) * kRaise, p3 = exp2_approx(s[i][n][3] - sub[n][1]) * kRaise;
           lsum[n][0] += p0 + p2;
           lsum[n][1] += p1 + p3;
-          // p is rounded to bf16 for the product (relative 2^-8 each at most, of either sign); the sum is not
-          p[i][n][0] = transpose8x8(pack_bf16x2(p0, p1));
-          p[i][n][1] = transpose8x8(pack_bf16x2(p2, p3));
+          const uint32_t p01 = pack_bf16x2(p0, p1), p23 = pack_bf16x2(p2, p3);
+          p[i][n][0] = transpose8x8(p01);
+          p[i][n][1] = transpose8x8(p23);
+          rest[i][n][0] = transpose8x8(pack_bf16x2(p0 - bf16_lo(p01), p1 - bf16_hi(p01)));
+          rest[i][n][1] = transpose8x8(pack_bf16x2(p2 - bf16_lo(p23), p3 - bf16_hi(p23)));
         }
       // output
 #pragma unroll
@@ -610,8 +615,10 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
 #pragma unroll
         for (int c = 0; c < D / 16; ++c)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n) {
             mma_bf16_16816(acc[c][n], va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], p[i][n][0], p[i][n][1]);
+            mma_bf16_16816(acc[c][n], va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], rest[i][n][0], rest[i][n][1]);
+          }
       }
     };
 #pragma unroll 1

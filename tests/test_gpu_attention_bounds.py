@@ -1,0 +1,48 @@
+"""Bounds and ranges of the attention operators that hold past what tests/test_gpu_attention.py asks for."""
+
+import numpy as np
+import pytest
+import torch
+
+import _attention_ref as ref
+from test_gpu_attention import FORMATS, _no_device_error, bf16, f64, i32, mx, random_cache, random_table  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def rows_of(cache, pages, n):
+    """k and v of the first n keys of a sequence, in 64 bits [n, kv_heads, dim]."""
+    out = []
+    for codes, scales in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)):
+        c, s = (t.cpu().numpy()[pages].swapaxes(1, 2) for t in (codes, scales))
+        out.append(ref.values(c.reshape(-1, *c.shape[2:])[:n], s.reshape(-1, *s.shape[2:])[:n], cache.format))
+    return out
+
+
+def check(got, lse, q, cache, table, lengths, scale):
+    """Scores are fp32 sums of exact products, off by d = 2^-15 S as in test_gpu_attention.py; a weight by 2 d +
+    2^-20 of the exponential and the sum, and by 2^-16 as the sum of two bf16 values (2^-8 each); the output
+    is rounded to bf16 once, by 2^-8 of itself:  |err| <= 2^-8 |o| + (2^-16 + 2 d + 2^-20) A."""
+    got, qq = f64(got), f64(q)
+    for b, n in enumerate(lengths):
+        k, v = rows_of(cache, table[b, : -(-n // cache.page_size)], n)
+        o, l, mag, size = ref.attention(qq[b], k, v, scale)
+        d = 2.0**-15 * size
+        lost = 2.0**-133 + n * 2.0**-126 * np.abs(v).max()
+        bad = ~(np.abs(got[b] - o) <= 2.0**-8 * np.abs(o) + (2.0**-16 + 2 * d[:, None] + 2.0**-20) * mag + lost)
+        assert not bad.any(), (b, n, int(bad.sum()), got[b][bad][:4], o[bad][:4])
+        if lse is not None:
+            assert (np.abs(f64(lse)[b] - l) <= d + 2.0**-20 + 2.0**-22 * np.abs(l)).all(), (b, n)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,heads,kv", [(64, 4, 2), (64, 24, 2), (128, 8, 1), (128, 16, 1), (256, 3, 1), (256, 20, 2)])
+def test_output_is_rounded_once(mx, fmt, dim, heads, kv):
+    """Values of both signs whose sum is far smaller than they are: a weight rounded to 8 bits would show."""
+    rng = np.random.default_rng(dim + heads)
+    lengths = [3, 40, 129, 700, 6000]
+    cache = random_cache(mx, rng, 110, kv, dim, 64, fmt)
+    table = random_table(rng, cache, lengths)
+    q = bf16(rng, (len(lengths), heads, dim), 0.05)
+    out, lse = mx.paged_attention(q, cache, i32(table), i32(lengths), scale=0.1, return_lse=True)
+    check(out, lse, q, cache, table, lengths, 0.1)
