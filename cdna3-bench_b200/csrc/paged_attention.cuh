@@ -315,15 +315,27 @@ __device__ __forceinline__ uint32_t v_factor(uint32_t b0, uint32_t b1) {
 }
 
 // V operand words of one pair of keys: for each of the lane's D / 8 values, (key a, key b) as
-// bf16x2 times the keys' factors.
-template <int D, int kFmt>
-__device__ __forceinline__ void v_pairs(const uint32_t* a, const uint32_t* b, uint32_t factor, uint32_t (&o)[D / 8]) {
+// bf16x2 times the keys' factors.  E4M3: `most` follows the largest magnitudes, each half of it, and with
+// kNan the NaN codes become NaN.
+template <int D, int kFmt, bool kNan>
+__device__ __forceinline__ void v_pairs(const uint32_t* a, const uint32_t* b, uint32_t factor, uint32_t (&o)[D / 8], uint32_t& most) {
   if constexpr (kFmt == kFmtE4M3) {
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      // the two codes in the high bytes of the halves; low bytes are masked away
-      const uint32_t x = prmt(a[i / 4], b[i / 4], ((4 + (i & 3)) << 12) | ((i & 3) << 4));
-      o[i] = mul_bf16x2(((x >> 4) & 0x07F007F0u) | (x & 0x80008000u), factor);
+    for (int i = 0; i < D / 8; i += 2) {
+      uint32_t m[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // the two codes in the high bytes of the halves; low bytes are masked away
+        const uint32_t x = prmt(a[i / 4], b[i / 4], ((4 + ((i + j) & 3)) << 12) | (((i + j) & 3) << 4));
+        m[j] = (x >> 4) & 0x07F007F0u;
+        uint32_t v = m[j] | (x & 0x80008000u);
+        if constexpr (kNan) {
+          if ((v & 0x7FFFu) == 0x07F0u) v |= 0x7FC0u;
+          if ((v & 0x7FFF0000u) == 0x07F00000u) v |= 0x7FC00000u;
+        }
+        o[i + j] = mul_bf16x2(v, factor);
+      }
+      most = __vimax3_u16x2(most, m[0], m[1]);
     }
   } else {
 #pragma unroll
@@ -337,6 +349,8 @@ __device__ __forceinline__ void v_pairs(const uint32_t* a, const uint32_t* b, ui
     }
   }
 }
+// Whether v_pairs met a NaN code, all ones: moved into bf16 it would be 480, 0x07F0, the most there can be.
+__device__ __forceinline__ bool has_nan_code(uint32_t most) { return ((most + 0x00100010u) & 0x08000800u) != 0; }
 
 template <int D, int kFmt, int NT>
 __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn_kernel(const __grid_constant__ AttnArgs a) {
@@ -389,12 +403,13 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
       const int units = attn_units(a, seq, kUnitKeys);
       first = static_cast<int>(static_cast<long long>(units) * me.index / me.of);
       tile_last = min(static_cast<int>(static_cast<long long>(units) * (me.index + 1) / me.of) * kAttnWarps * KT, tile_last);
-#pragma unroll
-      for (int i = 0; i < KT; ++i) {
-        const int at = (first * kAttnWarps + warp) * KT + i;
-        page[i] = at < tile_last ? __ldg(table + (at >> tile_shift)) : 0;
-      }
     }
+    const int tile_first = (first * kAttnWarps + warp) * KT;
+    auto first_pages = [&]() {
+#pragma unroll
+      for (int i = 0; i < KT; ++i) page[i] = tile_first + i < tile_last ? __ldg(table + ((tile_first + i) >> tile_shift)) : 0;
+    };
+    if (!a.cluster) first_pages();
     const int head = me.head_chunk / a.chunks, chunk = me.head_chunk - head * a.chunks;
     const int h0 = head * a.group + chunk * kHeads;                  // first q head
     const int nh = min(kHeads, a.group - chunk * kHeads);            // q heads here
@@ -402,7 +417,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
     // Copies into the ring, one commit group per step; the pages of the step after are on their way.
     // `good` has KT bits for each of the last copies: whether the tile's page is one of the cache's.
     uint32_t good = 0;
-    int copy_tile = (first * kAttnWarps + warp) * KT, copy_slot = 0;
+    int copy_tile = tile_first, copy_slot = 0;
     const uint32_t page_rows = static_cast<uint32_t>(a.cache.heads) << a.cache.page_shift;
     const size_t head_rows = static_cast<size_t>(head) << a.cache.page_shift;
     const uint8_t* k_lane = a.cache.k_codes + head_rows * kRowBytes + 16 * lane;
@@ -468,20 +483,23 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
 
     float acc[D / 16][NT][4];
     float m[NT][2], sub[NT][2], lsum[NT][2];  // reference maximum, the same or 0 before any score, sum of p
+    auto clear = [&]() {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i)
+        for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
-      m[n][0] = m[n][1] = -kInf;
-      sub[n][0] = sub[n][1] = 0.0f;
-      lsum[n][0] = lsum[n][1] = 0.0f;
-    }
+          for (int j = 0; j < 4; ++j) acc[i][n][j] = 0.0f;
+        m[n][0] = m[n][1] = -kInf;
+        sub[n][0] = sub[n][1] = 0.0f;
+        lsum[n][0] = lsum[n][1] = 0.0f;
+      }
+    };
+    clear();
 
-    int slot = 0;
-    // One step; `ragged`: the sequence ends inside it, or a page of it is missing.
-    auto do_step = [&](int tile, uint32_t have, uint32_t at, auto ragged) {
+    uint32_t most = 0;  // of V's codes: see has_nan_code
+    // One step; `ragged`: the sequence ends inside it, or a page of it is missing; `careful`: see below.
+    auto do_step = [&](int tile, uint32_t have, uint32_t at, auto ragged, auto careful) {
       // scores
       float s[KT][NT][4];
 #pragma unroll
@@ -610,8 +628,8 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
             }
         }
         uint32_t va[D / 8], vb[D / 8];
-        v_pairs<D, kFmt>(w[0], w[1], v_factor(vs[0], vs[1]), va);
-        v_pairs<D, kFmt>(w[2], w[3], v_factor(vs[2], vs[3]), vb);
+        v_pairs<D, kFmt, decltype(careful)::value>(w[0], w[1], v_factor(vs[0], vs[1]), va, most);
+        v_pairs<D, kFmt, decltype(careful)::value>(w[2], w[3], v_factor(vs[2], vs[3]), vb, most);
 #pragma unroll
         for (int c = 0; c < D / 16; ++c)
 #pragma unroll
@@ -621,17 +639,38 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
           }
       }
     };
+    auto walk = [&](auto careful) {
+      int slot = 0;
 #pragma unroll 1
-    for (int tile = (first * kAttnWarps + warp) * KT; tile < tile_last; tile += a.stride) {
-      cp_async_wait<kRing - 2>();
-      __syncwarp();  // every lane's copies have landed, and all lanes have left the slot copied into next
-      copy_next();
-      const uint32_t at = ring + slot * KT * kTile, have = (good >> (KT * (kRing - 1))) & ((1u << KT) - 1);
-      slot = slot + 1 == kRing ? 0 : slot + 1;
-      if (have == (1u << KT) - 1 && (tile + KT) * 16 <= len) do_step(tile, have, at, std::false_type{});
-      else if (have) do_step(tile, have, at, std::true_type{});
-    }
-    cp_async_wait<0>();
+      for (int tile = tile_first; tile < tile_last; tile += a.stride) {
+        cp_async_wait<kRing - 2>();
+        __syncwarp();  // every lane's copies have landed, and all lanes have left the slot copied into next
+        copy_next();
+        const uint32_t at = ring + slot * KT * kTile, have = (good >> (KT * (kRing - 1))) & ((1u << KT) - 1);
+        slot = slot + 1 == kRing ? 0 : slot + 1;
+        if constexpr (decltype(careful)::value) {
+          if (have) do_step(tile, have, at, std::true_type{}, careful);
+        } else if (have == (1u << KT) - 1 && (tile + KT) * 16 <= len) {
+          do_step(tile, have, at, std::false_type{}, careful);
+        } else if (have) {
+          do_step(tile, have, at, std::true_type{}, careful);
+        }
+      }
+      cp_async_wait<0>();
+    };
+    walk(std::false_type{});
+    // A NaN code among the values: this warp's steps once more, with care for them.  The first walk only
+    // follows whether there was one (16 of its 400 instructions per tile): a branch for it in the loop cost 14 %.
+    if constexpr (kFmt == kFmtE4M3)
+      if (__any_sync(0xffffffffu, has_nan_code(most))) {
+        __syncwarp();  // all lanes have left the ring
+        clear();
+        copy_tile = tile_first, copy_slot = 0;
+        first_pages();
+#pragma unroll 1
+        for (int i = 0; i < kRing - 1; ++i) copy_next();
+        walk(std::true_type{});
+      }
     // Not earlier: the blocks of a call after this one would fill up the SMs that are busy already.
     griddep_launch_dependents();
     __syncthreads();  // the rings become the buffer of the parts

@@ -22,14 +22,17 @@ def rows_of(cache, pages, n):
 def check(got, lse, q, cache, table, lengths, scale):
     """Scores are fp32 sums of exact products, off by d = 2^-15 S as in test_gpu_attention.py; a weight by 2 d +
     2^-20 of the exponential and the sum, and by 2^-16 as the sum of two bf16 values (2^-8 each); the output
-    is rounded to bf16 once, by 2^-8 of itself:  |err| <= 2^-8 |o| + (2^-16 + 2 d + 2^-20) A."""
+    is rounded to bf16 once, by 2^-8 of itself:  |err| <= 2^-8 |o| + (2^-16 + 2 d + 2^-20) A.  What is NaN has to
+    be NaN, and nothing else."""
     got, qq = f64(got), f64(q)
     for b, n in enumerate(lengths):
         k, v = rows_of(cache, table[b, : -(-n // cache.page_size)], n)
         o, l, mag, size = ref.attention(qq[b], k, v, scale)
         d = 2.0**-15 * size
-        lost = 2.0**-133 + n * 2.0**-126 * np.abs(v).max()
-        bad = ~(np.abs(got[b] - o) <= 2.0**-8 * np.abs(o) + (2.0**-16 + 2 * d[:, None] + 2.0**-20) * mag + lost)
+        lost = 2.0**-133 + n * 2.0**-126 * np.nanmax(np.abs(v))
+        nan = np.isnan(o)
+        assert np.array_equal(np.isnan(got[b]), nan), (b, n)
+        bad = ~nan & ~(np.abs(got[b] - o) <= 2.0**-8 * np.abs(o) + (2.0**-16 + 2 * d[:, None] + 2.0**-20) * mag + lost)
         assert not bad.any(), (b, n, int(bad.sum()), got[b][bad][:4], o[bad][:4])
         if lse is not None:
             assert (np.abs(f64(lse)[b] - l) <= d + 2.0**-20 + 2.0**-22 * np.abs(l)).all(), (b, n)
@@ -46,3 +49,24 @@ def test_output_is_rounded_once(mx, fmt, dim, heads, kv):
     q = bf16(rng, (len(lengths), heads, dim), 0.05)
     out, lse = mx.paged_attention(q, cache, i32(table), i32(lengths), scale=0.1, return_lse=True)
     check(out, lse, q, cache, table, lengths, 0.1)
+
+
+@pytest.mark.parametrize("dim,heads,kv", [(64, 4, 2), (64, 32, 2), (128, 8, 2), (128, 24, 2), (256, 6, 2)])
+@pytest.mark.parametrize("longest,seqs", [(5, 6), (700, 6), (30000, 2), (900, 130)])
+def test_nan_codes_of_values_are_nan(mx, dim, heads, kv, longest, seqs):
+    """The two E4M3 codes that are NaN, in single values of every sequence but the last: at the first and last key and in
+    between, in all places of a word.  Their own outputs are NaN, as kv_cache_read says, and no others."""
+    rng = np.random.default_rng(dim + longest)
+    lengths = [longest] + [int(n) for n in rng.integers(3, longest + 1, seqs - 1)]
+    cache = random_cache(mx, rng, sum(-(-n // 64) for n in lengths) + 1, kv, dim, 64, "mxfp8")
+    table = random_table(rng, cache, lengths)
+    q = bf16(rng, (seqs, heads, dim))
+    want = mx.paged_attention(q, cache, i32(table), i32(lengths))
+    codes = cache.v_codes.cpu().numpy()
+    for b, n in enumerate(lengths[:-1]):
+        for key in {0, n - 1, n // 2, int(rng.integers(n))}:
+            codes[table[b, key // 64], rng.integers(kv), key % 64, rng.integers(dim)] = (0x7F, 0xFF)[key % 2]
+    cache.v_codes.copy_(torch.from_numpy(codes))
+    out, lse = mx.paged_attention(q, cache, i32(table), i32(lengths), return_lse=True)
+    assert not want.isnan().any() and torch.equal(out[-1], want[-1])
+    check(out, lse, q, cache, table, lengths, dim ** -0.5)
