@@ -20,11 +20,12 @@
 //           keys t, t + 4, t + 8, t + 12, which lie in different banks, and holds the D / 8 values from
 //           g D / 8 on: all in one 32-value group, so one scale byte per key.  The codes become bf16 by
 //           moving their fields into place, which is the value times 2^-120 (E4M3) or 2^-126
-//           (E2M1), and one exact multiply by scale * 2^64, which leaves v * 2^-kCarry (kCarry = 56 or
-//           62); p carries 2^kCarry.  bf16 has the range for any scale below 2^64 whatever the other
-//           keys' scales are; larger ones count as 2^63.  (f16 here, with the hardware's conversion
-//           and a scale relative to a running one, measured 5 to 8 % faster and would lose weights
-//           below 2^-36 and values 2^-20 below the largest: not taken.)
+//           (E2M1), and one exact multiply by scale * 2^63, which leaves v * 2^-kCarry (kCarry = 57 or
+//           63); p carries 2^kCarry.  bf16 has the range for the scale bytes 64 .. 191, whatever the other
+//           keys' are.  A warp that meets another one takes its keys again, in up to three parts of
+//           their own power of two each (see walk).  (f16 here, with the hardware's conversion and a scale
+//           relative to a running one, measured 5 to 8 % faster and would lose weights below
+//           2^-36 and values 2^-20 below the largest: not taken.)
 //           P^T is two bf16 operands whose sum holds 16 bits of each weight, so the output is rounded once.
 //           The transposition between S^T's accumulators and P^T's operands is one movmatrix each per 8 keys.
 // What bounds it, measured: E4M3 D = 128, 8 heads to a kv head, 2 x 131072 keys: 94 % of the HBM copy
@@ -306,13 +307,16 @@ __device__ __forceinline__ void e8m0x4_bf16x2(uint32_t w, uint32_t& lo, uint32_t
 __device__ __forceinline__ float bf16_lo(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t x) { return __uint_as_float(x & 0xFFFF0000u); }
 
-// bf16x2 multiplier of two keys' scale bytes (see kCarry at the top): 2^(b - 63), at most 2^127
-// (0x7F00), NaN for 255.
-__device__ __forceinline__ uint32_t v_factor(uint32_t b0, uint32_t b1) {
-  uint32_t r;
-  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(mul_bf16x2(e8m0x2_bf16x2(prmt(b0, b1, 0x0040)), 0x5F805F80u)), "r"(0x7F007F00u));
-  return r;
+// bf16x2 multiplier of two keys' scale bytes (see kCarry at the top): 2^(byte - 64), for bytes of 64 .. 191.
+__device__ __forceinline__ uint32_t v_factor(uint32_t b0, uint32_t b1) { return prmt(b0, b1, 0x5410) * 128u + 0x1F801F80u; }
+// All scale bytes come in three classes, 0 .. 63, 64 .. 191 and 192 .. 255; the multiplier 2^(byte - 64 + 64 (1 - cls)) of
+// one of class `cls` as bf16, zero for another class's, NaN for 255.
+__device__ __forceinline__ uint32_t v_class_factor(uint32_t byte, int cls) {
+  if (static_cast<int>(byte + 64) >> 7 != cls) return 0;
+  return byte == 255 ? 0x7FC0u : (byte + 63 + 64 * (1 - cls)) << 7;
 }
+// Whether one of the lane's scale bytes w (as many as mask has 0x80s) is outside 64 .. 191.
+__device__ __forceinline__ bool odd_scales(uint32_t both, uint32_t mask) { return (both & mask) != mask; }
 
 // V operand words of one pair of keys: for each of the lane's D / 8 values, (key a, key b) as
 // bf16x2 times the keys' factors.  E4M3: `most` follows the largest magnitudes, each half of it, and with
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
   constexpr int KT = attn_tiles(D, kFmt), kUnitKeys = attn_unit_keys(D, kFmt);
   constexpr int kKw = kRowBytes / kGroups / 16;  // words of K codes per lane, key and group: 2 or 1
   constexpr int kVw = kRowBytes / 32;            // words of V codes per lane and key
-  constexpr float kRaise = kFmt == kFmtE4M3 ? 0x1p56f : 0x1p62f;  // 2^kCarry: what p carries, and v its inverse
+  constexpr float kRaise = kFmt == kFmtE4M3 ? 0x1p57f : 0x1p63f;  // 2^kCarry: what p carries, and v its inverse
   constexpr float kRise = 8.0f;                               // see below
   constexpr int kStride = D + 4;                              // floats per head of a warp's part in shared memory
   constexpr float kInf = __builtin_huge_valf();
@@ -497,9 +501,50 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
     };
     clear();
 
-    uint32_t most = 0;  // of V's codes: see has_nan_code
+    // Largest of V's codes, see has_nan_code; or why else the keys have to be taken again with care (kHuge: values
+    // of 2^56 and more may be among them, whose sum could leave the range of fp32).
+    uint32_t most = 0;
+    constexpr uint32_t kCare = 0x07F007F0u, kHuge = 0x0EF00EF0u;
+    float raise = kRaise;
+    // Looks closer at a step that has value scales out of the usual range: groups of zeros (byte 0) are none of
+    // those, nor are rows of no key.
+    auto look_at_scales = [&](int tile, uint32_t have, uint32_t at) {
+      const int key = lane >> 1;
+#pragma unroll 1
+      for (int i = 0; i < KT; ++i) {
+        if (!((have >> i) & 1) || (tile + i) * 16 + key >= len) continue;
+        const uint32_t codes = at + i * kTile + (16 + key) * kRowBytes, scales = at + i * kTile + 32 * kRowBytes + (16 + key) * kGroups;
+#pragma unroll 1
+        for (int b = (lane & 1) * (kGroups / 2), e = b + kGroups / 2; b < e; ++b) {
+          const uint32_t byte = lds_u8(scales + b);
+          if (byte - 64u < 128u) continue;
+          uint32_t any = byte;
+          if (byte == 0) {
+#pragma unroll
+            for (int u = 0; u < kRowBytes / kGroups; u += 16) {
+              const uint4 x = lds128(codes + ((b * (kRowBytes / kGroups) + u) ^ (16 * attn_swizzle<D, kFmt, true>(key))));
+              any |= (x.x | x.y | x.z | x.w) & (kFmt == kFmtE4M3 ? 0x7F7F7F7Fu : 0x77777777u);
+            }
+          }
+          if (any) most = max(most, byte >= 192 ? kHuge : kCare);
+        }
+      }
+    };
     // One step; `ragged`: the sequence ends inside it, or a page of it is missing; `careful`: see below.
     auto do_step = [&](int tile, uint32_t have, uint32_t at, auto ragged, auto careful) {
+      uint32_t usual = 0xFFFFFFFFu;  // see odd_scales; the 16 keys' value scales are dealt to the lanes
+      constexpr uint32_t kUsual = kGroups == 2 ? 0x80u : (kGroups == 4 ? 0x8080u : 0x80808080u);
+      if constexpr (!decltype(careful)::value) {
+#pragma unroll
+        for (int i = 0; i < KT; ++i) {
+          const uint32_t sa = at + i * kTile + 32 * kRowBytes + 16 * kGroups + lane * (kGroups / 2);
+          uint32_t w;
+          if constexpr (kGroups == 2) w = lds_u8(sa);
+          else if constexpr (kGroups == 4) asm volatile("ld.shared.u16 %0, [%1];" : "=r"(w) : "r"(sa));
+          else w = lds32(sa);
+          usual &= w ^ (w << 1);
+        }
+      }
       // scores
       float s[KT][NT][4];
 #pragma unroll
@@ -560,7 +605,8 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
           }
       }
       // The reference m follows the running maximum only when a score passes it by kRise: p stays
-      // below 2^(kCarry + kRise), and most steps need no exchange between lanes and no rescaling.
+      // below 2^(kCarry + kRise), and most steps need no exchange between lanes and no rescaling.  (With care it
+      // follows at once: large values have no room for 2^kRise.)
       float top[NT][2];
       bool rise = false;
 #pragma unroll
@@ -570,36 +616,42 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
           top[n][j] = fmaxf(s[0][n][j], s[0][n][j + 2]);
 #pragma unroll
           for (int i = 1; i < KT; ++i) top[n][j] = fmaxf(top[n][j], fmaxf(s[i][n][j], s[i][n][j + 2]));
-          rise |= top[n][j] > m[n][j] + kRise;
+          rise |= top[n][j] > m[n][j] + (decltype(careful)::value ? 0.0f : kRise);
         }
-      if (__any_sync(0xffffffffu, rise)) {
+      const bool odd = odd_scales(usual, kUsual);
+      // One vote for both; scales may be odd in rows of no key, which must not move the reference.
+      if (__any_sync(0xffffffffu, rise || odd)) {
+        if (odd) look_at_scales(tile, have, at);
+        if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float u = fmaxf(m[n][j], top[n][j]);
-            u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 4));
-            u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 8));
-            u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 16));
-            const float base = u == -kInf ? 0.0f : u;  // no score yet
-            const float fade = exp2_approx(m[n][j] - base);
-            m[n][j] = u;
-            sub[n][j] = base;
-            lsum[n][j] *= fade;
+            for (int j = 0; j < 2; ++j) {
+              float u = fmaxf(m[n][j], top[n][j]);
+              u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 4));
+              u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 8));
+              u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 16));
+              const float base = u == -kInf ? 0.0f : u;  // no score yet
+              const float fade = exp2_approx(m[n][j] - base);
+              m[n][j] = u;
+              sub[n][j] = base;
+              lsum[n][j] *= fade;
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) acc[c][n][j] *= fade, acc[c][n][j + 2] *= fade;
-          }
+              for (int c = 0; c < D / 16; ++c) acc[c][n][j] *= fade, acc[c][n][j + 2] *= fade;
+            }
+        }
       }
       // p as the sum of two bf16 values, the rounded weight and what that rounding left: relative 2^-16 at
       // most (each rounds by 2^-8), where the rounded weight alone is off by as much as the output's own rounding.
       uint32_t p[KT][NT][2], rest[KT][NT][2];
+      const float up = decltype(careful)::value ? raise : kRaise;
 #pragma unroll
       for (int i = 0; i < KT; ++i)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           // times 2^kCarry, not the exponent plus kCarry: that sum would be rounded to 2^-19
-          const float p0 = exp2_approx(s[i][n][0] - sub[n][0]) * kRaise, p1 = exp2_approx(s[i][n][1] - sub[n][1]) * kRaise;
-          const float p2 = exp2_approx(s[i][n][2] - sub[n][0]) * kRaise, p3 = exp2_approx(s[i][n][3] - sub[n][1]) * kRaise;
+          const float p0 = exp2_approx(s[i][n][0] - sub[n][0]) * up, p1 = exp2_approx(s[i][n][1] - sub[n][1]) * up;
+          const float p2 = exp2_approx(s[i][n][2] - sub[n][0]) * up, p3 = exp2_approx(s[i][n][3] - sub[n][1]) * up;
           lsum[n][0] += p0 + p2;
           lsum[n][1] += p1 + p3;
           const uint32_t p01 = pack_bf16x2(p0, p1), p23 = pack_bf16x2(p2, p3);
@@ -628,15 +680,38 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
             }
         }
         uint32_t va[D / 8], vb[D / 8];
-        v_pairs<D, kFmt, decltype(careful)::value>(w[0], w[1], v_factor(vs[0], vs[1]), va, most);
-        v_pairs<D, kFmt, decltype(careful)::value>(w[2], w[3], v_factor(vs[2], vs[3]), vb, most);
+        if constexpr (decltype(careful)::value) {
+#pragma unroll 1
+          for (int cls = 0; cls < 3; ++cls) {
+            uint32_t f[4];
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c)
+            for (int j = 0; j < 4; ++j) f[j] = v_class_factor(vs[j], cls);
+            if (!__any_sync(0xffffffffu, (f[0] | f[1] | f[2] | f[3]) != 0)) continue;
+            v_pairs<D, kFmt, true>(w[0], w[1], f[0] | f[1] << 16, va, most);
+            v_pairs<D, kFmt, true>(w[2], w[3], f[2] | f[3] << 16, vb, most);
+            const float unit = cls == 0 ? 0x1p-64f : (cls == 1 ? 1.0f : 0x1p64f);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_bf16_16816(acc[c][n], va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], p[i][n][0], p[i][n][1]);
-            mma_bf16_16816(acc[c][n], va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], rest[i][n][0], rest[i][n][1]);
+            for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma_bf16_16816(o, va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], p[i][n][0], p[i][n][1]);
+                mma_bf16_16816(o, va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], rest[i][n][0], rest[i][n][1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[c][n][j] = fmaf(o[j], unit, acc[c][n][j]);
+              }
           }
+        } else {
+          v_pairs<D, kFmt, false>(w[0], w[1], v_factor(vs[0], vs[1]), va, most);
+          v_pairs<D, kFmt, false>(w[2], w[3], v_factor(vs[2], vs[3]), vb, most);
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_bf16_16816(acc[c][n], va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], p[i][n][0], p[i][n][1]);
+              mma_bf16_16816(acc[c][n], va[2 * c], va[2 * c + 1], vb[2 * c], vb[2 * c + 1], rest[i][n][0], rest[i][n][1]);
+            }
+        }
       }
     };
     auto walk = [&](auto careful) {
@@ -659,18 +734,24 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
       cp_async_wait<0>();
     };
     walk(std::false_type{});
-    // A NaN code among the values: this warp's steps once more, with care for them.  The first walk only
-    // follows whether there was one (16 of its 400 instructions per tile): a branch for it in the loop cost 14 %.
-    if constexpr (kFmt == kFmtE4M3)
-      if (__any_sync(0xffffffffu, has_nan_code(most))) {
-        __syncwarp();  // all lanes have left the ring
-        clear();
-        copy_tile = tile_first, copy_slot = 0;
-        first_pages();
+    // A NaN code among the values, or a value scale out of the usual range: this warp's steps once more,
+    // with care for them.  The first walk only follows whether there was one (a branch for NaN codes in its loop cost
+    // 14 %, the largest code 6 %).
+    if (__any_sync(0xffffffffu, has_nan_code(most))) {
+      __syncwarp();  // all lanes have left the ring
+      const bool huge = __any_sync(0xffffffffu, most >= kHuge);
+      if (huge) raise = kRaise * 0x1p-40f;
+      clear();
+      copy_tile = tile_first, copy_slot = 0;
+      first_pages();
 #pragma unroll 1
-        for (int i = 0; i < kRing - 1; ++i) copy_next();
-        walk(std::true_type{});
+      for (int i = 0; i < kRing - 1; ++i) copy_next();
+      walk(std::true_type{});
+      if (huge) {  // the sums are 2^-40 of what they stand for, as if the reference were 40 more
+#pragma unroll
+        for (int n = 0; n < NT; ++n) m[n][0] += 40.0f, m[n][1] += 40.0f;
       }
+    }
     // Not earlier: the blocks of a call after this one would fill up the SMs that are busy already.
     griddep_launch_dependents();
     __syncthreads();  // the rings become the buffer of the parts

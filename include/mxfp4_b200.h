@@ -292,8 +292,8 @@ int mxfp4_kv_cache_read(const mxfp4_kv_cache* cache, const int* slots, int token
 /* Attention of one new token per sequence: out[s][h] = softmax(scale * q[s][h] . k) v over the
  * first lengths[s] keys of the sequence, key j being row j % page_size of page
  * page_table[s][j / page_size] of kv head h / (num_heads / num_kv_heads); the keys and values are
- * those mxfp4_kv_cache_read returns before its rounding to bf16 (value scales of 2**64 and more count as
- * 2**63, and scores past the range of fp32 as infinite).  lse (NULL: not wanted) fp32 [seqs][num_heads] is the natural log of the sum of
+ * those mxfp4_kv_cache_read returns before its rounding to bf16 (scores past the range of fp32 count as
+ * infinite).  lse (NULL: not wanted) fp32 [seqs][num_heads] is the natural log of the sum of
  * exp(scale * q . k).  A length of zero or less gives zeros and -inf.  Page-table entries past a
  * sequence's last page are not read.
  * q bf16 [seqs] rows of num_heads * head_dim, q_stride elements apart (a multiple of 8); out bf16

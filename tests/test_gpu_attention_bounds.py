@@ -70,3 +70,74 @@ def test_nan_codes_of_values_are_nan(mx, dim, heads, kv, longest, seqs):
     out, lse = mx.paged_attention(q, cache, i32(table), i32(lengths), return_lse=True)
     assert not want.isnan().any() and torch.equal(out[-1], want[-1])
     check(out, lse, q, cache, table, lengths, dim ** -0.5)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,heads,kv", [(64, 3, 1), (64, 12, 1), (128, 8, 1), (128, 16, 1), (256, 5, 1)])
+def test_value_scales_of_the_whole_range(mx, fmt, dim, heads, kv):
+    """A sequence per scale byte of V, from the smallest to the largest whose values bf16 holds: none of them is
+    lost, and none counts as another."""
+    rng = np.random.default_rng(dim)
+    last = 245 if fmt == "mxfp8" else 251
+    bytes_ = [*range(0, 66), 100, 140, *range(188, 195), 220, last - 1, last]
+    n = 37
+    lengths = [n] * len(bytes_)
+    cache = random_cache(mx, rng, len(bytes_), kv, dim, 64, fmt)
+    table = random_table(rng, cache, lengths)
+    for b, byte in enumerate(bytes_):
+        cache.v_scales[table[b, 0]] = byte
+    q = bf16(rng, (len(bytes_), heads, dim), 0.05)
+    out, lse = mx.paged_attention(q, cache, i32(table), i32(lengths), scale=0.1, return_lse=True)
+    check(out, lse, q, cache, table, lengths, 0.1)
+    assert (out.float().abs().amax((1, 2)) > 0).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,heads,kv", [(64, 4, 2), (128, 12, 1), (256, 2, 1)])
+@pytest.mark.parametrize("longest,seqs", [(40, 8), (700, 8), (20000, 3)])
+def test_value_scales_of_all_sizes_together(mx, fmt, dim, heads, kv, longest, seqs):
+    """Groups of a sequence from classes far apart, a key of tiny or huge values among ordinary ones, and keys whose
+    weight decides which of them counts: in full steps and at the end of a sequence."""
+    rng = np.random.default_rng(longest + dim)
+    lengths = [longest] + [int(n) for n in rng.integers(1, longest + 1, seqs - 1)]
+    cache = random_cache(mx, rng, sum(-(-n // 64) for n in lengths) + 1, kv, dim, 64, fmt)
+    table = random_table(rng, cache, lengths)
+    scales = cache.v_scales.cpu().numpy()
+    for b, n in enumerate(lengths):
+        pages = table[b, : -(-n // 64)]
+        if b % 4 == 0:
+            scales[pages] = rng.integers(0, 240, scales[pages].shape)
+        elif b % 4 == 1:
+            scales[pages] = rng.integers(30, 100, scales[pages].shape)
+        elif b % 4 == 2:  # one key's groups
+            scales[pages[-1], :, (n - 1) % 64] = 20
+            scales[pages[0], :, 0, 0] = 230
+        else:
+            scales[pages] = rng.choice([0, 62, 63, 64, 65], scales[pages].shape)
+    cache.v_scales.copy_(torch.from_numpy(scales))
+    q = bf16(rng, (seqs, heads, dim))
+    out, lse = mx.paged_attention(q, cache, i32(table), i32(lengths), return_lse=True)
+    check(out, lse, q, cache, table, lengths, dim ** -0.5)
+    again = mx.paged_attention(q, cache, i32(table), i32(lengths))
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_groups_of_zeros_among_values(mx, fmt, dim):
+    """The coder gives them scale byte 0, which is the smallest scale there is when the codes are not zeros."""
+    rng = np.random.default_rng(dim)
+    n = 150
+    cache = mx.new_kv_cache(6, 1, dim, 64, fmt)
+    k, v = bf16(rng, (2 * n, 1, dim)), bf16(rng, (2 * n, 1, dim))
+    v[:, :, dim // 2:] = 0
+    v[3:9, :, :32] = -0.0
+    v[n + 100, :, dim // 2:] = 2.0**-119  # nearly a group of zeros, in the second sequence
+    pos = np.arange(n)
+    table = np.array([[0, 1, 2], [3, 4, 5]])
+    slots = np.r_[pos, 192 + pos]
+    mx.kv_cache_write(cache, k, v, i32(slots))
+    q = bf16(rng, (2, 4, dim))
+    out, lse = mx.paged_attention(q, cache, i32(table), i32([n, n]), return_lse=True)
+    check(out, lse, q, cache, table, [n, n], dim ** -0.5)
+    assert (out[0, :, dim // 2:] == 0).all() and (out[1, :, dim // 2:] > 0).all()
