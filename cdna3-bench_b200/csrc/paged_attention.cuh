@@ -13,9 +13,10 @@
 //   scores  S^T[key][head] = K Q^T, K as the 16-row operand (m16n8k16, f16): row g is key
 //           pi(g) = g / 2 + 4 (g % 2), row g + 8 key pi(g) + 8.  Lane (g, t) holds their values 32 b + 8 t
 //           .. + 7 of each 32-value group b (any order of the values serves, if q has the same).  The
-//           codes convert exactly to f16; q is scaled per head by a power of two so that f16
-//           holds every bf16 bit of it, and each group's fp32 partial is multiplied by the key's
-//           scale.
+//           codes convert exactly to f16; q is scaled per head by a power of two, with which f16
+//           holds every bf16 bit of values down to 2^-31 of the head's largest, and each group's
+//           fp32 partial is multiplied by the key's scale.  Where q has smaller ones, or a scale byte is outside
+//           64 .. 191, q goes through in levels of 31 binades each (see walk).
 //   output  O^T[d][head] = V^T P^T, V as the 16-row operand (m16n8k16, bf16).  With pi, lane (g, t) needs
 //           keys t, t + 4, t + 8, t + 12, which lie in different banks, and holds the D / 8 values from
 //           g D / 8 on: all in one 32-value group, so one scale byte per key.  The codes become bf16 by
@@ -356,6 +357,18 @@ __device__ __forceinline__ void v_pairs(const uint32_t* a, const uint32_t* b, ui
 // Whether v_pairs met a NaN code, all ones: moved into bf16 it would be 480, 0x07F0, the most there can be.
 __device__ __forceinline__ bool has_nan_code(uint32_t most) { return ((most + 0x00100010u) & 0x08000800u) != 0; }
 
+// Exponent of a finite bf16 that is not zero: |x| is in [2^e, 2^(e + 1)).
+__device__ __forceinline__ int bf16_exponent(uint32_t mag) { return mag >= 0x80u ? static_cast<int>(mag >> 7) - 127 : -102 - __clz(mag); }
+// The level of a query value, scaled by 2^shift so that the head's largest is in [2^14, 2^15).
+__device__ __forceinline__ int q_level(uint32_t mag, int shift) { return (14 - (bf16_exponent(mag) + shift)) / 31; }
+// x * 2^(shift + 31 * level) in f16 if x is of that level (exact: 8 bits of at least 2^-16), else zero.
+__device__ __forceinline__ uint32_t q_of_level(uint32_t x, int shift, int level) {
+  const uint32_t mag = x & 0x7FFFu;
+  if (mag >= 0x7F80u) return level ? 0u : (mag > 0x7F80u ? 0x7FFFu : 0x7C00u | (x & 0x8000u));
+  if (mag == 0 || q_level(mag, shift) != level) return 0;
+  return __half_as_ushort(__float2half_rn(ldexpf(__uint_as_float(x << 16), shift + 31 * level)));
+}
+
 template <int D, int kFmt, int NT>
 __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int kGroups = D / 32, kHeads = 8 * NT, kRing = attn_ring(D, kFmt);
@@ -455,19 +468,24 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
     // Q operand: head g of n-tile n, values 32 b + 8 t .. + 7, scaled into f16
     uint32_t q[NT][kGroups][4];
     float mult[NT][2];  // of heads 2t, 2t+1: scale * log2(e) / the power of two
+    bool held = true;   // f16 and fp32 hold all of that
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const bool real = 8 * n + g < nh;
       const __nv_bfloat16* src = a.q + a.q_stride * seq + static_cast<size_t>(h0 + 8 * n + g) * D + 8 * t;
-      uint32_t amax = 0;
+      uint32_t large = 0, least = 0x7FFF7FFFu;  // least: magnitudes - 0x8001 in signed 16 bits, of zero the most
 #pragma unroll
       for (int b = 0; b < kGroups; ++b) {
         uint4 x = make_uint4(0, 0, 0, 0);
         if (real) x = *reinterpret_cast<const uint4*>(src + 32 * b);
         q[n][b][0] = x.x, q[n][b][1] = x.y, q[n][b][2] = x.z, q[n][b][3] = x.w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) amax = max(amax, max(q[n][b][i] & 0x7FFFu, (q[n][b][i] >> 16) & 0x7FFFu));
+        for (int i = 0; i < 4; i += 2) {
+          large = __vimax3_u16x2(large, q[n][b][i] & 0x7FFF7FFFu, q[n][b][i + 1] & 0x7FFF7FFFu);
+          least = __vimin3_s16x2(least, (q[n][b][i] | 0x80008000u) - 0x00010001u, (q[n][b][i + 1] | 0x80008000u) - 0x00010001u);
+        }
       }
+      uint32_t amax = max(large & 0xFFFFu, large >> 16);
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       // largest |q| into [2^14, 2^15): shift = 14 - floor(log2), at most 114
@@ -480,7 +498,10 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
           const __half2 h = __floats2half2_rn(bf16_lo(q[n][b][i]) * two, bf16_hi(q[n][b][i]) * two);
           q[n][b][i] = *reinterpret_cast<const uint32_t*>(&h);
         }
+      // values of 2^-16 and more there keep all their bits
+      const int low = min(static_cast<int>(least << 16) >> 16, static_cast<int>(least) >> 16) + 0x8001;
       const float back = a.scale * 1.4426950408889634f * __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+      held &= !real || ((low >> 7) + shift >= 127 - 16 && (a.scale == 0.0f || (fabsf(back) >= 0x1p-126f && fabsf(back) < kInf)));
 #pragma unroll
       for (int j = 0; j < 2; ++j) mult[n][j] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + j));
     }
@@ -503,46 +524,138 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
 
     // Largest of V's codes, see has_nan_code; or why else the keys have to be taken again with care (kHuge: values
     // of 2^56 and more may be among them, whose sum could leave the range of fp32).
-    uint32_t most = 0;
     constexpr uint32_t kCare = 0x07F007F0u, kHuge = 0x0EF00EF0u;
+    uint32_t most = held ? 0 : kCare;
     float raise = kRaise;
-    // Looks closer at a step that has value scales out of the usual range: groups of zeros (byte 0) are none of
-    // those, nor are rows of no key.
+    // For a walk with care: the power of two of the lane's own head in the q operand, of heads 2t and 2t + 1, and the levels.
+    int own_shift[NT], shift_of[NT][2], levels = 1;
+    auto q_at = [&](int n) { return a.q + a.q_stride * seq + static_cast<size_t>(h0 + 8 * n + g) * D + 8 * t; };
+    // Looks closer at a step that has scales out of the usual range: groups of zeros (byte 0) are none of
+    // those, nor are rows of no key.  A lane has one key's scales of K or of V.
     auto look_at_scales = [&](int tile, uint32_t have, uint32_t at) {
-      const int key = lane >> 1;
+      const int key = lane & 15, of_v = lane >> 4;
 #pragma unroll 1
       for (int i = 0; i < KT; ++i) {
         if (!((have >> i) & 1) || (tile + i) * 16 + key >= len) continue;
-        const uint32_t codes = at + i * kTile + (16 + key) * kRowBytes, scales = at + i * kTile + 32 * kRowBytes + (16 + key) * kGroups;
+        const uint32_t codes = at + i * kTile + lane * kRowBytes, scales = at + i * kTile + 32 * kRowBytes + lane * kGroups;
+        const uint32_t swizzle = 16 * (of_v ? attn_swizzle<D, kFmt, true>(key) : attn_swizzle<D, kFmt, false>(key));
 #pragma unroll 1
-        for (int b = (lane & 1) * (kGroups / 2), e = b + kGroups / 2; b < e; ++b) {
+        for (int b = 0; b < kGroups; ++b) {
           const uint32_t byte = lds_u8(scales + b);
           if (byte - 64u < 128u) continue;
           uint32_t any = byte;
           if (byte == 0) {
 #pragma unroll
             for (int u = 0; u < kRowBytes / kGroups; u += 16) {
-              const uint4 x = lds128(codes + ((b * (kRowBytes / kGroups) + u) ^ (16 * attn_swizzle<D, kFmt, true>(key))));
+              const uint4 x = lds128(codes + ((b * (kRowBytes / kGroups) + u) ^ swizzle));
               any |= (x.x | x.y | x.z | x.w) & (kFmt == kFmtE4M3 ? 0x7F7F7F7Fu : 0x77777777u);
             }
           }
-          if (any) most = max(most, byte >= 192 ? kHuge : kCare);
+          if (any) most = max(most, of_v && byte >= 192 ? kHuge : kCare);
         }
       }
     };
+    // Scores of a tile's keys key_g (the first two of a head pair's) and key_g + 8, without mult.
+    auto scores = [&](uint32_t at, float (&s)[NT][4]) {
+      uint32_t two[2][kGroups / 2];  // the two keys' scales, a bf16x2 per pair of groups
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t sa = at + 32 * kRowBytes + (key_g + 8 * h) * kGroups;
+        uint32_t w[(kGroups + 3) / 4];
+        if constexpr (kGroups == 2) {
+          asm volatile("ld.shared.u16 %0, [%1];" : "=r"(w[0]) : "r"(sa));
+          two[h][0] = e8m0x2_bf16x2(w[0]);
+        } else {
+          lds_words<kGroups / 4>(sa, w);
+#pragma unroll
+          for (int b = 0; b < kGroups; b += 4) e8m0x4_bf16x2(w[b / 4], two[h][b / 2], two[h][b / 2 + 1]);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kGroups; ++b) {
+        uint32_t f[2][4];  // [key][value pairs 8t + 2j]
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = key_g + 8 * h;
+          const int byte = b * (kRowBytes / kGroups) + 4 * kKw * t;
+          uint32_t w[kKw];
+          lds_words<kKw>(at + key * kRowBytes + (byte ^ (16 * attn_swizzle<D, kFmt, false>(key))), w);
+          if constexpr (kFmt == kFmtE4M3) {
+            e4m3x4_to_f16x2(w[0], f[h][0], f[h][1]);
+            e4m3x4_to_f16x2(w[1], f[h][2], f[h][3]);
+          } else {
+            e2m1x8_to_f16x2(w[0], f[h]);
+          }
+        }
+        const float s0 = b & 1 ? bf16_hi(two[0][b / 2]) : bf16_lo(two[0][b / 2]);
+        const float s1 = b & 1 ? bf16_hi(two[1][b / 2]) : bf16_lo(two[1][b / 2]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          mma_f16_16816(d, f[0][0], f[1][0], f[0][1], f[1][1], q[n][b][0], q[n][b][1]);
+          mma_f16_16816(d, f[0][2], f[1][2], f[0][3], f[1][3], q[n][b][2], q[n][b][3]);
+          s[n][0] = fmaf(d[0], s0, s[n][0]);
+          s[n][1] = fmaf(d[1], s0, s[n][1]);
+          s[n][2] = fmaf(d[2], s1, s[n][2]);
+          s[n][3] = fmaf(d[3], s1, s[n][3]);
+        }
+      }
+    };
+    // The same in powers of two, for any scale byte and query: levels of the query one after another, and the factors
+    // of each group's sum put together as exponents.
+    auto scores_with_care = [&](uint32_t at, float (&s)[NT][4]) {
+      int of_scale;
+      const float base = frexpf(a.scale, &of_scale) * 1.4426950408889634f;
+#pragma unroll 1
+      for (int level = 0; level < levels; ++level)
+#pragma unroll 1
+        for (int b = 0; b < kGroups; ++b) {
+          uint32_t f[2][4], byte[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int key = key_g + 8 * h;
+            byte[h] = lds_u8(at + 32 * kRowBytes + key * kGroups + b);
+            uint32_t w[kKw];
+            lds_words<kKw>(at + key * kRowBytes + ((b * (kRowBytes / kGroups) + 4 * kKw * t) ^ (16 * attn_swizzle<D, kFmt, false>(key))), w);
+            if constexpr (kFmt == kFmtE4M3) {
+              e4m3x4_to_f16x2(w[0], f[h][0], f[h][1]);
+              e4m3x4_to_f16x2(w[1], f[h][2], f[h][3]);
+            } else {
+              e2m1x8_to_f16x2(w[0], f[h]);
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint4 x4 = make_uint4(0, 0, 0, 0);
+            if (8 * n + g < nh) x4 = *reinterpret_cast<const uint4*>(q_at(n) + 32 * b);
+            uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              x[i] = q_of_level(x[i] & 0xFFFFu, own_shift[n], level) | q_of_level(x[i] >> 16, own_shift[n], level) << 16;
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma_f16_16816(d, f[0][0], f[1][0], f[0][1], f[1][1], x[0], x[1]);
+            mma_f16_16816(d, f[0][2], f[1][2], f[0][3], f[1][3], x[2], x[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int by = static_cast<int>(byte[j >> 1]) - 127 + of_scale - shift_of[n][j & 1] - 31 * level;
+              s[n][j] += byte[j >> 1] == 255 ? __uint_as_float(0x7FC00000u) : ldexpf(d[j] * base, by);
+            }
+          }
+        }
+    };
     // One step; `ragged`: the sequence ends inside it, or a page of it is missing; `careful`: see below.
     auto do_step = [&](int tile, uint32_t have, uint32_t at, auto ragged, auto careful) {
-      uint32_t usual = 0xFFFFFFFFu;  // see odd_scales; the 16 keys' value scales are dealt to the lanes
-      constexpr uint32_t kUsual = kGroups == 2 ? 0x80u : (kGroups == 4 ? 0x8080u : 0x80808080u);
+      uint32_t usual = 0xFFFFFFFFu;  // see odd_scales; a key's scales of K or V to each lane
+      constexpr uint32_t kUsual = kGroups == 2 ? 0x8080u : 0x80808080u;
       if constexpr (!decltype(careful)::value) {
 #pragma unroll
         for (int i = 0; i < KT; ++i) {
-          const uint32_t sa = at + i * kTile + 32 * kRowBytes + 16 * kGroups + lane * (kGroups / 2);
-          uint32_t w;
-          if constexpr (kGroups == 2) w = lds_u8(sa);
-          else if constexpr (kGroups == 4) asm volatile("ld.shared.u16 %0, [%1];" : "=r"(w) : "r"(sa));
-          else w = lds32(sa);
-          usual &= w ^ (w << 1);
+          const uint32_t sa = at + i * kTile + 32 * kRowBytes + lane * kGroups;
+          uint32_t w[2];
+          if constexpr (kGroups == 2) asm volatile("ld.shared.u16 %0, [%1];" : "=r"(w[0]) : "r"(sa));
+          else lds_words<kGroups / 4>(sa, w);
+          usual &= w[0] ^ (w[0] << 1);
+          if constexpr (kGroups == 8) usual &= w[1] ^ (w[1] << 1);
         }
       }
       // scores
@@ -551,55 +664,14 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
       for (int i = 0; i < KT; ++i) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.0f;
-        uint32_t two[2][kGroups / 2];  // the two keys' scales, a bf16x2 per pair of groups
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t sa = at + i * kTile + 32 * kRowBytes + (key_g + 8 * h) * kGroups;
-          uint32_t w[(kGroups + 3) / 4];
-          if constexpr (kGroups == 2) {
-            asm volatile("ld.shared.u16 %0, [%1];" : "=r"(w[0]) : "r"(sa));
-            two[h][0] = e8m0x2_bf16x2(w[0]);
-          } else {
-            lds_words<kGroups / 4>(sa, w);
-#pragma unroll
-            for (int b = 0; b < kGroups; b += 4) e8m0x4_bf16x2(w[b / 4], two[h][b / 2], two[h][b / 2 + 1]);
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < kGroups; ++b) {
-          uint32_t f[2][4];  // [key][value pairs 8t + 2j]
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int key = key_g + 8 * h;
-            const int byte = b * (kRowBytes / kGroups) + 4 * kKw * t;
-            uint32_t w[kKw];
-            lds_words<kKw>(at + i * kTile + key * kRowBytes + (byte ^ (16 * attn_swizzle<D, kFmt, false>(key))), w);
-            if constexpr (kFmt == kFmtE4M3) {
-              e4m3x4_to_f16x2(w[0], f[h][0], f[h][1]);
-              e4m3x4_to_f16x2(w[1], f[h][2], f[h][3]);
-            } else {
-              e2m1x8_to_f16x2(w[0], f[h]);
-            }
-          }
-          const float s0 = b & 1 ? bf16_hi(two[0][b / 2]) : bf16_lo(two[0][b / 2]);
-          const float s1 = b & 1 ? bf16_hi(two[1][b / 2]) : bf16_lo(two[1][b / 2]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma_f16_16816(d, f[0][0], f[1][0], f[0][1], f[1][1], q[n][b][0], q[n][b][1]);
-            mma_f16_16816(d, f[0][2], f[1][2], f[0][3], f[1][3], q[n][b][2], q[n][b][3]);
-            s[i][n][0] = fmaf(d[0], s0, s[i][n][0]);
-            s[i][n][1] = fmaf(d[1], s0, s[i][n][1]);
-            s[i][n][2] = fmaf(d[2], s1, s[i][n][2]);
-            s[i][n][3] = fmaf(d[3], s1, s[i][n][3]);
-          }
-        }
+        if constexpr (decltype(careful)::value) scores_with_care(at + i * kTile, s[i]);
+        else scores(at + i * kTile, s[i]);
         // in powers of two, those of no key at -inf
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            s[i][n][j] *= mult[n][j & 1];
+            if constexpr (!decltype(careful)::value) s[i][n][j] *= mult[n][j & 1];
             if constexpr (decltype(ragged)::value)
               if (!((have >> i) & 1) || (tile + i) * 16 + key_g + 8 * (j >> 1) >= len) s[i][n][j] = -kInf;
           }
@@ -734,13 +806,37 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
       cp_async_wait<0>();
     };
     walk(std::false_type{});
-    // A NaN code among the values, or a value scale out of the usual range: this warp's steps once more,
-    // with care for them.  The first walk only follows whether there was one (a branch for NaN codes in its loop cost
-    // 14 %, the largest code 6 %).
+    // A NaN code among the values, a scale out of the usual range, or a query that the operand does not hold:
+    // this warp's steps once more, with care for them.  The first walk only follows whether there was one (a branch
+    // for NaN codes in its loop cost 14 %, the largest code 6 %).
     if (__any_sync(0xffffffffu, has_nan_code(most))) {
       __syncwarp();  // all lanes have left the ring
       const bool huge = __any_sync(0xffffffffu, most >= kHuge);
       if (huge) raise = kRaise * 0x1p-40f;
+      int deepest = 0;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        uint32_t amax = 0, least = 0x7F80u;  // magnitudes other than zero
+        if (8 * n + g < nh)
+#pragma unroll 1
+          for (int d = 0; d < D; d += 32)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t mag = reinterpret_cast<const uint16_t*>(q_at(n))[d + i] & 0x7FFFu;
+              amax = max(amax, mag);
+              if (mag) least = min(least, mag);
+            }
+#pragma unroll
+        for (int x = 1; x < 4; x <<= 1) {
+          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, x));
+          least = min(least, __shfl_xor_sync(0xffffffffu, least, x));
+        }
+        own_shift[n] = 14 + 127 - max(static_cast<int>(amax >> 7), 27);
+        if (least < 0x7F80u) deepest = max(deepest, q_level(least, own_shift[n]));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) shift_of[n][j] = __shfl_sync(0xffffffffu, own_shift[n], 4 * (2 * t + j));
+      }
+      levels = 1 + __reduce_max_sync(0xffffffffu, deepest);
       clear();
       copy_tile = tile_first, copy_slot = 0;
       first_pages();

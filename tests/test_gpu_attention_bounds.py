@@ -141,3 +141,76 @@ def test_groups_of_zeros_among_values(mx, fmt, dim):
     out, lse = mx.paged_attention(q, cache, i32(table), i32([n, n]), return_lse=True)
     check(out, lse, q, cache, table, [n, n], dim ** -0.5)
     assert (out[0, :, dim // 2:] == 0).all() and (out[1, :, dim // 2:] > 0).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,heads,kv,step", [(64, 4, 2, 90), (64, 20, 2, 35), (128, 8, 1, 40), (128, 16, 1, 13), (256, 3, 1, 17), (256, 9, 1, 12)])
+@pytest.mark.parametrize("longest", [30, 3000])
+def test_small_query_values_count(mx, fmt, dim, heads, kv, step, longest):
+    """Query values 2^step smaller from group to group against keys as much larger: every group has the same share
+    of a score, so none may be rounded as a part of the largest."""
+    rng = np.random.default_rng(dim + step)
+    lengths = [longest, 17, longest // 2]
+    cache = random_cache(mx, rng, sum(-(-n // 64) for n in lengths) + 1, kv, dim, 64, fmt)
+    table = random_table(rng, cache, lengths)
+    groups = np.arange(dim // 32)
+    mid = (groups[-1] * step) // 2
+    q = bf16(rng, (3, heads, dim)).unflatten(2, (-1, 32))
+    q *= torch.from_numpy(np.exp2(mid - groups * float(step))).cuda()[:, None].bfloat16()
+    cache.k_scales.add_(torch.from_numpy(((groups * step - mid) % 256).astype(np.uint8)).cuda())
+    out, lse = mx.paged_attention(q.flatten(2), cache, i32(table), i32(lengths), return_lse=True)
+    check(out, lse, q.flatten(2), cache, table, lengths, dim ** -0.5)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,heads", [(64, 3), (128, 16), (256, 2)])
+def test_small_query_values_beside_zeros_of_keys(mx, fmt, dim, heads):
+    """Within one group: the key is zero where the query is large, so the small values alone make the score."""
+    rng = np.random.default_rng(dim)
+    lengths = [200, 70, 16, 16]
+    cache = random_cache(mx, rng, 12, 1, dim, 64, fmt)
+    table = random_table(rng, cache, lengths)
+    q = bf16(rng, (4, heads, dim))
+    for b, power in enumerate((30, 60, 100, 126)):
+        q[b, :, ::8] *= 2.0**power
+        q[b, :, 1::8] *= 2.0**-100  # and smaller ones yet
+    if fmt == "mxfp8":
+        cache.k_codes[..., ::8] = 0
+    else:
+        cache.k_codes[..., ::4] &= 0xF0
+    out, lse = mx.paged_attention(q, cache, i32(table), i32(lengths), return_lse=True)
+    check(out, lse, q, cache, table, lengths, dim ** -0.5)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,heads", [(64, 3), (128, 16), (256, 2)])
+@pytest.mark.parametrize("q_power,k_power,scale_power", [(-110, 110, 0), (110, -110, 0), (0, 100, -100), (100, 20, -120), (-60, -60, 120),
+                                                         (126, -117, -9), (-120, 0, 120), (60, 63, -123), (-120, 124, -4), (-100, 124, -24), (120, -118, -2)])
+def test_queries_and_keys_of_every_size(mx, fmt, dim, heads, q_power, k_power, scale_power):
+    """Ordinary scores from factors that no product of two of them need hold."""
+    rng = np.random.default_rng(dim)
+    lengths = [300, 20]
+    cache = random_cache(mx, rng, 8, 1, dim, 64, fmt, spread=1)
+    table = random_table(rng, cache, lengths)
+    cache.k_scales.add_(k_power % 256)
+    q = (bf16(rng, (2, heads, dim)).float() * 2.0**q_power).bfloat16()
+    scale = dim ** -0.5 * 2.0**scale_power
+    out, lse = mx.paged_attention(q, cache, i32(table), i32(lengths), scale=scale, return_lse=True)
+    check(out, lse, q, cache, table, lengths, scale)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_key_groups_of_zeros_and_heads_of_zeros(mx, fmt):
+    """A head padded with zeros, as the coder stores it (scale byte 0), and a query of zeros beside one that is not."""
+    rng = np.random.default_rng(2)
+    n = 150
+    cache = mx.new_kv_cache(3, 2, 128, 64, fmt)
+    k, v = bf16(rng, (n, 2, 128)), bf16(rng, (n, 2, 128))
+    k[:, :, 96:] = 0
+    k[40:50, 0, 32:64] = -0.0
+    mx.kv_cache_write(cache, k, v, i32(np.arange(n)))
+    q = bf16(rng, (1, 4, 128))
+    q[0, 1] = 0
+    table = np.array([[0, 1, 2]])
+    out, lse = mx.paged_attention(q, cache, i32(table), i32([n]), return_lse=True)
+    check(out, lse, q, cache, table, [n], 128 ** -0.5)
