@@ -71,14 +71,30 @@ const int* index_vector(PyObject* o, int64_t n, c10::Device dev, const char* wha
 }
 
 struct Cache {
-  const mxfp4_kv_cache* c;
+  mxfp4_kv_cache c;
   c10::Device dev;
 };
-// `address` of the C structure and the device's index, both from an MXKVCache.
-Cache cache_of(PyObject* address, PyObject* index) {
-  void* p = PyLong_AsVoidPtr(address);
+// From an MXKVCache: its four tensors, the address of the C structure that describes them and the device's index.
+// The memory is the tensors' own as they are now: they may have been given another storage since, or lost it.
+Cache cache_of(PyObject* native) {
+  if (!PyTuple_Check(native) || PyTuple_GET_SIZE(native) != 6) refuse("cache must be an MXKVCache");
+  const void* p = PyLong_AsVoidPtr(PyTuple_GET_ITEM(native, 4));
   if (!p && PyErr_Occurred()) throw python_error();
-  return {static_cast<const mxfp4_kv_cache*>(p), c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(integer(index, "device")))};
+  Cache r = {*static_cast<const mxfp4_kv_cache*>(p),
+             c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(integer(PyTuple_GET_ITEM(native, 5), "device")))};
+  uint8_t* at[4];
+  for (int i = 0; i < 4; ++i) {
+    const at::Tensor* t = tensor(PyTuple_GET_ITEM(native, i));
+    const int64_t width = i >= 2 ? r.c.head_dim / 32 : (r.c.format == MXFP4_KV_MXFP8 ? r.c.head_dim : r.c.head_dim / 2);
+    const int64_t rows = int64_t(r.c.num_pages) * r.c.num_kv_heads * r.c.page_size;
+    if (!t || t->scalar_type() != at::kByte || t->device() != r.dev || !t->is_contiguous() || t->dim() != 4 ||
+        t->size(0) != r.c.num_pages || t->size(1) != r.c.num_kv_heads || t->size(2) != r.c.page_size || t->size(3) != width ||
+        static_cast<int64_t>(t->storage().nbytes()) < t->storage_offset() + rows * width)
+      refuse("the cache's tensors are no longer those it was made of: type, shape, device or storage has changed");
+    at[i] = static_cast<uint8_t*>(t->data_ptr());
+  }
+  r.c.k_codes = at[0], r.c.v_codes = at[1], r.c.k_scales = at[2], r.c.v_scales = at[3];
+  return r;
 }
 
 // Uninitialised contiguous memory: at::empty without the dispatcher's walk (0.3 us less each).
@@ -166,32 +182,32 @@ ENTRY(qk_norm_rope, 10)
   END_HANDLE_TH_ERRORS
 }
 
-// qkv, num_heads, num_kv_heads, cos, sin, positions, q_weight, k_weight, eps, interleaved, cache, device, slots
-ENTRY(qk_norm_rope_cache, 13)
+// qkv, num_heads, num_kv_heads, cos, sin, positions, q_weight, k_weight, eps, interleaved, cache, slots
+ENTRY(qk_norm_rope_cache, 12)
   const int heads = integer(args[1], "num_heads"), kv_heads = integer(args[2], "num_kv_heads");
-  const Cache c = cache_of(args[10], args[11]);
-  if (kv_heads != c.c->num_kv_heads) refuse("num_kv_heads differs from the cache's");
-  int dim = c.c->head_dim;
+  const Cache c = cache_of(args[10]);
+  if (kv_heads != c.c.num_kv_heads) refuse("num_kv_heads differs from the cache's");
+  int dim = c.c.head_dim;
   const Rope r = rope_of(args[0], heads, kv_heads, dim, args + 3);
   const double eps = real(args[8]);
   const bool inter = truth(args[9]);
   if (r.qkv->device() != c.dev) refuse("qkv must be on the cache's GPU");
-  const int* slots = index_vector(args[12], r.tokens, c.dev, "slots");
+  const int* slots = index_vector(args[11], r.tokens, c.dev, "slots");
   const c10::DeviceGuard guard(c.dev);
   at::Tensor q = fresh({r.tokens, heads, dim}, at::kBFloat16, c.dev);
   check(g_entries.qk_norm_rope_cache(r.qkv->data_ptr(), r.stride, r.tokens, heads, r.cos, r.sin, r.rows, r.rot, inter,
-                                     r.positions, r.q_weight, r.k_weight, r.weight_dtype, eps, q.data_ptr(), c.c, slots,
+                                     r.positions, r.q_weight, r.k_weight, r.weight_dtype, eps, q.data_ptr(), &c.c, slots,
                                      stream_of(c.dev)),
         "mxfp4_qk_norm_rope_cache");
   return THPVariable_Wrap(std::move(q));
   END_HANDLE_TH_ERRORS
 }
 
-// cache, device, k, v, slots
-ENTRY(kv_cache_write, 5)
-  const Cache c = cache_of(args[0], args[1]);
-  const int64_t heads = c.c->num_kv_heads, dim = c.c->head_dim;
-  const at::Tensor* t[2] = {tensor(args[2]), tensor(args[3])};
+// cache, k, v, slots
+ENTRY(kv_cache_write, 4)
+  const Cache c = cache_of(args[0]);
+  const int64_t heads = c.c.num_kv_heads, dim = c.c.head_dim;
+  const at::Tensor* t[2] = {tensor(args[1]), tensor(args[2])};
   int64_t stride[2];
   for (int i = 0; i < 2; ++i) {
     if (!t[i] || t[i]->scalar_type() != at::kBFloat16 || t[i]->device() != c.dev || t[i]->dim() != 3 || t[i]->size(0) != t[0]->size(0) ||
@@ -200,25 +216,25 @@ ENTRY(kv_cache_write, 5)
     stride[i] = t[0]->size(0) > 1 ? t[i]->stride(0) : heads * dim;
   }
   const int tokens = static_cast<int>(as_int(t[0]->size(0), "tokens"));
-  const int* slots = index_vector(args[4], tokens, c.dev, "slots");
+  const int* slots = index_vector(args[3], tokens, c.dev, "slots");
   const c10::DeviceGuard guard(c.dev);
-  check(g_entries.write(c.c, t[0]->data_ptr(), stride[0], t[1]->data_ptr(), stride[1], slots, tokens, stream_of(c.dev)),
+  check(g_entries.write(&c.c, t[0]->data_ptr(), stride[0], t[1]->data_ptr(), stride[1], slots, tokens, stream_of(c.dev)),
         "mxfp4_kv_cache_write");
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
 
-// cache, device, slots
-ENTRY(kv_cache_read, 3)
-  const Cache c = cache_of(args[0], args[1]);
-  const at::Tensor* s = tensor(args[2]);
+// cache, slots
+ENTRY(kv_cache_read, 2)
+  const Cache c = cache_of(args[0]);
+  const at::Tensor* s = tensor(args[1]);
   if (!s || s->dim() != 1) refuse("slots must be a vector");
   const int tokens = static_cast<int>(as_int(s->size(0), "tokens"));
-  const int* slots = index_vector(args[2], tokens, c.dev, "slots");
+  const int* slots = index_vector(args[1], tokens, c.dev, "slots");
   const c10::DeviceGuard guard(c.dev);
-  at::Tensor k = fresh({tokens, c.c->num_kv_heads, c.c->head_dim}, at::kBFloat16, c.dev);
-  at::Tensor v = fresh({tokens, c.c->num_kv_heads, c.c->head_dim}, at::kBFloat16, c.dev);
-  check(g_entries.read(c.c, slots, tokens, k.data_ptr(), v.data_ptr(), stream_of(c.dev)), "mxfp4_kv_cache_read");
+  at::Tensor k = fresh({tokens, c.c.num_kv_heads, c.c.head_dim}, at::kBFloat16, c.dev);
+  at::Tensor v = fresh({tokens, c.c.num_kv_heads, c.c.head_dim}, at::kBFloat16, c.dev);
+  check(g_entries.read(&c.c, slots, tokens, k.data_ptr(), v.data_ptr(), stream_of(c.dev)), "mxfp4_kv_cache_read");
   PyObject *pk = THPVariable_Wrap(std::move(k)), *pv = THPVariable_Wrap(std::move(v));
   PyObject* both = pk && pv ? PyTuple_Pack(2, pk, pv) : nullptr;
   Py_XDECREF(pk);
@@ -227,39 +243,39 @@ ENTRY(kv_cache_read, 3)
   END_HANDLE_TH_ERRORS
 }
 
-// q, cache, device, page_table, lengths, scale, return_lse, out
-ENTRY(paged_attention, 8)
-  const Cache c = cache_of(args[1], args[2]);
-  const int64_t dim = c.c->head_dim;
-  const at::Tensor *q = tensor(args[0]), *table = tensor(args[3]);
+// q, cache, page_table, lengths, scale, return_lse, out
+ENTRY(paged_attention, 7)
+  const Cache c = cache_of(args[1]);
+  const int64_t dim = c.c.head_dim;
+  const at::Tensor *q = tensor(args[0]), *table = tensor(args[2]);
   if (!q || q->scalar_type() != at::kBFloat16 || q->device() != c.dev || q->dim() != 3 || q->size(2) != dim || q->stride(2) != 1)
     refuse("q must be bfloat16 [seqs, num_heads, head_dim] on the cache's GPU");
   const int seqs = static_cast<int>(as_int(q->size(0), "seqs")), heads = static_cast<int>(as_int(q->size(1), "num_heads"));
-  if (heads == 0 || heads % c.c->num_kv_heads || (heads > 1 && q->stride(1) != dim))
+  if (heads == 0 || heads % c.c.num_kv_heads || (heads > 1 && q->stride(1) != dim))
     refuse("q: num_heads must be a multiple of num_kv_heads, a sequence's heads contiguous");
   if (!table || table->scalar_type() != at::kInt || table->device() != c.dev || table->dim() != 2 || table->size(0) != seqs ||
       table->size(1) == 0 || (table->size(1) > 1 && table->stride(1) != 1))
     refuse("page_table must be int32 [seqs, max_pages] on the cache's GPU with contiguous rows");
   const int pages = static_cast<int>(as_int(table->size(1), "max_pages"));
-  const int* lengths = index_vector(args[4], seqs, c.dev, "lengths");
-  const double scale = args[5] == Py_None ? 1.0 / std::sqrt(static_cast<double>(dim)) : real(args[5]);
+  const int* lengths = index_vector(args[3], seqs, c.dev, "lengths");
+  const double scale = args[4] == Py_None ? 1.0 / std::sqrt(static_cast<double>(dim)) : real(args[4]);
   if (!std::isfinite(static_cast<float>(scale))) refuse("scale must be finite in fp32");
   const c10::DeviceGuard guard(c.dev);
   at::Tensor out, lse;
-  if (args[7] == Py_None) {
+  if (args[6] == Py_None) {
     out = fresh({seqs, heads, dim}, at::kBFloat16, c.dev);
   } else {
-    const at::Tensor* o = tensor(args[7]);
+    const at::Tensor* o = tensor(args[6]);
     if (!o || o->scalar_type() != at::kBFloat16 || o->device() != c.dev || o->sizes() != q->sizes() || !o->is_contiguous())
       refuse("out must be contiguous bfloat16 [seqs, num_heads, head_dim] on the cache's GPU");
     out = *o;
   }
-  const bool want_lse = truth(args[6]);
+  const bool want_lse = truth(args[5]);
   if (want_lse) lse = fresh({seqs, heads}, at::kFloat, c.dev);
-  const size_t bytes = g_entries.attention_bytes(c.c, seqs, heads, pages);
+  const size_t bytes = g_entries.attention_bytes(&c.c, seqs, heads, pages);
   at::Tensor workspace;
   if (bytes) workspace = fresh({static_cast<int64_t>(bytes)}, at::kByte, c.dev);
-  check(g_entries.attention(q->data_ptr(), seqs > 1 ? q->stride(0) : heads * dim, c.c, static_cast<const int*>(table->data_ptr()),
+  check(g_entries.attention(q->data_ptr(), seqs > 1 ? q->stride(0) : heads * dim, &c.c, static_cast<const int*>(table->data_ptr()),
                             seqs > 1 ? table->stride(0) : pages, pages, lengths, seqs, heads, static_cast<float>(scale), out.data_ptr(),
                             want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, bytes ? workspace.data_ptr() : nullptr, bytes,
                             stream_of(c.dev)),

@@ -51,12 +51,13 @@ class MXKVCache:
     (``format="mxfp8"``) or ``[..., head_dim // 2]`` pairs of E2M1 codes (``"mxfp4"``, even element in
     the low nibble); ``k_scales`` / ``v_scales``: uint8 ``[..., head_dim // 32]`` E8M0 bytes.  The
     tensors are contiguous and stay the caller's: the object only refers to them, always to the same
-    ones (its attributes are read-only).  head_dim 64, 128 or 256; page_size 16, 32, 64, 128 or 256.
+    ones (its attributes are read-only), and each call takes their memory as it is then: a tensor
+    that has been given other storage of the same form serves, another form is refused.  head_dim 64, 128 or 256; page_size 16, 32, 64, 128 or 256.
     :func:`new_kv_cache` allocates one.
     """
 
     __slots__ = ("k_codes", "v_codes", "k_scales", "v_scales", "format", "num_pages", "num_kv_heads", "page_size",
-                 "head_dim", "device", "_index", "_struct", "_address")
+                 "head_dim", "device", "_struct", "_native")
 
     def __init__(self, k_codes, v_codes, k_scales, v_scales, format: str = "mxfp8"):
         _check(format in KV_FORMATS, "format must be 'mxfp8' or 'mxfp4'")
@@ -73,8 +74,9 @@ class MXKVCache:
             _check(tuple(t.shape) == (pages, heads, size, dim // 32), "scales shape")
         struct = _lib.KVCache(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                               pages, heads, size, dim, KV_FORMATS[format])
+        native = (k_codes, v_codes, k_scales, v_scales, ctypes.addressof(struct), k_codes.get_device())
         for name, value in zip(self.__slots__, (k_codes, v_codes, k_scales, v_scales, format, pages, heads, size, dim,
-                                                k_codes.device, k_codes.get_device(), struct, ctypes.addressof(struct))):
+                                                k_codes.device, struct, native)):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value):
@@ -123,7 +125,7 @@ def qk_norm_rope_cache(qkv, num_heads: int, num_kv_heads: int, cos, sin, cache: 
     if not isinstance(cache, MXKVCache):
         raise RuntimeError("cache must be an MXKVCache")
     return (_native or _binding()).qk_norm_rope_cache(qkv, num_heads, num_kv_heads, cos, sin, positions, q_weight, k_weight, eps,
-                                                      interleaved, cache._address, cache._index, slots)
+                                                      interleaved, cache._native, slots)
 
 
 def kv_cache_write(cache: MXKVCache, k, v, slots) -> None:
@@ -133,7 +135,7 @@ def kv_cache_write(cache: MXKVCache, k, v, slots) -> None:
     ``quantize_mxfp4(..., rule="ocp")`` and :func:`quantize_act_mx8`."""
     if not isinstance(cache, MXKVCache):
         raise RuntimeError("cache must be an MXKVCache")
-    (_native or _binding()).kv_cache_write(cache._address, cache._index, k, v, slots)
+    (_native or _binding()).kv_cache_write(cache._native, k, v, slots)
 
 
 def kv_cache_read(cache: MXKVCache, slots):
@@ -141,7 +143,7 @@ def kv_cache_read(cache: MXKVCache, slots):
     head_dim]``; a negative slot reads zeros, the scale byte 255 NaN."""
     if not isinstance(cache, MXKVCache):
         raise RuntimeError("cache must be an MXKVCache")
-    return (_native or _binding()).kv_cache_read(cache._address, cache._index, slots)
+    return (_native or _binding()).kv_cache_read(cache._native, slots)
 
 
 def paged_attention(q, cache: MXKVCache, page_table, lengths, scale: float | None = None, return_lse: bool = False,
@@ -160,4 +162,4 @@ def paged_attention(q, cache: MXKVCache, page_table, lengths, scale: float | Non
     """
     if not isinstance(cache, MXKVCache):
         raise RuntimeError("cache must be an MXKVCache")
-    return (_native or _binding()).paged_attention(q, cache._address, cache._index, page_table, lengths, scale, return_lse, out)
+    return (_native or _binding()).paged_attention(q, cache._native, page_table, lengths, scale, return_lse, out)

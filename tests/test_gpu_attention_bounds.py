@@ -214,3 +214,45 @@ def test_key_groups_of_zeros_and_heads_of_zeros(mx, fmt):
     table = np.array([[0, 1, 2]])
     out, lse = mx.paged_attention(q, cache, i32(table), i32([n]), return_lse=True)
     check(out, lse, q, cache, table, [n], 128 ** -0.5)
+
+
+# ------------------------------------------------------------------------------- the cache's tensors
+def test_a_cache_follows_its_tensors_storage(mx):
+    """Each call takes the memory that the tensors have then, and refuses tensors of another form or without storage."""
+    rng = np.random.default_rng(3)
+    cache = random_cache(mx, rng, 6, 2, 64, 16, "mxfp8")
+    names = ("k_codes", "v_codes", "k_scales", "v_scales")
+    table, lengths, slots = i32([[1, 3, 5]]), i32([40]), i32([17, 18, 90])
+    q, k, qkv = bf16(rng, (1, 4, 64)), bf16(rng, (3, 2, 64)), bf16(rng, (3, 8 * 64))
+    want, rows = mx.paged_attention(q, cache, table, lengths), mx.kv_cache_read(cache, slots)
+    for name in names:  # moved elsewhere: the same bytes at other addresses, the old ones overwritten
+        t = getattr(cache, name)
+        old, moved = t.data, t.detach().clone()
+        t.data = moved
+        old.fill_(0)
+    assert torch.equal(mx.paged_attention(q, cache, table, lengths), want)
+    assert all(torch.equal(a, b) for a, b in zip(mx.kv_cache_read(cache, slots), rows))
+    mx.kv_cache_write(cache, k, k, slots)
+    assert (cache.k_codes[1, :, 1] != 0).any()  # slot 17
+
+    calls = [lambda: mx.paged_attention(q, cache, table, lengths), lambda: mx.kv_cache_read(cache, slots),
+             lambda: mx.kv_cache_write(cache, k, k, slots), lambda: mx.qk_norm_rope_cache(qkv, 4, 2, None, None, cache, slots)]
+    for name in names:
+        t = getattr(cache, name)
+        good = t.data
+        for other in (good.cpu(), good[:3], good[..., :1], good.to(torch.int32), good.transpose(0, 2),
+                      torch.empty((0,), dtype=torch.uint8, device="cuda")):
+            t.data = other
+            for call in calls:
+                with pytest.raises(RuntimeError, match="cache's tensors"):
+                    call()
+        t.data = good
+        storage, n = t.untyped_storage(), t.numel()
+        saved = t.clone()
+        storage.resize_(n - 1)
+        for call in calls:
+            with pytest.raises(RuntimeError, match="cache's tensors"):
+                call()
+        storage.resize_(n)
+        t.copy_(saved)
+    mx.paged_attention(q, cache, table, lengths)
