@@ -497,7 +497,8 @@ __device__ __forceinline__ void cp_async_wait() {
 // first), 2.0 -> 1.8 us for the smallest calls in a graph.
 //
 // Two tokens of one launch that name the same slot: the later one is stored (every block looks
-// through the slots behind its own; the caller keeps a launch to 4096 tokens).
+// through the slots behind its own; the caller keeps a launch to 4096 tokens).  One whose position is outside
+// the tables is not stored, and does not keep another from it.
 template <int LPR, int kFmt, bool kInter>
 __global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(const __grid_constant__ RowArgs a, int first) {
   constexpr int kRows = 32 / LPR;  // turned keys a warp works on at a time; 2 * kRows of other rows
@@ -610,7 +611,19 @@ __global__ void __launch_bounds__(kRowThreads, kRowBlocks) head_rows_kernel(cons
         for (int u = t + 1 + threadIdx.x; u < end; u += kRowThreads) later |= __ldg(a.slots + u) == slot;
       }
     }
-    if (__syncthreads_or(later)) slot = -1;
+    if (__syncthreads_or(later)) {
+      bool stored = true;  // whether one of them is: its position has to be in the tables
+      if (a.rot && a.positions) {
+        stored = false;
+        for (int u = t + 1 + threadIdx.x, end = first + gridDim.x; u < end; u += kRowThreads)
+          if (__ldg(a.slots + u) == slot) {
+            const int pu = __ldg(a.positions + u);
+            stored |= pu >= 0 && pu < a.table_rows;
+          }
+        stored = __syncthreads_or(stored);
+      }
+      if (stored) slot = -1;
+    }
   }
   if (q0 < a.q_heads) {
     LaneTurn16 turn;

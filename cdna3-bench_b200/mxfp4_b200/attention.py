@@ -119,7 +119,7 @@ def qk_norm_rope_cache(qkv, num_heads: int, num_kv_heads: int, cos, sin, cache: 
 
     ``slots`` int32 ``[tokens]``: token t goes to row ``slots[t] % page_size`` of page ``slots[t] //
     page_size``; a negative slot stores nothing (a batch's padding); of two tokens with one slot the
-    later is stored.  Keys are coded from the unrounded rotated value, values from ``qkv`` as they
+    later is stored (of those whose positions the tables have).  Keys are coded from the unrounded rotated value, values from ``qkv`` as they
     are.  ``cos`` and ``sin`` may be None (no rotation).  Returns q.
     """
     if not isinstance(cache, MXKVCache):

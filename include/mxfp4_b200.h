@@ -273,7 +273,8 @@ int mxfp4_qk_norm_rope(const void* qkv, long long row_stride, int tokens, int nu
 
 /* The same pass with the keys (normed, rotated, then coded without a rounding in between) and the
  * values written into `cache` (its num_kv_heads and head_dim) at slots[token]; a negative slot
- * stores nothing.  Of two tokens with the same slot the later one is stored.  The stored codes are
+ * stores nothing.  Of two tokens with the same slot the later one is stored (a token whose position is outside the
+ * tables is none of them).  The stored codes are
  * those of the key computed in 64 bits, so they do not depend on how a sum was ordered. */
 int mxfp4_qk_norm_rope_cache(const void* qkv, long long row_stride, int tokens, int num_heads, const float* cos,
                              const float* sin, int table_rows, int rot, int interleaved, const int* positions,

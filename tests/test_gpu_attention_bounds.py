@@ -256,3 +256,32 @@ def test_a_cache_follows_its_tensors_storage(mx):
         storage.resize_(n)
         t.copy_(saved)
     mx.paged_attention(q, cache, table, lengths)
+
+
+# ------------------------------------------------------------------------------------------- slots
+@pytest.mark.parametrize("tokens,later", [(2, 1), (7, 3), (200, 150), (200, 199), (4096, 4095), (5000, 4500)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_a_token_without_a_position_does_not_take_a_slot_from_another(mx, tokens, later, shift):
+    """Token 0 and a later one name a slot; the later one's position is outside the tables, so it is not stored: the
+    first one's rows are, whether one launch holds both or not.  A third token, in between, wins where it is good."""
+    rng = np.random.default_rng(tokens)
+    kv, dim, page = 2, 64, 16
+    x = bf16(rng, (tokens, 6 * dim))  # 2 heads of each kind
+    angle = np.arange(8)[:, None] * 10000.0 ** (-np.arange(0, dim, 2) / dim)
+    cos, sin = (torch.from_numpy(f(angle).astype(np.float32)).cuda() for f in (np.cos, np.sin))
+    for between in {0, later // 2}:
+        cache = mx.new_kv_cache(-(-tokens // page) + 1, kv, dim, page)
+        want = mx.new_kv_cache(cache.num_pages, kv, dim, page)
+        slots, pos = np.arange(tokens), rng.integers(0, 8, tokens)
+        slots[later] = slots[between] = slots[0]
+        pos[later] = 8 if tokens % 2 else -1
+        pad = i32(np.r_[np.full(shift, 3), slots])[shift:]
+        mx.qk_norm_rope_cache(x, 2, kv, cos, sin, cache, pad, positions=i32(pos))
+        assert mx.device_error() == 0x202
+        alone = slots.copy()
+        alone[later] = -1
+        alone[:between] = np.where(alone[:between] == slots[0], -1, alone[:between])
+        mx.qk_norm_rope_cache(x, 2, kv, cos, sin, want, i32(alone), positions=i32(np.maximum(pos, 0) % 8))
+        for a, b in zip((cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales), (want.k_codes, want.v_codes, want.k_scales, want.v_scales)):
+            assert torch.equal(a, b)
+        assert mx.device_error() == 0
