@@ -6,7 +6,8 @@ One nvcc invocation over csrc/mxfp4_b200.cu (a single translation unit that incl
 kernels); the static CUDA runtime keeps the library independent of torch's runtime copy.  Beside
 it the host compiler builds ``_attention.so`` from csrc/attention_binding.cpp, the Python binding of
 the attention operators against torch's C++ headers (it holds no kernels and finds the library's
-entries at run time).
+entries at run time).  The library comes first and needs nvcc alone; where torch, its headers, Python's or a
+host compiler are missing, the binding is left out, which says so.
 """
 
 from __future__ import annotations
@@ -47,11 +48,28 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def up_to_date(out: str = OUT, of=None) -> bool:
+def up_to_date(out: str, of=None) -> bool:
     if not os.path.exists(out):
         return False
     t = os.path.getmtime(out)
     return all(os.path.getmtime(s) <= t for s in of or sources())
+
+
+def binding_needs() -> list:
+    """What build_binding needs and this host does not have."""
+    missing = []
+    try:
+        import torch
+
+        if not os.path.exists(os.path.join(os.path.dirname(torch.__file__), "include", "ATen", "ATen.h")):
+            missing.append("torch's C++ headers")
+    except ImportError:
+        missing.append("torch")
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        missing.append("Python.h")
+    if not shutil.which(os.environ.get("CXX", "g++")):
+        missing.append("a host C++ compiler")
+    return missing
 
 
 def build_binding(force: bool = False) -> str:
@@ -77,9 +95,17 @@ def build_binding(force: bool = False) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    build_binding(force)
-    if not force and up_to_date():
-        return OUT
+    if force or not up_to_date(OUT):
+        build_library(verbose)
+    missing = binding_needs()
+    if missing:
+        sys.stderr.write(f"_attention.so is not built, without {', '.join(missing)}: the attention operators need it in Python\n")
+    else:
+        build_binding(force)
+    return OUT
+
+
+def build_library(verbose: bool = False) -> str:
     cmd = [nvcc(), *NVCC_FLAGS, "-o", OUT + ".tmp", os.path.join(CSRC, "mxfp4_b200.cu")]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
