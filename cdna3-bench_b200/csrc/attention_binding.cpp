@@ -314,4 +314,12 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_attention", nullptr, -1, g_meth
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__attention() { return PyModule_Create(&g_module); }
+// MXFP4_BUILT_FOR: the torch and the Python compiled against; build.py looks for it in the file.
+PyMODINIT_FUNC PyInit__attention() {
+  PyObject* m = PyModule_Create(&g_module);
+  if (m && PyModule_AddStringConstant(m, "built_for", MXFP4_BUILT_FOR) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -16,10 +16,11 @@ word (:func:`mxfp4_b200.device_error`: 0x201 slot, 0x202 position, 0x203 page, 0
 from __future__ import annotations
 
 import ctypes
+import os
 
 import torch
 
-from . import _lib
+from . import _lib, build
 from .kernels import _check, _require_cuda
 
 KV_FORMATS = {"mxfp8": _lib.KV_MXFP8, "mxfp4": _lib.KV_MXFP4}
@@ -34,6 +35,8 @@ def _binding():
     bound to the library that :mod:`mxfp4_b200._lib` loads.  As there, no fallback."""
     global _native
     if _native is None:
+        if os.path.exists(build.BINDING_OUT) and not build.binding_fits():
+            raise RuntimeError("_attention.so was built for another torch or Python: build it with `python -m mxfp4_b200.build`")
         try:
             from . import _attention
         except ImportError as e:

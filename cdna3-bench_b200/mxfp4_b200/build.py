@@ -72,16 +72,29 @@ def binding_needs() -> list:
     return missing
 
 
+def built_for() -> str:
+    """The torch and the Python that run here: _attention.so holds this text of those it was compiled against."""
+    import torch
+
+    return f"_attention.so for torch {torch.__version__}, C++ ABI {int(torch.compiled_with_cxx11_abi())}, {sysconfig.get_config_var('SOABI')}"
+
+
+def binding_fits() -> bool:
+    """Whether the _attention.so that is there was compiled against the torch and the Python that run here."""
+    with open(BINDING_OUT, "rb") as f:
+        return built_for().encode() + b"\0" in f.read()
+
+
 def build_binding(force: bool = False) -> str:
     """_attention.so; torch's own libraries are already loaded when it is imported."""
-    if not force and up_to_date(BINDING_OUT, (BINDING, os.path.join(INCLUDE, "mxfp4_b200.h"))):
+    if not force and up_to_date(BINDING_OUT, (BINDING, os.path.join(INCLUDE, "mxfp4_b200.h"))) and binding_fits():
         return BINDING_OUT
     import torch
 
     home = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DMXFP4_BUILT_FOR="{built_for()}"',
            "-isystem", os.path.join(home, "include"), "-isystem", os.path.join(home, "include", "torch", "csrc", "api", "include"),
            "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
            "-o", BINDING_OUT + ".tmp", BINDING,

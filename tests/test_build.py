@@ -20,7 +20,7 @@ def ran(monkeypatch, tmp_path):
         commands.append(what)
         if codes.get(what, 0) == 0:
             with open(cmd[cmd.index("-o") + 1], "wb") as f:
-                f.write(" ".join(cmd).encode())
+                f.write(" ".join(cmd).encode().replace(b'"', b"\0"))
         return subprocess.CompletedProcess(cmd, codes.get(what, 0), "", "")
 
     monkeypatch.setattr(build.subprocess, "run", run)
@@ -54,3 +54,32 @@ def test_a_failing_host_compiler_is_an_error_after_the_library(ran):
     with pytest.raises(RuntimeError, match="_attention.so"):
         build.build()
     assert os.path.exists(build.OUT) and commands == ["library", "binding"]
+
+
+def test_a_binding_for_another_torch_or_python_is_built_again(ran, monkeypatch):
+    commands, _ = ran
+    build.build()
+    build.build()
+    assert commands == ["library", "binding"]
+    monkeypatch.setattr(build.sysconfig, "get_config_var", lambda name: "cpython-399-x86_64-linux-gnu")
+    build.build()
+    assert commands == ["library", "binding", "binding"]
+    import torch
+
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + "1")
+    build.build()
+    assert commands == ["library", "binding", "binding", "binding"]
+
+
+def test_a_binding_for_another_torch_is_refused(monkeypatch):
+    """Before it is loaded: its view of a tensor is another one."""
+    import torch
+
+    from mxfp4_b200 import attention
+
+    assert build.binding_fits()
+    monkeypatch.setattr(attention, "_native", None)
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + "1")
+    with pytest.raises(RuntimeError, match="another torch or Python"):
+        attention._binding()
+    assert attention._native is None
