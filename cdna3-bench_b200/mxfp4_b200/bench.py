@@ -134,45 +134,50 @@ def bench_quantize(shapes, n_iter: int = 20, rule: str = "ocp") -> list[dict]:
     return out
 
 
-def attention_calls(seqs: int, heads: int, kv_heads: int, dim: int, length: int, format: str, copies: int = 2) -> dict:
-    """name -> (call(i), bytes each input read and each output written once): norm, rotation and cache write of a
-    prompt of `length` tokens, the read-back of its rows, and one token's attention for `seqs` sequences of
-    `length` keys, over `copies` copies of the inputs (i picks one)."""
+ATTENTION_OPS = ("norm_rope_cache", "read", "attention")
+
+
+def attention_call(op: str, seqs: int, heads: int, kv_heads: int, dim: int, length: int, format: str, copies: int = 2):
+    """(call(i), bytes each input read and each output written once) of norm, rotation and cache write of a
+    prompt of `length` tokens, of the read-back of its rows, or of one token's attention for `seqs` sequences of
+    `length` keys, over `copies` copies of the inputs (i picks one).  Makes the inputs of that one alone."""
     dev = torch.device("cuda:0")
     page = 64
-    pages = -(-length // page)
+    pages = -(-length // page) * (seqs if op == "attention" else 1)
     gen = torch.Generator(device=dev).manual_seed(0)
+    caches = [at.new_kv_cache(pages, kv_heads, dim, page, format, dev) for _ in range(copies)]
+    row = 2 * kv_heads * (dim // (1 if format == "mxfp8" else 2) + dim // 32)
+    if op != "norm_rope_cache":
+        for c in caches:  # values to read
+            for t in (c.k_codes, c.v_codes):
+                t.random_(0, 100, generator=gen)
+            for t in (c.k_scales, c.v_scales):
+                t.random_(117, 121, generator=gen)
+    if op == "attention":
+        q = torch.randn(seqs, heads, dim, generator=gen, device=dev, dtype=torch.bfloat16)
+        lens = torch.full((seqs,), length, dtype=torch.int32, device=dev)
+        table = torch.randperm(pages, generator=gen, device=dev).to(torch.int32).view(seqs, -1)
+        return lambda i: at.paged_attention(q, caches[i], table, lens), seqs * (length * row + 4 * heads * dim)
+    slots = torch.arange(length, dtype=torch.int32, device=dev)
+    if op == "read":
+        return lambda i: at.kv_cache_read(caches[i], slots), length * (row + 4 * kv_heads * dim)
     angle = torch.arange(length, device=dev)[:, None] * 10000.0 ** (-torch.arange(0, dim, 2, device=dev) / dim)
     cos, sin = angle.cos().float(), angle.sin().float()
-    slots = torch.arange(length, dtype=torch.int32, device=dev)
     w = torch.ones(dim, dtype=torch.bfloat16, device=dev)
-    qkv = [torch.randn(length, (heads + 2 * kv_heads) * dim, generator=gen, device=dev).bfloat16() for _ in range(copies)]
-    q = torch.randn(seqs, heads, dim, generator=gen, device=dev).bfloat16()
-    lens = torch.full((seqs,), length, dtype=torch.int32, device=dev)
-    table = torch.randperm(seqs * pages, generator=gen, device=dev).to(torch.int32).view(seqs, pages)
-    caches = [at.new_kv_cache(seqs * pages, kv_heads, dim, page, format, dev) for _ in range(copies)]
-    for c in caches:  # values to read
-        for t in (c.k_codes, c.v_codes):
-            t.random_(0, 100, generator=gen)
-        for t in (c.k_scales, c.v_scales):
-            t.random_(117, 121, generator=gen)
-    row = 2 * kv_heads * (dim // (1 if format == "mxfp8" else 2) + dim // 32)
-    return {
-        "norm_rope_cache": (lambda i: at.qk_norm_rope_cache(qkv[i], heads, kv_heads, cos, sin, caches[i], slots, q_weight=w, k_weight=w),
-                            length * (heads * dim * 4 + 2 * kv_heads * dim * 2 + row + dim * 4)),
-        "read": (lambda i: at.kv_cache_read(caches[i], slots), length * (row + 4 * kv_heads * dim)),
-        "attention": (lambda i: at.paged_attention(q, caches[i], table, lens), seqs * (length * row + 4 * heads * dim)),
-    }
+    qkv = [torch.randn(length, (heads + 2 * kv_heads) * dim, generator=gen, device=dev, dtype=torch.bfloat16) for _ in range(copies)]
+    return (lambda i: at.qk_norm_rope_cache(qkv[i], heads, kv_heads, cos, sin, caches[i], slots, q_weight=w, k_weight=w),
+            length * (heads * dim * 4 + 2 * kv_heads * dim * 2 + row + dim * 4))
 
 
 def bench_attention(specs, n_iter: int = 30) -> list[dict]:
-    """The calls of :func:`attention_calls` in both cache formats, from a CUDA graph of `n_iter` of each."""
+    """The calls of :func:`attention_call` in both cache formats, from a CUDA graph of `n_iter` of each."""
     hbm = cm.load_peaks().hbm_gbs
     out = []
     for spec in specs:
         seqs, heads, kv_heads, dim, length = spec
         for fmt in at.KV_FORMATS:
-            for name, (fn, nbytes) in attention_calls(*spec, fmt).items():
+            for name in ATTENTION_OPS:
+                fn, nbytes = attention_call(name, *spec, fmt)
                 for i in range(2):
                     fn(i)
                 torch.cuda.synchronize()
@@ -193,7 +198,7 @@ def bench_attention(specs, n_iter: int = 30) -> list[dict]:
                 log.info("%s %s seqs=%d heads=%d/%d dim=%d length=%d: %.1f us %.0f GB/s (HBM copy peak %.0f)", name, fmt, seqs, heads,
                          kv_heads, dim, length, us, rec["gbs"], hbm)
                 out.append(rec)
-                del graph
+                del graph, fn
     return out
 
 

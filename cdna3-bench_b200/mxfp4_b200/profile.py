@@ -2,8 +2,8 @@
 
     # run one entry point `--iters` times (wrap the command in ncu)
     python -m mxfp4_b200.profile one --path tc --M 4608 --N 9216 --K 3072
-    # the same for an attention operator
-    python -m mxfp4_b200.profile attention --op attention --format mxfp8 --seqs 2 --length 131072
+    # the same for an attention operator (inputs past the 126 MB L2, and no more than a capture can keep)
+    python -m mxfp4_b200.profile attention --op attention --format mxfp8 --seqs 2 --length 65536
     # summarise a launch list (ncu --metrics gpu__time_duration.sum --clock-control none --csv --log-file L.csv)
     python -m mxfp4_b200.profile launches L.csv
     # summarise a capture (ncu -i R.ncu-rep --page raw --csv > R.csv)
@@ -149,14 +149,14 @@ def run_one(path: str, M: int, N: int, K: int, iters: int, seed: int) -> None:
 
 
 def run_attention(op: str, fmt: str, spec, iters: int) -> None:
-    """`iters` calls of one attention operator on seeded inputs (bench.attention_calls)."""
+    """`iters` calls of one attention operator on seeded inputs (bench.attention_call), one copy of them."""
     import torch
 
     from . import bench
 
-    call, nbytes = bench.attention_calls(*spec, fmt)[op]
-    for i in range(iters):
-        call(i & 1)
+    call, nbytes = bench.attention_call(op, *spec, fmt, copies=1)
+    for _ in range(iters):
+        call(0)
     torch.cuda.synchronize()
     print(f"{op} {fmt} seqs,heads,kv_heads,dim,length={','.join(map(str, spec))} iters={iters} bytes={nbytes}")
 
