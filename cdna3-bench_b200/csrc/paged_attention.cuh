@@ -29,15 +29,19 @@
 //           2^-36 and values 2^-20 below the largest: not taken.)
 //           P^T is two bf16 operands whose sum holds 16 bits of each weight, so the output is rounded once.
 //           The transposition between S^T's accumulators and P^T's operands is one movmatrix each per 8 keys.
-// What bounds it, measured: E4M3 D = 128, 8 heads to a kv head, 2 x 131072 keys: 94 % of the HBM copy
-// rate in steady state (89.9 us for 554 MB); 387 instructions per tile, of them 190 for V.  E2M1 is
-// bound by issue: 400 instructions per tile for half the bytes, 67 % of the issue slots, 56 % of the
-// copy rate (78.0 us); with 1, 2, 3, 4 tiles to a step 83, 78, 76, 75 us there but 80, 76, 82, 90 on 256 x 1000
-// keys; five blocks of 96 registers 89; the left shifts of its decode as multiplications by a number the
-// compiler does not know 77, and as much slower elsewhere.  D = 64: 74 % (E4M3), D = 256: 89 % (E4M3)
-// and 62 % (E2M1, 4 heads to a kv head).  Two tiles to a step against one: 91 -> 84 us on 2 x
-// ~115k keys; three resident blocks of 167 registers against four of 127: 91 -> 87 us there.  Loads
-// straight into registers (no ring): 111 us there, 12 warps cannot both hold the bytes and compute.
+// What bounds it, measured: E4M3 D = 128, 8 heads to a kv head, 2 x 131072 keys: 102 us for 554 MB, 82 % of the
+// HBM copy rate; E2M1 88 us, 50 %.  452 and 460 instructions per tile (2 x 65536 keys, starts and ends
+// included), 54 and 63 % of the issue slots, ALU pipe 57 and 54 %, tensor pipe 23 and 26 %: the issue slots, and bursts
+// of products that wait for the tensor pipe.  D = 64: 57 % (E4M3), D = 256: 70 % (E4M3) and 48 % (E2M1, 4 heads to
+// a kv head).  Of that the second product of the weights is 5 % (E2M1 10 %, 16 heads to a kv head 16 to 18 %), the
+// look for NaN codes 6 % (E4M3), for scales out of the usual range 1 to 3 %.
+// One tile to a step against two, E2M1: 94 us, and 92 against 87 on 256 x 1000 keys; four resident blocks
+// of 127 registers against three of 168, E4M3: 109 us against 92 on 2 x ~115k keys.
+// Measured with one product of the weights and without those looks, as are the comparisons of forms below and at
+// attn_plan: three and four tiles to a step 76 and 75 us against 78 for E2M1 there but 82 and 90 against 76 on 256 x
+// 1000 keys; five blocks of 96 registers 89; the left shifts of its decode as multiplications by a number the
+// compiler does not know 77, and as much slower elsewhere; E4M3 loads straight into registers (no ring) 111
+// against 87 us on 2 x ~115k keys, 12 warps cannot both hold the bytes and compute.
 //
 // A head's keys are cut into units of kAttnWarps steps, and the heads into pieces of at most `share`
 // units, share so that there are about as many pieces as blocks are resident: one block to a piece,
@@ -64,11 +68,11 @@ namespace mxb {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = 32 * kAttnWarps;
-// Pieces per resident block, where the heads are many: 1, 2, 3, 4 measured 66, 62, 60, 64 us on 32 x 4096 keys
-// (E4M3, 8 kv heads), 44, 42, 43, 45 us on 64 ragged sequences (E2M1).
+// Pieces per resident block, where the heads are many: 1, 2, 3, 4 measured 65, 61, 65, 69 us on 32 x 4096 keys
+// (E4M3, 8 kv heads), 49, 48, 49, 51 us on 64 ragged sequences (E2M1).
 constexpr int kAttnPieces = 2;
-// Units to a block of a cluster, at most: 4, 8, 16, 32 measured 64, 48, 48, 48 us on 256 sequences of up to
-// 1000 keys, 26, 26, 26, 41 us on 16 of up to 8192.
+// Units to a block of a cluster, at most: 4, 8, 16, 32 measured 89, 57, 57, 57 us on 256 sequences of up to
+// 1000 keys, 30, 30, 30, 49 us on 16 of up to 8192 (E4M3).
 constexpr int kAttnClusterSteps = 16;
 
 // Tiles of 16 keys a warp takes in one step; steps in its ring; blocks resident per SM (the kernel's
@@ -76,7 +80,9 @@ constexpr int kAttnClusterSteps = 16;
 __host__ __device__ constexpr int attn_tiles(int dim, int fmt) { return dim == 256 && fmt == kFmtE4M3 ? 1 : 2; }
 __host__ __device__ constexpr int attn_ring(int dim, int fmt) { return (dim == 256 && fmt == kFmtE4M3) || dim == 64 ? 3 : 2; }
 __host__ __device__ constexpr int attn_resident(int dim, int fmt, int nt) {
-  // 16 heads to a kv head, 2 x 131072 keys: 104 us (E4M3) and 96 (E2M1) with two blocks, 118 and 104 with three
+  // 16 heads to a kv head, D = 128, two blocks against three: E2M1 116 and 127 us on 2 x 131072 keys, 82 and 81 on 32 x
+  // 4096, 46 and 42 on 64 ragged, 10.5 and 13.3 on 8 x 1000 (three spill); E4M3 129 us with two on 2 x 131072, 104 and
+  // 118 with one product of the weights
   if (nt == 2) return dim == 128 ? 2 : 3;
   return dim == 256 ? 2 : (dim == 128 && fmt == kFmtE4M3 ? 3 : 4);
 }

@@ -157,7 +157,7 @@ def paged_attention(q, cache: MXKVCache, page_table, lengths, scale: float | Non
     the cache's num_kv_heads: query head h reads kv head ``h // (num_heads // num_kv_heads)``.
     ``page_table`` int32 ``[seqs, max_pages]`` (rows apart by max_pages or more): key j of sequence s is row ``j %
     page_size`` of page ``page_table[s, j // page_size]``, j < ``lengths[s]`` (int32); entries past the last
-    page a sequence needs are not read.  A length of zero gives a row of zeros.  ``scale`` defaults to
+    page a sequence needs may hold anything.  A length of zero gives a row of zeros.  ``scale`` defaults to
     ``head_dim ** -0.5``.  Returns bf16 ``[seqs, num_heads, head_dim]`` (``out`` if given), with
     ``return_lse`` also fp32 ``[seqs, num_heads]``: the natural log of the sum of exp(scale * q . k), -inf
     for an empty sequence.  ``out`` may be ``q`` itself, and must not overlap it otherwise.  The same call

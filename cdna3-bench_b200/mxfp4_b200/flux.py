@@ -13,8 +13,9 @@ MLP down (3072 x 12288).  :class:`FluxChain` runs them chained as the block uses
 with bf16 activations between the steps (each GEMM writes bf16, accumulates fp32) and torch
 element-wise ops for the residuals and the GELU.  Given a :class:`QKTurn`, the chain also norms and
 rotates the query and key heads of qkv as the block does before its attention (24 heads of 128,
-interleaved pairs; :func:`mxfp4_b200.qk_norm_rope`), and a is the turned query.  Every op writes into buffers allocated once,
-so one forward can be captured in a CUDA graph and replayed.  :func:`reference_rows` is the same
+interleaved pairs; :func:`mxfp4_b200.qk_norm_rope`), and a is the turned query: the turned heads
+come in new tensors, and the query is copied.  Every other op writes into buffers allocated once.
+One forward can be captured in a CUDA graph and replayed.  :func:`reference_rows` is the same
 sequence in fp32 on the CPU for a subset of rows (the chain is row-wise, so any row's output
 depends on that row's input only): the parity check of the chain.
 """

@@ -296,7 +296,7 @@ int mxfp4_kv_cache_read(const mxfp4_kv_cache* cache, const int* slots, int token
  * those mxfp4_kv_cache_read returns before its rounding to bf16 (scores past the range of fp32 count as
  * infinite).  lse (NULL: not wanted) fp32 [seqs][num_heads] is the natural log of the sum of
  * exp(scale * q . k).  A length of zero or less gives zeros and -inf.  Page-table entries past a
- * sequence's last page are not read.
+ * sequence's last page may hold anything.
  * q bf16 [seqs] rows of num_heads * head_dim, q_stride elements apart (a multiple of 8); out bf16
  * [seqs][num_heads][head_dim]; page_table rows page_stride ints apart.  Results do not depend on
  * timing: the same call gives the same bits.
