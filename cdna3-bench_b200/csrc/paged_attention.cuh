@@ -363,6 +363,16 @@ __device__ __forceinline__ void v_pairs(const uint32_t* a, const uint32_t* b, ui
 // Whether v_pairs met a NaN code, all ones: moved into bf16 it would be 480, 0x07F0, the most there can be.
 __device__ __forceinline__ bool has_nan_code(uint32_t most) { return ((most + 0x00100010u) & 0x08000800u) != 0; }
 
+// A part of a head (a warp's, a block's) is a reference m, the sum l of p and the sums o of p v.  Where values of 2^56
+// and more are among them, o is kept in units of 1 / kHugeUnit, so that it stays in the range of fp32, and l
+// negative to say so.  Parts are joined in small units if one of them is (`any`).
+constexpr float kHugeUnit = 0x1p-40f;
+__device__ __forceinline__ float part_factor(float f, float l, bool any) { return any && !(l < 0.0f) ? f * kHugeUnit : f; }
+__device__ __forceinline__ uint2 attn_output(const float4& o, float r, bool any) {
+  const float up = any ? 1.0f / kHugeUnit : 1.0f;
+  return make_uint2(pack_bf16x2(o.x * r * up, o.y * r * up), pack_bf16x2(o.z * r * up, o.w * r * up));
+}
+
 // Exponent of a finite bf16 that is not zero: |x| is in [2^e, 2^(e + 1)).
 __device__ __forceinline__ int bf16_exponent(uint32_t mag) { return mag >= 0x80u ? static_cast<int>(mag >> 7) - 127 : -102 - __clz(mag); }
 // The level of a query value, scaled by 2^shift so that the head's largest is in [2^14, 2^15).
@@ -533,6 +543,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
     constexpr uint32_t kCare = 0x07F007F0u, kHuge = 0x0EF00EF0u;
     uint32_t most = held ? 0 : kCare;
     float raise = kRaise;
+    bool huge = false;
     // For a walk with care: the power of two of the lane's own head in the q operand, of heads 2t and 2t + 1, and the levels.
     int own_shift[NT], shift_of[NT][2], levels = 1;
     auto q_at = [&](int n) { return a.q + a.q_stride * seq + static_cast<size_t>(h0 + 8 * n + g) * D + 8 * t; };
@@ -557,7 +568,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
               any |= (x.x | x.y | x.z | x.w) & (kFmt == kFmtE4M3 ? 0x7F7F7F7Fu : 0x77777777u);
             }
           }
-          if (any) most = max(most, of_v && byte >= 192 ? kHuge : kCare);
+          if (any) most = max(most, of_v && byte >= 192 && byte != 255 ? kHuge : kCare);
         }
       }
     };
@@ -817,8 +828,8 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
     // for NaN codes in its loop cost 14 %, the largest code 6 %).
     if (__any_sync(0xffffffffu, has_nan_code(most))) {
       __syncwarp();  // all lanes have left the ring
-      const bool huge = __any_sync(0xffffffffu, most >= kHuge);
-      if (huge) raise = kRaise * 0x1p-40f;
+      huge = __any_sync(0xffffffffu, most >= kHuge);
+      if (huge) raise = kRaise * kHugeUnit;
       int deepest = 0;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -849,10 +860,6 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
 #pragma unroll 1
       for (int i = 0; i < kRing - 1; ++i) copy_next();
       walk(std::true_type{});
-      if (huge) {  // the sums are 2^-40 of what they stand for, as if the reference were 40 more
-#pragma unroll
-        for (int n = 0; n < NT; ++n) m[n][0] += 40.0f, m[n][1] += 40.0f;
-      }
     }
     // Not earlier: the blocks of a call after this one would fill up the SMs that are busy already.
     griddep_launch_dependents();
@@ -868,7 +875,7 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int h = 8 * n + 2 * t + j;
-        if (g == 0) sm_m[warp * kHeads + h] = m[n][j], sm_l[warp * kHeads + h] = l;
+        if (g == 0) sm_m[warp * kHeads + h] = m[n][j], sm_l[warp * kHeads + h] = huge ? l * (-1.0f / kHugeUnit) : l;
         float* dst = sm + (warp * kHeads + h) * kStride + g * (D / 8);
 #pragma unroll
         for (int c = 0; c < D / 16; ++c)
@@ -885,30 +892,32 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
 #pragma unroll
       for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, sm_m[w * kHeads + h]);
       const float base = top == -kInf ? 0.0f : top;
+      bool any = false;  // a part of small unit
+#pragma unroll
+      for (int w = 0; w < kAttnWarps; ++w) any |= sm_l[w * kHeads + h] < 0.0f;
       float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       float l = 0.0f;
 #pragma unroll
       for (int w = 0; w < kAttnWarps; ++w) {
         const float f = exp2_approx(sm_m[w * kHeads + h] - base);
         const float4 x4 = *reinterpret_cast<const float4*>(sm + (w * kHeads + h) * kStride + d);
-        l = fmaf(sm_l[w * kHeads + h], f, l);
-        o.x = fmaf(x4.x, f, o.x), o.y = fmaf(x4.y, f, o.y), o.z = fmaf(x4.z, f, o.z), o.w = fmaf(x4.w, f, o.w);
+        const float lw = sm_l[w * kHeads + h], fo = part_factor(f, lw, any);
+        l = fmaf(fabsf(lw), f, l);
+        o.x = fmaf(x4.x, fo, o.x), o.y = fmaf(x4.y, fo, o.y), o.z = fmaf(x4.z, fo, o.z), o.w = fmaf(x4.w, fo, o.w);
       }
       l *= 1.0f / kRaise;
       if (whole) {
         const float r = l == 0.0f ? 0.0f : 1.0f / l;  // no key in reach (bad pages): zeros
         const size_t at = static_cast<size_t>(seq) * a.q_heads + h0 + h;
-        uint2 o2;
-        o2.x = pack_bf16x2(o.x * r, o.y * r), o2.y = pack_bf16x2(o.z * r, o.w * r);
-        *reinterpret_cast<uint2*>(a.out + at * D + d) = o2;
+        *reinterpret_cast<uint2*>(a.out + at * D + d) = attn_output(o, r, any);
         if (a.lse && d == 0) a.lse[at] = l == 0.0f ? -kInf : (top + log2f(l)) * 0.6931471805599453f;
       } else if (a.cluster) {
         // over the first warp's part, which no other thread reads here
         *reinterpret_cast<float4*>(sm + h * kStride + d) = o;
-        if (d == 0) sm_joined[h] = top, sm_joined[kHeads + h] = l;
+        if (d == 0) sm_joined[h] = top, sm_joined[kHeads + h] = any ? -l : l;
       } else {
         *reinterpret_cast<float4*>(part + h * D + d) = o;
-        if (d == 0) part[kHeads * D + 2 * h] = top, part[kHeads * D + 2 * h + 1] = l;
+        if (d == 0) part[kHeads * D + 2 * h] = top, part[kHeads * D + 2 * h + 1] = any ? -l : l;
       }
     }
     if (a.cluster > 1) {  // every block of the cluster gets here: none returns before
@@ -929,19 +938,21 @@ __global__ void __launch_bounds__(kAttnThreads, attn_resident(D, kFmt, NT)) attn
 #pragma unroll
         for (int c = 0; c < 8; ++c) top = fmaxf(top, m_of[c]);
         const float base = top == -kInf ? 0.0f : top;
-        float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
+        bool any = false;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) any |= l_of[c] < 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          const float f = exp2_approx(m_of[c] - base);
-          l = fmaf(l_of[c], f, l);
-          o[0] = fmaf(o_of[c].x, f, o[0]), o[1] = fmaf(o_of[c].y, f, o[1]);
-          o[2] = fmaf(o_of[c].z, f, o[2]), o[3] = fmaf(o_of[c].w, f, o[3]);
+          const float f = exp2_approx(m_of[c] - base), fo = part_factor(f, l_of[c], any);
+          l = fmaf(fabsf(l_of[c]), f, l);
+          o.x = fmaf(o_of[c].x, fo, o.x), o.y = fmaf(o_of[c].y, fo, o.y);
+          o.z = fmaf(o_of[c].z, fo, o.z), o.w = fmaf(o_of[c].w, fo, o.w);
         }
         const float r = l == 0.0f ? 0.0f : 1.0f / l;
         const size_t at = static_cast<size_t>(seq) * a.q_heads + h0 + h;
-        uint2 o2;
-        o2.x = pack_bf16x2(o[0] * r, o[1] * r), o2.y = pack_bf16x2(o[2] * r, o[3] * r);
-        *reinterpret_cast<uint2*>(a.out + at * D + d) = o2;
+        *reinterpret_cast<uint2*>(a.out + at * D + d) = attn_output(o, r, any);
         if (a.lse && d == 0) a.lse[at] = l == 0.0f ? -kInf : (top + log2f(l)) * 0.6931471805599453f;
       }
       cluster_sync_all();  // the others may still read this block's part
@@ -977,7 +988,13 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const __grid_co
   if (pieces == 1) return;
   auto part_of = [&](int c) { return a.parts + static_cast<size_t>(slot + c) * kHeads * (D + 2); };
   float top = -kInf;
-  for (int c = threadIdx.x & 31; c < pieces; c += 32) top = fmaxf(top, part_of(c)[kHeads * D + 2 * h]);
+  bool any = false;  // a part of small unit
+  for (int c = threadIdx.x & 31; c < pieces; c += 32) {
+    const float2 ml = *reinterpret_cast<const float2*>(part_of(c) + kHeads * D + 2 * h);
+    top = fmaxf(top, ml.x);
+    any |= ml.y < 0.0f;
+  }
+  any = __any_sync(0xffffffffu, any);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
   const float base = top == -kInf ? 0.0f : top;
@@ -988,9 +1005,9 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const __grid_co
     const float* part = part_of(c);
     const float2 ml = *reinterpret_cast<const float2*>(part + kHeads * D + 2 * h);
     const float4 x4 = *reinterpret_cast<const float4*>(part + h * D + d);
-    const float f = exp2_approx(ml.x - base);
-    l = fmaf(ml.y, f, l);
-    o.x = fmaf(x4.x, f, o.x), o.y = fmaf(x4.y, f, o.y), o.z = fmaf(x4.z, f, o.z), o.w = fmaf(x4.w, f, o.w);
+    const float f = exp2_approx(ml.x - base), fo = part_factor(f, ml.y, any);
+    l = fmaf(fabsf(ml.y), f, l);
+    o.x = fmaf(x4.x, fo, o.x), o.y = fmaf(x4.y, fo, o.y), o.z = fmaf(x4.z, fo, o.z), o.w = fmaf(x4.w, fo, o.w);
   }
   sums[team][threadIdx.x - team * kLanes] = o;
   if (d == 0) ls[team] = l;
@@ -1003,9 +1020,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const __grid_co
     l += ls[i];
   }
   const float r = l == 0.0f ? 0.0f : 1.0f / l;
-  uint2 o2;
-  o2.x = pack_bf16x2(o.x * r, o.y * r), o2.y = pack_bf16x2(o.z * r, o.w * r);
-  *reinterpret_cast<uint2*>(a.out + at * D + d) = o2;
+  *reinterpret_cast<uint2*>(a.out + at * D + d) = attn_output(o, r, any);
   if (a.lse && threadIdx.x == 0) a.lse[at] = l == 0.0f ? -kInf : (top + log2f(l)) * 0.6931471805599453f;
 }
 

@@ -123,6 +123,33 @@ def test_value_scales_of_all_sizes_together(mx, fmt, dim, heads, kv, longest, se
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,heads,kv", [(64, 12, 3), (128, 20, 1), (256, 4, 2)])
+@pytest.mark.parametrize("longest,seqs", [(60, 150), (700, 40), (20000, 3)])
+def test_sums_beside_values_of_any_size(mx, fmt, dim, heads, kv, longest, seqs):
+    """lse is as exact beside huge values as elsewhere, with scores near zero and in many short sums; a NaN scale
+    loses no bits of the smallest values beside it; huge values of single keys meet other parts' ordinary ones."""
+    rng = np.random.default_rng(longest + dim)
+    lengths = [longest] + [int(n) for n in rng.integers(1, longest + 1, seqs - 1)]
+    cache = random_cache(mx, rng, sum(-(-n // 64) for n in lengths) + 1, kv, dim, 64, fmt)
+    table = random_table(rng, cache, lengths)
+    scales = cache.v_scales.cpu().numpy()
+    for b, n in enumerate(lengths):
+        pages = table[b, : -(-n // 64)]
+        if b % 3 == 0:
+            for key in rng.integers(0, n, 3):
+                scales[pages[key // 64], :, key % 64, rng.integers(dim // 32)] = rng.integers(192, 245)
+        elif b % 3 == 1:
+            scales[pages] = rng.integers(0, 60, scales[pages].shape)
+            scales[pages[0], :, 0, 1] = 255
+        else:
+            scales[pages] = rng.integers(0, 245, scales[pages].shape)
+    cache.v_scales.copy_(torch.from_numpy(scales))
+    q = bf16(rng, (seqs, heads, dim), 0.01)
+    out, lse = mx.paged_attention(q, cache, i32(table), i32(lengths), scale=0.01, return_lse=True)
+    check(out, lse, q, cache, table, lengths, 0.01)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_groups_of_zeros_among_values(mx, fmt, dim):
     """The coder gives them scale byte 0, which is the smallest scale there is when the codes are not zeros."""
