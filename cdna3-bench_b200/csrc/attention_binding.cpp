@@ -268,6 +268,12 @@ ENTRY(paged_attention, 7)
     const at::Tensor* o = tensor(args[6]);
     if (!o || o->scalar_type() != at::kBFloat16 || o->device() != c.dev || o->sizes() != q->sizes() || !o->is_contiguous())
       refuse("out must be contiguous bfloat16 [seqs, num_heads, head_dim] on the cache's GPU");
+    const int64_t row = heads * dim, stride = seqs > 1 ? q->stride(0) : row, size = seqs * row;
+    const int64_t off = (static_cast<const char*>(o->data_ptr()) - static_cast<const char*>(q->data_ptr())) / 2;  // of out in q
+    if (size > 0 && off < (seqs - 1) * stride + row && -off < size && !(off == 0 && stride == row)) {
+      const int64_t in_row = off >= 0 && stride > row ? off % stride : 0;  // q's rows may leave room for all of out
+      if (in_row < row || in_row + size > stride) refuse("out overlaps q without being q itself");
+    }
     out = *o;
   }
   const bool want_lse = truth(args[5]);

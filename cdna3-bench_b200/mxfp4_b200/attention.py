@@ -160,7 +160,7 @@ def paged_attention(q, cache: MXKVCache, page_table, lengths, scale: float | Non
     page a sequence needs may hold anything.  A length of zero gives a row of zeros.  ``scale`` defaults to
     ``head_dim ** -0.5``.  Returns bf16 ``[seqs, num_heads, head_dim]`` (``out`` if given), with
     ``return_lse`` also fp32 ``[seqs, num_heads]``: the natural log of the sum of exp(scale * q . k), -inf
-    for an empty sequence.  ``out`` may be ``q`` itself, and must not overlap it otherwise.  The same call
+    for an empty sequence.  ``out`` may be ``q`` itself, and is refused if it overlaps it otherwise.  The same call
     gives the same bits.
     """
     if not isinstance(cache, MXKVCache):

@@ -312,3 +312,25 @@ def test_a_token_without_a_position_does_not_take_a_slot_from_another(mx, tokens
         for a, b in zip((cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales), (want.k_codes, want.v_codes, want.k_scales, want.v_scales)):
             assert torch.equal(a, b)
         assert mx.device_error() == 0
+
+
+# ---------------------------------------------------------------------------------------- refusals
+def test_out_over_a_part_of_q_is_refused(mx):
+    rng = np.random.default_rng(1)
+    cache = random_cache(mx, rng, 4, 1, 64, 16, "mxfp8")
+    table, lengths = i32([[0, 1], [2, 3], [1, 0]]), i32([20, 30, 7])
+    buf = bf16(rng, (8, 4, 64))
+    q = buf[2:5]
+    values = q.clone()
+    want = mx.paged_attention(values, cache, table, lengths)
+    wide = torch.zeros((3, 4 * 64 * 6), dtype=torch.bfloat16, device="cuda")
+    rows = wide[:, :256].unflatten(1, (4, 64))
+    rows.copy_(q)
+    flat = wide.view(-1)
+    for query, out in ((q, buf[1:4]), (q, buf[4:7]), (rows, flat[:768].view(3, 4, 64)), (rows, flat[1536 - 760:][:768].view(3, 4, 64)),
+                       (rows, flat[200:968].view(3, 4, 64)), (q, buf.view(-1)[2 * 256 + 8:][:768].view(3, 4, 64))):
+        with pytest.raises(RuntimeError, match="overlaps q"):
+            mx.paged_attention(query, cache, table, lengths, out=out)
+    for query, out in ((q, buf[5:8]), (buf[3:6], buf[:3]), (rows, flat[256:1024].view(3, 4, 64)), (rows, flat[1536 - 768:1536].view(3, 4, 64)), (q, q)):
+        query.copy_(values)
+        assert torch.equal(mx.paged_attention(query, cache, table, lengths, out=out), want)
